@@ -26,6 +26,7 @@ from __future__ import annotations
 import ctypes
 import importlib.util
 import os
+from typing import NamedTuple
 
 import torch  # noqa: F401  (loads libtorch / libc10 before the extension)
 
@@ -33,7 +34,8 @@ from ._build import EXT_NAME, EXT_PATH, LIB_PATH
 
 __all__ = [
     "mla_decode_naive", "mla_decode_fused", "mla_decode_split", "mla_decode_batched",
-    "mla_decode_paged", "mla_decode_mtp",
+    "mla_decode_paged", "mla_decode_mtp", "mla_decode_tree", "tree_mask", "mla_build_slots", "SlotPlan",
+    "mla_cache_write",
     "mla_combine", "mla_get_device_error", "NUM_HEADS", "HEAD_DIM", "HEAD_DIM_C",
     "HEAD_DIM_ROPE", "HEAD_DIM_K", "HEAD_DIM_V", "SOFTMAX_SCALE", "lib_path", "ext_path",
 ]
@@ -165,3 +167,104 @@ def mla_decode_mtp(query, cache, cu_seqlens=None, max_seq_len: int = -1,
     out, lse = _ext.mla_decode_mtp(query, cache, cu_seqlens, int(max_seq_len), float(softmax_scale),
                                    int(num_splits), bool(return_lse), out_dtype == torch.float32)
     return (out, lse) if return_lse else out
+
+
+def tree_mask(parents):
+    """Masks of draft trees for ``mla_decode_tree`` from each draft's parent.
+
+    parents  [k] or [B, k] ints (a tensor or nested lists): the index of draft i's
+             parent, an earlier draft, or -1 where it follows the cached context.
+    Returns an int64 CPU tensor of the same shape: bit j of entry i is set where j is
+    i itself or one of its ancestors.
+    """
+    par = torch.as_tensor(parents, dtype=torch.int64).cpu()
+    if par.dim() not in (1, 2) or not 1 <= par.shape[-1] <= 64:
+        raise ValueError("tree_mask: expected parents [k] or [B, k] with 1 <= k <= 64")
+    k = par.shape[-1]
+    if bool(((par < -1) | (par >= torch.arange(k))).any()):
+        raise ValueError("tree_mask: a draft's parent is an earlier draft, or -1")
+    flat = par.reshape(-1, k)
+    mask = torch.zeros_like(flat)
+    for i in range(k):
+        up = torch.gather(mask, 1, flat[:, i:i + 1].clamp(min=0))[:, 0]
+        bit = 1 << i if i < 63 else -(1 << 63)
+        mask[:, i] = torch.where(flat[:, i] >= 0, up, torch.zeros_like(up)) | bit
+    return mask.view(par.shape)
+
+
+def mla_decode_tree(query, kv_pages, block_table, seq_lens, tree_mask=None, max_seq_len: int = -1,
+                    softmax_scale: float = SOFTMAX_SCALE, num_splits: int = -1,
+                    return_lse: bool = False, out_dtype=None):
+    """Attention of a tree of drafted tokens over a paged latent cache.
+
+    query        [B, k, n_h, 576] fp16 or bf16, k <= 64, n_h <= 128: k drafts per
+                 sequence, whose own latent rows are the sequence's last k cache rows
+                 (``seq_lens`` counts them).
+    kv_pages, block_table, seq_lens
+                 as for ``mla_decode_paged``.
+    tree_mask    int64 [B, k], or [k] for one tree shared by all sequences: bit j of
+                 draft i's entry is set where i sees draft j (``ada_mla.tree_mask``
+                 makes it from parents).  None: a chain, draft i sees drafts 0..i.
+    Every draft sees the whole context before the drafts.  A draft's row that no draft
+    sees (a padded draft) may hold anything; a query that sees nothing gives zeros and
+    an LSE of -inf.  Returns O* [B, k, n_h, 512] (input dtype, or fp32 with
+    ``out_dtype=torch.float32``) and, with ``return_lse``, the natural-log LSE
+    [B, k, n_h] fp32.  Pass ``max_seq_len`` to avoid a device->host read.
+    """
+    if out_dtype not in (None, torch.float32, query.dtype):
+        raise ValueError(f"mla_decode_tree: out_dtype must be None, float32 or {query.dtype}")
+    out, lse = _ext.mla_decode_tree(query, kv_pages, block_table, seq_lens, tree_mask, int(max_seq_len),
+                                    float(softmax_scale), int(num_splits), bool(return_lse),
+                                    out_dtype == torch.float32)
+    return (out, lse) if return_lse else out
+
+
+class SlotPlan(NamedTuple):
+    """What ``mla_build_slots`` gives for a step's new tokens."""
+    slots: torch.Tensor      # int64 [num_tokens]: pool row of each new token, -1 = no page
+    positions: torch.Tensor  # int32 [num_tokens]: its position in its request
+    cu_new: torch.Tensor     # int32 [B + 1]: request b's tokens are cu_new[b]:cu_new[b + 1]
+    seq_lens: torch.Tensor   # int32 [B]: the requests' lengths after the step
+    free_head: torch.Tensor  # int32 [1]: first free page left (> len(free_pages): they ran out)
+
+
+def mla_build_slots(seq_lens, new_lens, block_table, free_pages, page_size: int, num_tokens: int,
+                    free_head=None) -> SlotPlan:
+    """Pages and slots for the tokens that a step appends to its requests, on the GPU.
+
+    seq_lens     int32 [B]: tokens each request holds.
+    new_lens     int32 [B]: tokens it appends.
+    block_table  int32 [B, max_blocks], written in place: request b's new pages follow
+                 the ceil(seq_lens[b] / page_size) it has.
+    free_pages   int32 [F]: pages to take, in order, from entry ``free_head`` on
+                 (int32 [1] on the device; None: 0).
+    num_tokens   sum of new_lens, or a bound on it (the host does not read it back).
+    Nothing but block_table is written in place, so a step can be planned again.  A
+    token without a page (the list or the table's row is used up) has slot -1, which
+    ``mla_cache_write`` skips.
+    """
+    return SlotPlan(*_ext.mla_build_slots(seq_lens, new_lens, block_table, free_pages, int(page_size),
+                                          int(num_tokens), free_head))
+
+
+def mla_cache_write(latent, slots, cache, norm_weight=None, eps: float = 1e-6, positions=None,
+                    cos_sin=None, interleaved: bool = True, kv_scales=None) -> None:
+    """Writes latent rows into the cache: RMS norm, rotary embedding, one rounding.
+
+    latent       [T, 576] fp16, bf16 or fp32 (rows may be strided: a slice of a wider
+                 projection): 512 latent columns, then 64 rope columns.
+    slots        int64 [T]: cache row of each (``mla_build_slots``); rows outside the
+                 cache are skipped.
+    cache        [rows, 576] or [num_pages, page_size, 576], fp16, bf16 or
+                 torch.float8_e4m3fn, written in place.
+    norm_weight  [512] in latent's dtype: RMS norm of the latent columns with ``eps``;
+                 None: they are stored as they are.
+    positions, cos_sin
+                 int32 [T] and fp32 [max_positions, 64] (cosines of the 32 angles, then
+                 their sines): rotates the rope columns, pairs (2i, 2i + 1), or
+                 (i, i + 32) with ``interleaved=False``; None: stored as they are.
+    kv_scales    fp32, one per cache row, written in place: with an e4m3 cache, row =
+                 cache * scale (what ``mla_decode_batched`` takes as ``kv_scale``).
+    """
+    _ext.mla_cache_write(latent, slots, cache, norm_weight, float(eps), positions, cos_sin,
+                         bool(interleaved), kv_scales)

@@ -295,6 +295,192 @@ std::vector<at::Tensor> mla_decode_paged(const at::Tensor &query, const at::Tens
     return {out, lse};
 }
 
+// Draft-tree decode over a paged cache (no reference counterpart).
+//   query [B, k, n_h, 576] fp16 or bf16 (k <= 64, n_h <= 128); kv_pages [num_pages,
+//   page_size, 576] in the same dtype; block_table int32 [B, max_blocks]; seq_lens
+//   int32 [B]; tree_mask int64 [B, k] or [k] (bit j of draft i's word: i sees draft
+//   j), or None for a chain.  max_seq_len < 0 reads max(seq_lens) from the device.
+// Returns (out [B, k, n_h, 512], lse [B, k, n_h] fp32 or empty).
+std::vector<at::Tensor> mla_decode_tree(const at::Tensor &query, const at::Tensor &kv_pages,
+                                        const at::Tensor &block_table, const at::Tensor &seq_lens,
+                                        const c10::optional<at::Tensor> &tree_mask, int64_t max_seq_len,
+                                        double softmax_scale, int64_t num_splits, bool return_lse,
+                                        bool out_fp32) {
+    check_cuda(query, "query");
+    check_cuda(kv_pages, "kv_pages");
+    check_cuda(block_table, "block_table");
+    check_cuda(seq_lens, "seq_lens");
+    const bool bf16 = query.scalar_type() == at::kBFloat16;
+    TORCH_CHECK((query.scalar_type() == at::kHalf || bf16) && kv_pages.scalar_type() == query.scalar_type(),
+                "mla_decode_tree: float16 or bfloat16 inputs (query and kv_pages alike) expected");
+    TORCH_CHECK(query.dim() == 4 && query.size(3) == MLA_B200_HEAD_DIM_K,
+                "mla_decode_tree: query must be [B, k, n_h, 576]");
+    TORCH_CHECK(kv_pages.dim() == 3 && kv_pages.size(2) == MLA_B200_HEAD_DIM_K,
+                "mla_decode_tree: kv_pages must be [num_pages, page_size, 576]");
+    const int64_t b = query.size(0), k = query.size(1), nh = query.size(2);
+    TORCH_CHECK(k >= 1 && k <= 64, "mla_decode_tree: 1 to 64 drafts expected");
+    TORCH_CHECK(nh >= 1 && nh <= 128, "mla_decode_tree: 1 to 128 heads expected");
+    TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == b,
+                "mla_decode_tree: block_table must be int32 [B, max_blocks]");
+    TORCH_CHECK(seq_lens.scalar_type() == at::kInt && seq_lens.dim() == 1 && seq_lens.size(0) == b,
+                "mla_decode_tree: seq_lens must be int32 [B]");
+    TORCH_CHECK(query.device() == kv_pages.device() && query.device() == block_table.device() &&
+                    query.device() == seq_lens.device(),
+                "mla_decode_tree: all tensors on one device");
+    const uint64_t *mask = nullptr;
+    int shared = 0;
+    if (tree_mask.has_value() && tree_mask->defined()) {
+        const at::Tensor &m = *tree_mask;
+        check_cuda(m, "tree_mask");
+        shared = m.dim() == 1;
+        TORCH_CHECK(m.scalar_type() == at::kLong && m.device() == query.device() &&
+                        ((shared && m.size(0) == k) || (m.dim() == 2 && m.size(0) == b && m.size(1) == k)),
+                    "mla_decode_tree: tree_mask must be int64 [B, k] or [k] on the query's device");
+        mask = reinterpret_cast<const uint64_t *>(m.data_ptr<int64_t>());
+    }
+    c10::cuda::CUDAGuard g(query.device());
+    if (max_seq_len < 0) max_seq_len = b > 0 ? std::max<int64_t>(seq_lens.max().item<int64_t>(), 0) : 0;
+    TORCH_CHECK(max_seq_len <= INT32_MAX, "mla_decode_tree: max_seq_len out of range");
+    at::Tensor out = at::empty({b, k, nh, MLA_B200_HEAD_DIM_V},
+                               query.options().dtype(out_fp32 ? at::kFloat : query.scalar_type()));
+    at::Tensor lse = at::empty({return_lse ? b : 0, k, nh}, query.options().dtype(at::kFloat));
+    at::Tensor w = workspace(query, mla_b200_workspace_size_tree((int)b, (int)k, (int)nh, (int)max_seq_len,
+                                                                 (int)num_splits));
+    auto *fn = bf16 ? mla_b200_decode_tree_bf16 : mla_b200_decode_tree_f16;
+    const int odt = out_fp32 ? MLA_B200_OUT_F32 : (bf16 ? MLA_B200_OUT_BF16 : MLA_B200_OUT_F16);
+    check_status(fn(query.data_ptr(), kv_pages.data_ptr(), block_table.data_ptr<int32_t>(),
+                    seq_lens.data_ptr<int32_t>(), mask, shared, (int)b, (int)k, (int)nh, (int)kv_pages.size(0),
+                    (int)kv_pages.size(1), (int)block_table.size(1), (int)max_seq_len, (float)softmax_scale,
+                    (int)num_splits, out.data_ptr(), odt, return_lse ? lse.data_ptr<float>() : nullptr,
+                    w.data_ptr(), w.numel(), stream_ptr()),
+                 "mla_decode_tree");
+    return {out, lse};
+}
+
+// Pages and slots for a step's new tokens (no reference counterpart); block_table is
+// written in place.  Returns (slots int64 [num_tokens], positions int32
+// [num_tokens], cu_new int32 [B + 1], new seq_lens int32 [B], new free_head int32 [1]).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> mla_build_slots(
+    const at::Tensor &seq_lens, const at::Tensor &new_lens, at::Tensor block_table, const at::Tensor &free_pages,
+    int64_t page_size, int64_t num_tokens, const c10::optional<at::Tensor> &free_head) {
+    check_cuda(seq_lens, "seq_lens");
+    check_cuda(new_lens, "new_lens");
+    check_cuda(free_pages, "free_pages");
+    TORCH_CHECK(block_table.is_cuda(), "block_table must be a CUDA tensor");
+    const int64_t b = seq_lens.size(0);
+    TORCH_CHECK(seq_lens.dim() == 1 && new_lens.dim() == 1 && new_lens.size(0) == b &&
+                    seq_lens.scalar_type() == at::kInt && new_lens.scalar_type() == at::kInt,
+                "mla_build_slots: seq_lens and new_lens must be int32 [B]");
+    TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == b &&
+                    (block_table.size(1) <= 1 || block_table.stride(1) == 1) &&
+                    (b <= 1 || block_table.stride(0) >= block_table.size(1)),
+                "mla_build_slots: block_table must be int32 [B, max_blocks] with dense rows");
+    TORCH_CHECK(free_pages.scalar_type() == at::kInt && free_pages.dim() == 1,
+                "mla_build_slots: free_pages must be int32 [F]");
+    TORCH_CHECK(page_size >= 1 && page_size <= INT32_MAX && num_tokens >= 0 && num_tokens <= INT32_MAX &&
+                    free_pages.size(0) <= INT32_MAX && block_table.size(1) <= INT32_MAX && b <= INT32_MAX,
+                "mla_build_slots: page_size or num_tokens out of range");
+    TORCH_CHECK(seq_lens.device() == new_lens.device() && seq_lens.device() == block_table.device() &&
+                    seq_lens.device() == free_pages.device(),
+                "mla_build_slots: all tensors on one device");
+    const int32_t *head = nullptr;
+    if (free_head.has_value() && free_head->defined()) {
+        check_cuda(*free_head, "free_head");
+        TORCH_CHECK(free_head->scalar_type() == at::kInt && free_head->numel() == 1 &&
+                        free_head->device() == seq_lens.device(),
+                    "mla_build_slots: free_head must be one int32 on the same device");
+        head = free_head->data_ptr<int32_t>();
+    }
+    c10::cuda::CUDAGuard g(seq_lens.device());
+    const auto opt = seq_lens.options();
+    at::Tensor slots = at::empty({num_tokens}, opt.dtype(at::kLong)), positions = at::empty({num_tokens}, opt);
+    at::Tensor cu_new = at::empty({b + 1}, opt), lens = at::empty({b}, opt), new_head = at::empty({1}, opt);
+    check_status(mla_b200_build_slots(seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
+                                      block_table.data_ptr<int32_t>(),
+                                      b > 1 ? block_table.stride(0) : block_table.size(1), (int)block_table.size(1),
+                                      free_pages.data_ptr<int32_t>(), (int)free_pages.size(0), head, (int)b,
+                                      (int)page_size, (int)num_tokens, slots.data_ptr<int64_t>(),
+                                      positions.data_ptr<int32_t>(), cu_new.data_ptr<int32_t>(),
+                                      lens.data_ptr<int32_t>(), new_head.data_ptr<int32_t>(), stream_ptr()),
+                 "mla_build_slots");
+    return {slots, positions, cu_new, lens, new_head};
+}
+
+// Latent rows into the cache (no reference counterpart); cache (and kv_scales) are
+// written in place.
+void mla_cache_write(const at::Tensor &latent, const at::Tensor &slots, at::Tensor cache,
+                     const c10::optional<at::Tensor> &norm_weight, double eps,
+                     const c10::optional<at::Tensor> &positions, const c10::optional<at::Tensor> &cos_sin,
+                     bool interleaved, const c10::optional<at::Tensor> &kv_scales) {
+    TORCH_CHECK(latent.is_cuda(), "latent must be a CUDA tensor");
+    check_cuda(slots, "slots");
+    check_cuda(cache, "cache");
+    auto dtype_of = [](at::ScalarType t) {
+        return t == at::kHalf ? (int)MLA_B200_DTYPE_F16
+               : t == at::kBFloat16 ? (int)MLA_B200_DTYPE_BF16
+               : t == at::kFloat ? (int)MLA_B200_DTYPE_F32
+               : t == at::kFloat8_e4m3fn ? (int)MLA_B200_DTYPE_E4M3 : -1;
+    };
+    const int in = dtype_of(latent.scalar_type()), to = dtype_of(cache.scalar_type());
+    TORCH_CHECK(in >= 0 && in != MLA_B200_DTYPE_E4M3,
+                "mla_cache_write: float16, bfloat16 or float32 latent rows expected");
+    TORCH_CHECK(to >= 0 && to != MLA_B200_DTYPE_F32,
+                "mla_cache_write: a float16, bfloat16 or float8_e4m3fn cache expected");
+    const int64_t t = latent.dim() == 2 ? latent.size(0) : -1;
+    TORCH_CHECK(t >= 0 && t <= INT32_MAX && latent.size(1) == MLA_B200_HEAD_DIM_K && latent.stride(1) == 1,
+                "mla_cache_write: latent must be [T, 576] with dense rows");
+    TORCH_CHECK(slots.scalar_type() == at::kLong && slots.dim() == 1 && slots.size(0) == t,
+                "mla_cache_write: slots must be int64 [T]");
+    TORCH_CHECK((cache.dim() == 2 || cache.dim() == 3) && cache.size(-1) == MLA_B200_HEAD_DIM_K,
+                "mla_cache_write: cache must be [rows, 576] or [num_pages, page_size, 576]");
+    TORCH_CHECK(latent.device() == slots.device() && latent.device() == cache.device(),
+                "mla_cache_write: all tensors on one device");
+    const int64_t rows = cache.numel() / MLA_B200_HEAD_DIM_K;
+    const void *w = nullptr;
+    if (norm_weight.has_value() && norm_weight->defined()) {
+        check_cuda(*norm_weight, "norm_weight");
+        TORCH_CHECK(norm_weight->scalar_type() == latent.scalar_type() && norm_weight->device() == latent.device() &&
+                        norm_weight->dim() == 1 && norm_weight->size(0) == MLA_B200_HEAD_DIM_V,
+                    "mla_cache_write: norm_weight must be [512] in the latent rows' dtype");
+        w = norm_weight->data_ptr();
+    }
+    const int32_t *pos = nullptr;
+    const float *cs = nullptr;
+    int max_pos = 0;
+    const bool has_pos = positions.has_value() && positions->defined();
+    TORCH_CHECK(has_pos == (cos_sin.has_value() && cos_sin->defined()),
+                "mla_cache_write: positions and cos_sin come together");
+    if (has_pos) {
+        check_cuda(*positions, "positions");
+        check_cuda(*cos_sin, "cos_sin");
+        TORCH_CHECK(positions->scalar_type() == at::kInt && positions->dim() == 1 && positions->size(0) == t &&
+                        positions->device() == latent.device(),
+                    "mla_cache_write: positions must be int32 [T]");
+        TORCH_CHECK(cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2 && cos_sin->size(0) <= INT32_MAX &&
+                        cos_sin->size(1) == MLA_B200_HEAD_DIM_ROPE && cos_sin->device() == latent.device(),
+                    "mla_cache_write: cos_sin must be float32 [max_positions, 64]");
+        pos = positions->data_ptr<int32_t>();
+        cs = cos_sin->data_ptr<float>();
+        max_pos = (int)cos_sin->size(0);
+    }
+    float *scales = nullptr;
+    const bool has_scales = kv_scales.has_value() && kv_scales->defined();
+    TORCH_CHECK(has_scales == (to == MLA_B200_DTYPE_E4M3),
+                "mla_cache_write: kv_scales goes with a float8_e4m3fn cache, and only with one");
+    if (has_scales) {
+        check_cuda(*kv_scales, "kv_scales");
+        TORCH_CHECK(kv_scales->scalar_type() == at::kFloat && kv_scales->numel() == rows &&
+                        kv_scales->device() == latent.device(),
+                    "mla_cache_write: kv_scales must be float32, one per cache row");
+        scales = kv_scales->data_ptr<float>();
+    }
+    c10::cuda::CUDAGuard g(latent.device());
+    check_status(mla_b200_cache_write(latent.data_ptr(), in, t > 1 ? latent.stride(0) : MLA_B200_HEAD_DIM_K,
+                                      slots.data_ptr<int64_t>(), (int)t, w, (float)eps, pos, cs, max_pos,
+                                      interleaved ? 1 : 0, cache.data_ptr(), to, rows, scales, stream_ptr()),
+                 "mla_cache_write");
+}
+
 // LSE merge of partials: part_o [P, rows, 512] fp32, part_lse [P, rows] fp32.
 std::vector<at::Tensor> mla_combine(const at::Tensor &part_o, const at::Tensor &part_lse,
                                     bool out_fp32) {
@@ -346,6 +532,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("query"), py::arg("kv_pages"), py::arg("block_table"), py::arg("seq_lens"),
           py::arg("max_seq_len") = -1, py::arg("softmax_scale") = 0.07216878364870322,
           py::arg("num_splits") = -1, py::arg("return_lse") = false, py::arg("out_fp32") = false);
+    m.def("mla_decode_tree", &mla_decode_tree, "draft-tree decode over a paged latent cache",
+          py::arg("query"), py::arg("kv_pages"), py::arg("block_table"), py::arg("seq_lens"),
+          py::arg("tree_mask") = py::none(), py::arg("max_seq_len") = -1,
+          py::arg("softmax_scale") = 0.07216878364870322, py::arg("num_splits") = -1,
+          py::arg("return_lse") = false, py::arg("out_fp32") = false);
+    m.def("mla_build_slots", &mla_build_slots, "pages and slots for a step's new tokens", py::arg("seq_lens"),
+          py::arg("new_lens"), py::arg("block_table"), py::arg("free_pages"), py::arg("page_size"),
+          py::arg("num_tokens"), py::arg("free_head") = py::none());
+    m.def("mla_cache_write", &mla_cache_write, "latent rows into the cache", py::arg("latent"), py::arg("slots"),
+          py::arg("cache"), py::arg("norm_weight") = py::none(), py::arg("eps") = 1e-6,
+          py::arg("positions") = py::none(), py::arg("cos_sin") = py::none(), py::arg("interleaved") = true,
+          py::arg("kv_scales") = py::none());
     m.def("mla_combine", &mla_combine, "log-sum-exp merge of partial decodes", py::arg("part_o"),
           py::arg("part_lse"), py::arg("out_fp32") = false);
     m.def("mla_get_device_error", &mla_get_device_error,

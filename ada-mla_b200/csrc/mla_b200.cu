@@ -21,7 +21,10 @@
 #include "mla_exchange.cuh"
 #include "mla_proj.cuh"
 #include "mla_simt.cuh"
+#include "mla_slots.cuh"
 #include "mla_tc.cuh"
+#include "mla_tree.cuh"
+#include "mla_write.cuh"
 
 using namespace mla;
 
@@ -50,11 +53,11 @@ int cuda_failure(cudaError_t e) {
 
 // Opts a tensor-core kernel instantiation (both schedules) into its dynamic
 // shared memory.
-template <bool kBf16, bool kPaged, bool kFp8 = false, bool kMtp = false, bool kRows = false>
+template <bool kBf16, bool kPaged, bool kFp8 = false, bool kMtp = false, bool kRows = false, bool kTree = false>
 bool set_tc_smem() {
-    return cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedChunked, kBf16, kPaged, kFp8, kMtp, kRows>,
+    return cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedChunked, kBf16, kPaged, kFp8, kMtp, kRows, kTree>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSmemBytes) == cudaSuccess &&
-           cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedBalanced, kBf16, kPaged, kFp8, kMtp, kRows>,
+           cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedBalanced, kBf16, kPaged, kFp8, kMtp, kRows, kTree>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSmemBytes) == cudaSuccess;
 }
 
@@ -100,7 +103,9 @@ int current_device(int *dev_out, DevInfo *info_out) {
             !set_tc_smem<false, true>() || !set_tc_smem<true, true>() ||
             !set_tc_smem<false, false, true>() || !set_tc_smem<false, false, true, false, true>() ||
             !set_tc_smem<false, false, false, true>() ||
-            !set_tc_smem<true, false, false, true>()) {
+            !set_tc_smem<true, false, false, true>() ||
+            !set_tc_smem<false, true, false, false, false, true>() ||
+            !set_tc_smem<true, true, false, false, false, true>()) {
             return cuda_failure(cudaGetLastError());
         }
         cudaLaunchConfig_t cfg = {};
@@ -257,12 +262,14 @@ struct WsLayout {
     int *item_off = nullptr;
     int4 *items = nullptr;
     int32_t *cu_virtual = nullptr;  // paged cache: sequence offsets built from seq_lens
+    unsigned long long *tree_seen = nullptr;  // draft tree: the drafts each row tile sees [batch]
     uint8_t *q8 = nullptr;          // fp8 cache: Q* as e4m3 hi and lo planes [2, B * n_h, 576]
     float *q_scale = nullptr;       // fp8 cache: [B * n_h]
     size_t bytes = 0;
 };
 
-WsLayout ws_layout(void *base, long long max_items, int num_heads, int batch, bool fp8 = false) {
+WsLayout ws_layout(void *base, long long max_items, int num_heads, int batch, bool fp8 = false,
+                   bool tree = false) {
     WsLayout L;
     size_t off = 0;
     const size_t o_bytes = (size_t)max_items * num_heads * kDV * sizeof(float);
@@ -280,6 +287,10 @@ WsLayout ws_layout(void *base, long long max_items, int num_heads, int batch, bo
     off = align_up(off + it_bytes, 256);
     L.cu_virtual = reinterpret_cast<int32_t *>(p + off);
     off = align_up(off + off_bytes, 256);
+    if (tree) {
+        L.tree_seen = reinterpret_cast<unsigned long long *>(p + off);
+        off = align_up(off + (size_t)batch * sizeof(unsigned long long), 256);
+    }
     if (fp8) {
         const size_t rows = (size_t)batch * num_heads;
         L.q8 = reinterpret_cast<uint8_t *>(p + off);
@@ -357,6 +368,15 @@ struct PagedArgs {
     long long pool_rows;
 };
 
+// A tree of `drafts` draft tokens per sequence over a paged cache: `tiles` row tiles
+// of up to `tile_drafts` drafts of `heads` rows each per sequence, each tile a
+// sequence of the work list (tc::TcTreeParams).
+struct TreeArgs {
+    const unsigned long long *mask;  // null: a chain
+    int mask_stride;
+    int drafts, heads, tiles, tile_drafts;
+};
+
 // Launch, with programmatic stream serialization when `dependent`: the kernel
 // may then start while its predecessor in the stream runs (the predecessor
 // allows it with griddep_launch) and waits for it (griddep_wait) before
@@ -389,6 +409,27 @@ void launch_tc(int clusters, const TcMaps &m, const tc::TcParams &tp, cudaStream
                      dim3(tc::kThreads), tc::kSmemBytes, stream, after_plan, m.cmap_s, m.cmap_o, m.qmap, tp);
 }
 
+template <int kSched, bool kBf16>
+void launch_tc_tree(int clusters, const TcMaps &m, const tc::TcTreeParams &tp, cudaStream_t stream) {
+    launch_dependent(tc::tc_decode_kernel<kSched, kBf16, true, false, false, false, true>, dim3(2 * clusters),
+                     dim3(tc::kThreads), tc::kSmemBytes, stream, true, m.cmap_s, m.cmap_o, m.qmap, tp);
+}
+
+template <typename OutT>
+void launch_tree_merge(const WsLayout &L, const WorkList &wl, const tc::TcTreeParams &tp, void *out, float *out_lse,
+                       cudaStream_t stream, bool chain) {
+    // a few tiles have many splits each: a block of 8 warps per row; many tiles have
+    // one or two: a warp per row
+    const dim3 block(32 * tree::kMergeWarps);
+    if (wl.batch < 8)
+        launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3((unsigned)tp.num_heads, (unsigned)wl.batch),
+                         block, 0, stream, chain, L.part_o, L.part_lse, wl, tp, static_cast<OutT *>(out), out_lse);
+    else
+        launch_dependent(tree::merge_kernel<OutT, 1>,
+                         dim3((unsigned)cdiv(tp.num_heads, tree::kMergeWarps), (unsigned)wl.batch), block, 0, stream,
+                         chain, L.part_o, L.part_lse, wl, tp, static_cast<OutT *>(out), out_lse);
+}
+
 // Shared driver of the split-KV paths: plan -> partial kernel -> combine.
 // pg (tensor-core path only): the cache is a page pool; cu_seqlens is ignored
 // and the sequences' offsets on a virtual packed axis are built from
@@ -399,7 +440,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
                      int num_splits, void *out, int out_dtype, float *out_lse, void *workspace,
                      size_t workspace_bytes, cudaStream_t stream, const PagedArgs *pg = nullptr,
                      const Fp8Args *f8 = nullptr, const MtpArgs *mtp = nullptr, int group = 1,
-                     const XchgArgs *xa = nullptr) {
+                     const XchgArgs *xa = nullptr, const TreeArgs *tr = nullptr) {
     int dev;
     DevInfo info;
     int st = current_device(&dev, &info);
@@ -445,7 +486,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
     const long long max_items = balanced ? (long long)batch + info.tc_clusters
                                          : max_items_for(batch, plan_total, chunk);
     if (max_items > (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
-    WsLayout L = ws_layout(workspace, max_items, num_heads, batch, f8 != nullptr);
+    WsLayout L = ws_layout(workspace, max_items, num_heads, batch, f8 != nullptr, tr != nullptr);
     if (workspace == nullptr || workspace_bytes < L.bytes) return MLA_B200_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
     const int32_t *seq_lens = nullptr;
@@ -488,7 +529,8 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             wl.nworkers = info.tc_clusters;
             bal_clusters = info.tc_clusters;
             plan_balanced_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, wl.item_cost, L.item_off, seq_lens,
-                                                         max_seq_len, L.cu_virtual, group, max_seq_len);
+                                                         max_seq_len, L.cu_virtual, group, max_seq_len,
+                                                         tr != nullptr ? tr->tiles : 1);
         }
     } else if (!planned) {
         wl.items = nullptr;
@@ -505,7 +547,20 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
         wl.cu_seqlens = cu_seqlens;  // read by the paged kernel
         plan_varlen_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, chunk, L.item_off, L.items,
                                                    (int)max_items, seq_lens, max_seq_len, L.cu_virtual,
-                                                   group, max_seq_len);
+                                                   group, max_seq_len, tr != nullptr ? tr->tiles : 1);
+    }
+    tc::TcTreeParams tree_p{};
+    if (tr != nullptr) {
+        tree_p.num_heads = num_heads;
+        tree_p.mask = tr->mask;
+        tree_p.seen = L.tree_seen;
+        tree_p.mask_stride = tr->mask_stride;
+        tree_p.drafts = tr->drafts;
+        tree_p.heads = tr->heads;
+        tree_p.tiles = tr->tiles;
+        tree_p.tile_drafts = tr->tile_drafts;
+        tree::seen_kernel<<<(unsigned)cdiv(batch, 256), 256, 0, stream>>>(
+            tr->mask, tr->mask_stride, tr->drafts, tr->tiles, tr->tile_drafts, batch, L.tree_seen);
     }
     bool tc_direct = false;  // the tcgen05 kernel wrote single-item sequences itself
     // A few long sequences chain decode -> merge -> next decode with programmatic
@@ -522,7 +577,8 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             // S-CTA: one box per ring slot (3 K-blocks x 96 rows); paged, one per
             // 32-row piece and slot.  O-CTA: one box per 32-row C tile (8 K-blocks).
             const long long map_rows = pg != nullptr ? pg->pool_rows : total_tokens;
-            const long long qrows = (long long)batch * num_heads;
+            const long long qrows = tr != nullptr ? (long long)(batch / tr->tiles) * tr->drafts * tr->heads
+                                                  : (long long)batch * num_heads;
             if (f8 != nullptr) {
                 st = make_tmap_fp8_s(&cmap_s, f8->cache8, map_rows);
                 if (st == MLA_B200_OK) st = make_tmap_fp8_o(&cmap_o, f8->cache8, map_rows);
@@ -582,7 +638,12 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             tc_direct = true;
             const int clusters = balanced ? bal_clusters : std::min(info.tc_clusters, wl.max_items);
             timing_mark(t_ev_start, stream);
-            if (mtp != nullptr) {
+            if (tr != nullptr) {
+                static_cast<tc::TcParams &>(tree_p) = tp;
+                tree_p.part_kind = tc::kOutF32;  // tree::merge_kernel
+                if (balanced) launch_tc_tree<kSchedBalanced, kBf16>(clusters, maps, tree_p, stream);
+                else launch_tc_tree<kSchedChunked, kBf16>(clusters, maps, tree_p, stream);
+            } else if (mtp != nullptr) {
                 if (balanced) launch_tc<kSchedBalanced, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
                 else launch_tc<kSchedChunked, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
             } else if (f8 != nullptr) {
@@ -612,6 +673,13 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
                 q, cache, wl, num_heads, scale * kLog2e, L.part_o, L.part_lse);
             timing_mark(t_ev_stop, stream);
         }
+    }
+    if (tr != nullptr) {
+        tree_p.num_heads = num_heads;
+        if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(L, wl, tree_p, out, out_lse, stream, chain);
+        else if constexpr (kBf16) launch_tree_merge<__nv_bfloat16>(L, wl, tree_p, out, out_lse, stream, chain);
+        else if constexpr (!std::is_same<T, float>::value) launch_tree_merge<__half>(L, wl, tree_p, out, out_lse, stream, chain);
+        return launch_status();
     }
     const long long rows = (long long)batch * num_heads;
     if (xa != nullptr) {
@@ -771,6 +839,59 @@ int decode_mtp(const void *query, const void *cache, const int32_t *cu_seqlens, 
 }  // namespace
 
 namespace {
+// Row tiles of the draft tree: as many whole drafts as 128 rows hold, the drafts
+// dealt evenly over the tiles.
+struct TreeTiles {
+    int tiles, tile_drafts;
+};
+
+TreeTiles tree_tiles(int drafts, int heads) {
+    const int fit = std::max(1, 128 / heads);
+    const int tiles = (int)cdiv(drafts, fit);
+    return {tiles, (int)cdiv(drafts, tiles)};
+}
+
+template <typename T>
+int decode_tree(const void *query, const void *kv_pages, const int32_t *block_table, const int32_t *seq_lens,
+                const uint64_t *mask, int shared_mask, int batch, int drafts, int heads, int num_pages, int page_size,
+                int max_blocks, int max_seq_len, float softmax_scale, int num_splits, void *out, int out_dtype,
+                float *out_lse, void *workspace, size_t workspace_bytes, void *stream) {
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    if (batch < 0 || drafts <= 0 || heads <= 0 || num_pages < 0 || page_size <= 0 || max_blocks < 0 || max_seq_len < 0)
+        return MLA_B200_ERR_INVALID_ARG;
+    if (batch > 0 && (query == nullptr || out == nullptr || block_table == nullptr || seq_lens == nullptr))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (num_pages > 0 && kv_pages == nullptr) return MLA_B200_ERR_INVALID_ARG;
+    if (kBf16 ? (out_dtype != MLA_B200_OUT_BF16 && out_dtype != MLA_B200_OUT_F32)
+              : (out_dtype != MLA_B200_OUT_F16 && out_dtype != MLA_B200_OUT_F32))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return MLA_B200_ERR_INVALID_ARG;
+    if (!aligned(query, 16) || !aligned(kv_pages, 16) || !aligned(out, 16) || !aligned(out_lse, 4) ||
+        !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(mask, 8))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (drafts > 64 || heads > 128 || page_size % tc::kTO != 0) return MLA_B200_ERR_UNSUPPORTED;
+    if ((long long)max_seq_len > (long long)max_blocks * page_size) return MLA_B200_ERR_INVALID_ARG;
+    const TreeTiles tt = tree_tiles(drafts, heads);
+    const long long pool_rows = (long long)num_pages * page_size;
+    const long long tiles = (long long)batch * tt.tiles;
+    if (pool_rows >= (1LL << 31) || tiles * std::max(max_seq_len, 1) >= (1LL << 31) || tiles > 65535 ||
+        (long long)batch * drafts * heads >= (1LL << 31))
+        return MLA_B200_ERR_UNSUPPORTED;
+    if (batch == 0) return MLA_B200_OK;
+    TreeArgs tr{reinterpret_cast<const unsigned long long *>(mask), shared_mask ? 0 : drafts, drafts, heads, tt.tiles,
+                tt.tile_drafts};
+    PagedArgs pg{block_table, seq_lens, max_blocks, page_size, pool_rows};
+    // (no pages or no tokens: every row's O is 0 and its LSE -inf, through the merge of no partials)
+    const bool empty = num_pages == 0 || max_seq_len == 0;
+    return run_split_decode<T>(static_cast<const T *>(query), static_cast<const T *>(kv_pages), nullptr, (int)tiles,
+                               tt.tile_drafts * heads, empty ? 0 : tiles * max_seq_len, empty ? 0 : max_seq_len,
+                               softmax_scale, num_splits, out, out_dtype, out_lse, workspace, workspace_bytes,
+                               static_cast<cudaStream_t>(stream), empty ? nullptr : &pg, nullptr, nullptr, 1, nullptr,
+                               &tr);
+}
+}  // namespace
+
+namespace {
 // Bounded-wait self test: one thread waits on an mbarrier that nothing will
 // complete, with the given limit, through the same wait loop the decode kernels
 // use; the wait records kErrSelfTest in the device error word and returns,
@@ -852,6 +973,24 @@ int run_proj(const void *x, const void *w, const void *rope, void *out, int batc
     launch_dependent(proj::proj_kernel, dim3(grid), dim3(proj::kThreads), smem, stream, false, wmap, xmap, p);
     timing_mark(t_ev_stop, stream);
     return launch_status();
+}
+}  // namespace
+
+namespace {
+template <typename InT, typename OutT>
+void launch_write(const write::WriteParams &p, bool vec, cudaStream_t stream) {
+    const unsigned grid = (unsigned)cdiv(p.num_tokens, write::kWarps);
+    if (vec) write::cache_write_kernel<InT, OutT, true><<<grid, 32 * write::kWarps, 0, stream>>>(p);
+    else write::cache_write_kernel<InT, OutT, false><<<grid, 32 * write::kWarps, 0, stream>>>(p);
+}
+
+template <typename InT>
+void launch_write_to(const write::WriteParams &p, int cache_dtype, cudaStream_t stream) {
+    // 16-byte loads where every row and the weights start on 16 bytes
+    const bool vec = aligned(p.latent, 16) && aligned(p.weight, 16) && p.stride * (long long)sizeof(InT) % 16 == 0;
+    if (cache_dtype == MLA_B200_DTYPE_F16) launch_write<InT, __half>(p, vec, stream);
+    else if (cache_dtype == MLA_B200_DTYPE_BF16) launch_write<InT, __nv_bfloat16>(p, vec, stream);
+    else launch_write<InT, __nv_fp8_storage_t>(p, vec, stream);
 }
 }  // namespace
 
@@ -953,7 +1092,7 @@ int mla_b200_plan(int batch, int num_heads, long long total_tokens, int max_seq_
 
 namespace {
 size_t workspace_bytes_for(int batch, int num_heads, long long total_tokens, int max_seq_len,
-                           int num_splits, bool fp8) {
+                           int num_splits, bool fp8, bool tree = false) {
     if (batch < 0 || num_heads <= 0 || total_tokens < 0) return 0;
     int num_sms = 0, dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -966,7 +1105,7 @@ size_t workspace_bytes_for(int batch, int num_heads, long long total_tokens, int
     long long max_items = max_items_for(batch, total_tokens, chunk);
     // an automatic split may run the balanced schedule: batch + one item per cluster
     if (num_splits <= 0) max_items = std::max(max_items, (long long)batch + std::max(1, num_sms / 2));
-    return ws_layout(nullptr, max_items, num_heads, batch, fp8).bytes;
+    return ws_layout(nullptr, max_items, num_heads, batch, fp8, tree).bytes;
 }
 }  // namespace
 
@@ -988,6 +1127,125 @@ size_t mla_b200_workspace_size_mtp(int batch, int num_tokens, int num_heads, lon
     if (max_seq_len <= 0 && batch > 0) max_seq_len = (int)cdiv(total_tokens, batch);
     return workspace_bytes_for(batch * num_tokens, num_heads, total_tokens * num_tokens, max_seq_len,
                                num_splits, false);
+}
+
+size_t mla_b200_workspace_size_tree(int batch, int num_drafts, int num_heads, int max_seq_len, int num_splits) {
+    if (batch < 0 || num_drafts <= 0 || num_heads <= 0 || max_seq_len < 0) return 0;
+    const TreeTiles tt = tree_tiles(num_drafts, num_heads);
+    const long long tiles = (long long)batch * tt.tiles;
+    if (tiles > 65535) return 0;
+    // (paged items start on 96-token boundaries, so they are at least as long as planned here)
+    return workspace_bytes_for((int)tiles, tt.tile_drafts * num_heads, tiles * max_seq_len, max_seq_len, num_splits,
+                               false, true);
+}
+
+int mla_b200_decode_tree_f16(const void *query, const void *kv_pages, const int32_t *block_table,
+                             const int32_t *seq_lens, const uint64_t *tree_mask, int shared_mask, int batch,
+                             int num_drafts, int num_heads, int num_pages, int page_size, int max_blocks_per_seq,
+                             int max_seq_len, float softmax_scale, int num_splits, void *out, int out_dtype,
+                             float *out_lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return decode_tree<__half>(query, kv_pages, block_table, seq_lens, tree_mask, shared_mask, batch, num_drafts,
+                               num_heads, num_pages, page_size, max_blocks_per_seq, max_seq_len, softmax_scale,
+                               num_splits, out, out_dtype, out_lse, workspace, workspace_bytes, stream);
+}
+
+int mla_b200_decode_tree_bf16(const void *query, const void *kv_pages, const int32_t *block_table,
+                              const int32_t *seq_lens, const uint64_t *tree_mask, int shared_mask, int batch,
+                              int num_drafts, int num_heads, int num_pages, int page_size, int max_blocks_per_seq,
+                              int max_seq_len, float softmax_scale, int num_splits, void *out, int out_dtype,
+                              float *out_lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return decode_tree<__nv_bfloat16>(query, kv_pages, block_table, seq_lens, tree_mask, shared_mask, batch,
+                                      num_drafts, num_heads, num_pages, page_size, max_blocks_per_seq, max_seq_len,
+                                      softmax_scale, num_splits, out, out_dtype, out_lse, workspace, workspace_bytes,
+                                      stream);
+}
+
+int mla_b200_build_slots(const int32_t *seq_lens, const int32_t *new_lens, int32_t *block_table,
+                         long long block_table_stride, int max_blocks_per_seq, const int32_t *free_pages,
+                         int num_free, const int32_t *free_head, int batch, int page_size, int num_tokens,
+                         int64_t *slots, int32_t *positions, int32_t *cu_new, int32_t *new_seq_lens,
+                         int32_t *new_free_head, void *stream) {
+    if (batch < 0 || max_blocks_per_seq < 0 || num_free < 0 || page_size <= 0 || num_tokens < 0 ||
+        block_table_stride < max_blocks_per_seq)
+        return MLA_B200_ERR_INVALID_ARG;
+    if (cu_new == nullptr || new_free_head == nullptr || (num_tokens > 0 && (slots == nullptr || positions == nullptr)))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (batch > 0 && (seq_lens == nullptr || new_lens == nullptr || new_seq_lens == nullptr ||
+                      (block_table == nullptr && max_blocks_per_seq > 0)))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (num_free > 0 && free_pages == nullptr) return MLA_B200_ERR_INVALID_ARG;
+    if (!aligned(seq_lens, 4) || !aligned(new_lens, 4) || !aligned(block_table, 4) || !aligned(free_pages, 4) ||
+        !aligned(free_head, 4) || !aligned(slots, 8) || !aligned(positions, 4) || !aligned(cu_new, 4) ||
+        !aligned(new_seq_lens, 4) || !aligned(new_free_head, 4))
+        return MLA_B200_ERR_INVALID_ARG;
+    int dev;
+    DevInfo info;
+    const int st = current_device(&dev, &info);
+    if (st != MLA_B200_OK) return st;
+    slots::SlotParams p;
+    p.seq_lens = seq_lens;
+    p.new_lens = new_lens;
+    p.table = block_table;
+    p.free_pages = free_pages;
+    p.free_head = free_head;
+    p.table_stride = block_table_stride;
+    p.batch = batch;
+    p.max_blocks = max_blocks_per_seq;
+    p.num_free = num_free;
+    p.page_size = page_size;
+    p.num_tokens = num_tokens;
+    p.slots = reinterpret_cast<long long *>(slots);
+    p.positions = positions;
+    p.cu_new = cu_new;
+    p.new_seq_lens = new_seq_lens;
+    p.new_free_head = new_free_head;
+    const int grid = (int)std::min<long long>(std::max(1LL, cdiv(num_tokens, slots::kThreads)), 2LL * info.sms);
+    slots::build_slots_kernel<<<grid, slots::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return launch_status();
+}
+
+int mla_b200_cache_write(const void *latent, int latent_dtype, long long latent_stride, const int64_t *slots,
+                         int num_tokens, const void *norm_weight, float eps, const int32_t *positions,
+                         const float *cos_sin, int max_positions, int interleaved, void *cache, int cache_dtype,
+                         long long cache_rows, float *kv_scales, void *stream) {
+    if (num_tokens < 0 || cache_rows < 0 || latent_stride < 0 || max_positions < 0) return MLA_B200_ERR_INVALID_ARG;
+    if (latent_dtype != MLA_B200_DTYPE_F16 && latent_dtype != MLA_B200_DTYPE_BF16 && latent_dtype != MLA_B200_DTYPE_F32)
+        return MLA_B200_ERR_INVALID_ARG;
+    if (cache_dtype != MLA_B200_DTYPE_F16 && cache_dtype != MLA_B200_DTYPE_BF16 && cache_dtype != MLA_B200_DTYPE_E4M3)
+        return MLA_B200_ERR_INVALID_ARG;
+    if (num_tokens > 0 && (latent == nullptr || slots == nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if (cache_rows > 0 && cache == nullptr) return MLA_B200_ERR_INVALID_ARG;
+    if ((cache_dtype == MLA_B200_DTYPE_E4M3) != (kv_scales != nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if ((positions == nullptr) != (cos_sin == nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if (norm_weight != nullptr && !(eps >= 0.f)) return MLA_B200_ERR_INVALID_ARG;
+    const size_t in_size = latent_dtype == MLA_B200_DTYPE_F32 ? 4 : 2;
+    if (!aligned(latent, in_size) || !aligned(norm_weight, in_size) || !aligned(slots, 8) || !aligned(positions, 4) ||
+        !aligned(cos_sin, 4) || !aligned(cache, 16) || !aligned(kv_scales, 4))
+        return MLA_B200_ERR_INVALID_ARG;
+    int dev;
+    DevInfo info;
+    const int st = current_device(&dev, &info);
+    if (st != MLA_B200_OK) return st;
+    if (num_tokens == 0 || cache_rows == 0) return MLA_B200_OK;
+    write::WriteParams p;
+    p.latent = latent;
+    p.stride = latent_stride;
+    p.slots = reinterpret_cast<const long long *>(slots);
+    p.positions = positions;
+    p.weight = norm_weight;
+    p.cos_sin = cos_sin;
+    p.max_pos = max_positions;
+    p.interleaved = interleaved;
+    p.eps = eps;
+    p.num_tokens = num_tokens;
+    p.cache = cache;
+    p.cache_rows = cache_rows;
+    p.kv_scales = kv_scales;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (latent_dtype == MLA_B200_DTYPE_F16) launch_write_to<__half>(p, cache_dtype, s);
+    else if (latent_dtype == MLA_B200_DTYPE_BF16) launch_write_to<__nv_bfloat16>(p, cache_dtype, s);
+    else launch_write_to<float>(p, cache_dtype, s);
+    return launch_status();
 }
 
 int mla_b200_decode_split_f16(const void *query, const void *cache, void *out, int num_heads,

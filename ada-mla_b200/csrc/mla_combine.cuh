@@ -269,7 +269,9 @@ __global__ void __launch_bounds__(32 * kRowsPerCombineBlock) combine_rows_kernel
 // a virtual packed axis, which the schedules then walk like a packed batch.
 // Called by all 1024 threads of one block; cu is complete and visible to the
 // block on return.
-__device__ void lens_to_offsets(const int32_t *lens, int batch, int max_len, int32_t *cu) {
+// Sequence b of the axis has the length lens[b / share] (draft trees: `share` row
+// tiles read one sequence).
+__device__ void lens_to_offsets(const int32_t *lens, int batch, int max_len, int32_t *cu, int share) {
     __shared__ int warp_tot[32];
     __shared__ int carry_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -277,7 +279,7 @@ __device__ void lens_to_offsets(const int32_t *lens, int batch, int max_len, int
     __syncthreads();
     for (int base = 0; base < batch; base += 1024) {
         const int b = base + tid;
-        const int len = b < batch ? min(max(lens[b], 0), max_len) : 0;
+        const int len = b < batch ? min(max(lens[share > 1 ? b / share : b], 0), max_len) : 0;
         int v = len;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -319,13 +321,14 @@ __global__ void __launch_bounds__(1024) plan_varlen_kernel(const int32_t *cu_seq
                                                            const int32_t *seq_lens = nullptr,
                                                            int max_len = 0,
                                                            int32_t *cu_out = nullptr,
-                                                           int group = 1, int dense_len = 0) {
+                                                           int group = 1, int dense_len = 0,
+                                                             int share = 1) {
     __shared__ int warp_tot[32];
     __shared__ int carry_s;
     griddep_launch();  // the decode kernel may start its set-up now
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (seq_lens != nullptr) {
-        lens_to_offsets(seq_lens, batch, max_len, cu_out);
+        lens_to_offsets(seq_lens, batch, max_len, cu_out, share);
         cu_seqlens = cu_out;
     }
     if (tid == 0) carry_s = 0;
@@ -383,13 +386,14 @@ __global__ void __launch_bounds__(1024) plan_balanced_kernel(const int32_t *cu_s
                                                              const int32_t *seq_lens = nullptr,
                                                              int max_len = 0,
                                                              int32_t *cu_out = nullptr,
-                                                             int group = 1, int dense_len = 0) {
+                                                             int group = 1, int dense_len = 0,
+                                                             int share = 1) {
     __shared__ int warp_tot[32];
     __shared__ int carry_s;
     griddep_launch();  // the decode kernel may start its set-up now
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (seq_lens != nullptr) {
-        lens_to_offsets(seq_lens, batch, max_len, cu_out);
+        lens_to_offsets(seq_lens, batch, max_len, cu_out, share);
         cu_seqlens = cu_out;
     }
     if (tid == 0) carry_s = 0;

@@ -64,6 +64,15 @@ typedef enum {
 /* Output element type for entry points that can emit either. */
 typedef enum { MLA_B200_OUT_F16 = 0, MLA_B200_OUT_F32 = 1, MLA_B200_OUT_BF16 = 2 } mla_b200_out_dtype;
 
+/* Element types of the entry points that take several (the first three numbered
+ * like mla_b200_out_dtype). */
+typedef enum {
+    MLA_B200_DTYPE_F16 = 0,
+    MLA_B200_DTYPE_F32 = 1,
+    MLA_B200_DTYPE_BF16 = 2,
+    MLA_B200_DTYPE_E4M3 = 3
+} mla_b200_dtype;
+
 /* Human-readable name of a status code (static string). */
 MLA_B200_API const char *mla_b200_status_string(int status);
 
@@ -239,6 +248,38 @@ MLA_B200_API int mla_b200_decode_mtp_bf16(const void *query, const void *cache,
                                           int out_dtype, float *out_lse, void *workspace,
                                           size_t workspace_bytes, void *stream);
 
+/* Draft trees over a paged cache (no counterpart in the reference): every
+ * sequence carries num_drafts queries, query [batch, num_drafts, num_heads, 576],
+ * whose latent rows are the last num_drafts rows of the sequence (seq_lens counts
+ * them).  Draft i sees every earlier row, and draft row j where bit j of
+ * tree_mask[b * num_drafts + i] is set (its ancestors and, usually, itself; bits at
+ * and past num_drafts are ignored).  shared_mask != 0: one tree for all sequences,
+ * tree_mask [num_drafts].  tree_mask NULL: a chain, draft i sees drafts 0..i.  A
+ * draft row that no draft sees may hold any bits (padded drafts); one that some
+ * draft sees is a number.  A query that sees no row at all: O = 0 and LSE = -inf.
+ * Sequences shorter than num_drafts have only their last drafts' rows.
+ * num_drafts <= 64, num_heads <= 128.  The drafts fill tiles of 128 / num_heads
+ * whole drafts, and each tile is one pass over the cache.  out [batch, num_drafts,
+ * num_heads, 512], out_lse [batch, num_drafts, num_heads] or NULL; otherwise the
+ * contract of mla_b200_decode_paged_f16 / _bf16.  Workspace:
+ * mla_b200_workspace_size_tree (0 for sizes that the decode refuses). */
+MLA_B200_API size_t mla_b200_workspace_size_tree(int batch, int num_drafts, int num_heads,
+                                                 int max_seq_len, int num_splits);
+MLA_B200_API int mla_b200_decode_tree_f16(const void *query, const void *kv_pages,
+                                          const int32_t *block_table, const int32_t *seq_lens,
+                                          const uint64_t *tree_mask, int shared_mask, int batch,
+                                          int num_drafts, int num_heads, int num_pages, int page_size,
+                                          int max_blocks_per_seq, int max_seq_len, float softmax_scale,
+                                          int num_splits, void *out, int out_dtype, float *out_lse,
+                                          void *workspace, size_t workspace_bytes, void *stream);
+MLA_B200_API int mla_b200_decode_tree_bf16(const void *query, const void *kv_pages,
+                                           const int32_t *block_table, const int32_t *seq_lens,
+                                           const uint64_t *tree_mask, int shared_mask, int batch,
+                                           int num_drafts, int num_heads, int num_pages, int page_size,
+                                           int max_blocks_per_seq, int max_seq_len, float softmax_scale,
+                                           int num_splits, void *out, int out_dtype, float *out_lse,
+                                           void *workspace, size_t workspace_bytes, void *stream);
+
 /* FP8 latent cache (no counterpart in the reference, which lists fp8 as future
  * work, README.md:407-408).  cache is e4m3 (OCP FP8, bias 7, no infinities)
  * with the layout of mla_b200_decode_batched_f16's cache (dense or packed) and
@@ -315,6 +356,50 @@ MLA_B200_API int mla_b200_decode_naive_f32(const float *query, const float *cach
 MLA_B200_API int mla_b200_decode_split_f16_noalloc(const void *query, const void *cache, void *out,
                                                    int num_heads, int seq_length, int num_splits,
                                                    void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Filling the paged latent cache                                            */
+/* ------------------------------------------------------------------------ */
+
+/* Pages and slots for the tokens a step appends (no reference counterpart: its
+ * cache is one contiguous tensor).  Request b holds seq_lens[b] tokens and appends
+ * new_lens[b] (negative counts are taken as 0).  Its new pages come from
+ * free_pages [num_free] in request order, starting at entry *free_head (device; NULL:
+ * 0), and go into block_table[b * block_table_stride + ...] after the
+ * ceil(seq_lens[b] / page_size) it has; entries past the end of the list are -1, and
+ * no page is taken for tokens past max_blocks_per_seq pages.  Outputs, all on the
+ * device: cu_new [batch + 1] exclusive sums of new_lens; for token t of the step,
+ * slots[t] = its pool row (page * page_size + offset; -1 where it has no page) and
+ * positions[t] = its position in its request; new_seq_lens [batch]; new_free_head
+ * [1] = *free_head + the pages taken (above num_free when the list ran out).  slots
+ * and positions have num_tokens entries: those past the step's tokens are -1 and 0,
+ * tokens past num_tokens get their pages only.  The call writes no input but
+ * block_table, and the same call again writes the same.  new_seq_lens and
+ * new_free_head may not be the inputs themselves. */
+MLA_B200_API int mla_b200_build_slots(const int32_t *seq_lens, const int32_t *new_lens,
+                                      int32_t *block_table, long long block_table_stride,
+                                      int max_blocks_per_seq, const int32_t *free_pages, int num_free,
+                                      const int32_t *free_head, int batch, int page_size, int num_tokens,
+                                      int64_t *slots, int32_t *positions, int32_t *cu_new,
+                                      int32_t *new_seq_lens, int32_t *new_free_head, void *stream);
+
+/* Latent rows into the cache (no reference counterpart).  latent: num_tokens rows
+ * of 576, latent_stride elements apart (F16, BF16 or F32).  norm_weight [512] in the
+ * same type, or NULL: columns 0..511 become x * rsqrt(mean(x^2) + eps) * weight.
+ * positions [num_tokens] with cos_sin [max_positions, 64] fp32 (the 32 angles'
+ * cosines, then their sines), or both NULL: columns 512..575 are rotated, pairs
+ * (2i, 2i + 1) when interleaved, else (i, i + 32).  Row t goes to cache row slots[t]
+ * of cache [cache_rows, 576] (a page pool is its rows): F16, BF16, or E4M3 with
+ * kv_scales [cache_rows] fp32, where the row's scale (largest value / 448, at least
+ * the smallest normal number; 1 for zeros) is kept and the row stored divided by it
+ * (what mla_b200_decode_batched_fp8_scaled reads).  A row whose slot is outside
+ * [0, cache_rows) or whose position is outside [0, max_positions) is not written.
+ * Two rows with one slot leave either.  cache is 16-byte aligned. */
+MLA_B200_API int mla_b200_cache_write(const void *latent, int latent_dtype, long long latent_stride,
+                                      const int64_t *slots, int num_tokens, const void *norm_weight,
+                                      float eps, const int32_t *positions, const float *cos_sin,
+                                      int max_positions, int interleaved, void *cache, int cache_dtype,
+                                      long long cache_rows, float *kv_scales, void *stream);
 
 /* ------------------------------------------------------------------------ */
 /* The per-head projections on either side of the decode                     */
