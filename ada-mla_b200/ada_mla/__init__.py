@@ -35,7 +35,7 @@ from ._build import EXT_NAME, EXT_PATH, LIB_PATH
 __all__ = [
     "mla_decode_naive", "mla_decode_fused", "mla_decode_split", "mla_decode_batched",
     "mla_decode_paged", "mla_decode_mtp", "mla_decode_tree", "tree_mask", "mla_build_slots", "SlotPlan",
-    "mla_cache_write",
+    "mla_cache_write", "mla_prefill",
     "mla_combine", "mla_get_device_error", "NUM_HEADS", "HEAD_DIM", "HEAD_DIM_C",
     "HEAD_DIM_ROPE", "HEAD_DIM_K", "HEAD_DIM_V", "SOFTMAX_SCALE", "lib_path", "ext_path",
 ]
@@ -268,3 +268,30 @@ def mla_cache_write(latent, slots, cache, norm_weight=None, eps: float = 1e-6, p
     """
     _ext.mla_cache_write(latent, slots, cache, norm_weight, float(eps), positions, cos_sin,
                          bool(interleaved), kv_scales)
+
+
+def mla_prefill(query, k_nope, k_rope, v, cu_seqlens_q=None, cu_seqlens_k=None, max_seq_len_q: int = -1,
+                max_seq_len_k: int = -1, softmax_scale: float = SOFTMAX_SCALE, causal: bool = True,
+                return_lse: bool = False):
+    """Attention over prompts in expanded form: per-head keys and values, and one rope
+    key per token shared by the heads.
+
+    query        [Tq, n_h, 192] fp16 or bf16: 128 columns for k_nope, 64 for k_rope.
+    k_nope, v    [Tk, n_h, 128], usually the two halves of one up-projection of the
+                 latent rows (views: any strides with a dense last dimension whose
+                 steps are multiples of 16 bytes).
+    k_rope       [Tk, 64].
+    cu_seqlens_q, cu_seqlens_k
+                 int32 [B + 1] on the device: sequence b's queries and keys.  Without
+                 them the inputs are dense: [B, Lq, n_h, 192], [B, Lk, n_h, 128],
+                 [B, Lk, 64].  Pass the longest lengths to avoid device->host reads.
+    causal       query i of a sequence sees keys 0 .. i + Lk - Lq: its queries are its
+                 last Lq tokens, so a chunk of a prompt sees all that came before.
+    Returns [.., n_h, 128] in the inputs' dtype and, with ``return_lse``, the
+    natural-log LSE [.., n_h] fp32 (for merging with attention over other keys).  A
+    query that sees no key gives zeros and -inf.  The form for single tokens is the
+    decode over the latent cache (``mla_decode_paged``, ``absorbed``).
+    """
+    out, lse = _ext.mla_prefill(query, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, int(max_seq_len_q),
+                                int(max_seq_len_k), float(softmax_scale), bool(causal), bool(return_lse))
+    return (out, lse) if return_lse else out

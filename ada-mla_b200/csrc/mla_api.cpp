@@ -357,6 +357,96 @@ std::vector<at::Tensor> mla_decode_tree(const at::Tensor &query, const at::Tenso
     return {out, lse};
 }
 
+// Attention over prompts in expanded form (no reference counterpart).
+//   query [Tq, n_h, 192], k_nope and v [Tk, n_h, 128], k_rope [Tk, 64], fp16 or bf16
+//   alike, packed by int32 cu_seqlens_q / cu_seqlens_k [B + 1]; or, without them,
+//   [B, Lq, n_h, 192], [B, Lk, n_h, 128], [B, Lk, 64].  Any strides with a dense last
+//   dimension and 16-byte multiples.  max_seq_len_* < 0 reads them from the device.
+// Returns (out [.., n_h, 128], lse [.., n_h] fp32 or empty).
+std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k_nope, const at::Tensor &k_rope,
+                                    const at::Tensor &v, const c10::optional<at::Tensor> &cu_seqlens_q,
+                                    const c10::optional<at::Tensor> &cu_seqlens_k, int64_t max_seq_len_q,
+                                    int64_t max_seq_len_k, double softmax_scale, bool causal, bool return_lse) {
+    const bool packed = cu_seqlens_q.has_value() && cu_seqlens_q->defined();
+    TORCH_CHECK(packed == (cu_seqlens_k.has_value() && cu_seqlens_k->defined()),
+                "mla_prefill: cu_seqlens_q and cu_seqlens_k come together");
+    const int64_t lead = packed ? 1 : 2;
+    const bool bf16 = query.scalar_type() == at::kBFloat16;
+    TORCH_CHECK(query.scalar_type() == at::kHalf || bf16, "mla_prefill: float16 or bfloat16 inputs expected");
+    auto check = [&](const at::Tensor &t, const char *name, int64_t heads, int64_t width) {
+        TORCH_CHECK(t.is_cuda() && t.device() == query.device(), name, " must be a CUDA tensor on the query's device");
+        TORCH_CHECK(t.scalar_type() == query.scalar_type(), "mla_prefill: ", name, " must have the query's dtype");
+        TORCH_CHECK(t.dim() == lead + (heads > 0 ? 2 : 1) && t.size(-1) == width && (heads <= 0 || t.size(-2) == heads),
+                    "mla_prefill: ", name, " has the wrong shape");
+        TORCH_CHECK(t.numel() == 0 || t.stride(-1) == 1, "mla_prefill: ", name, " must have a dense last dimension");
+        TORCH_CHECK(packed || t.size(0) <= 1 || t.size(1) == 0 || t.stride(0) == t.size(1) * t.stride(1),
+                    "mla_prefill: ", name, "'s sequences must follow one another");
+        TORCH_CHECK(t.numel() == 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                                       (t.size(lead - 1) <= 1 || t.stride(lead - 1) % 8 == 0) &&
+                                       (heads <= 1 || t.stride(lead) % 8 == 0)),
+                    "mla_prefill: ", name, " must start and step in multiples of 16 bytes");
+    };
+    TORCH_CHECK(query.is_cuda() && query.dim() == lead + 2 && query.size(-2) >= 1,
+                "mla_prefill: query must be a CUDA tensor [Tq, n_h, 192] (packed) or [B, Lq, n_h, 192]");
+    const int64_t nh = query.size(-2);
+    check(query, "query", nh, MLA_B200_HEAD_DIM + MLA_B200_HEAD_DIM_ROPE);
+    check(k_nope, "k_nope", nh, MLA_B200_HEAD_DIM);
+    check(v, "v", nh, MLA_B200_HEAD_DIM);
+    check(k_rope, "k_rope", 0, MLA_B200_HEAD_DIM_ROPE);
+    for (int64_t d = 0; d < lead; ++d)
+        TORCH_CHECK(k_nope.size(d) == v.size(d) && k_nope.size(d) == k_rope.size(d) &&
+                        (packed || d > 0 || k_nope.size(0) == query.size(0)),
+                    "mla_prefill: k_nope, k_rope and v must have the same tokens");
+    c10::cuda::CUDAGuard g(query.device());
+    const int32_t *cu_q = nullptr, *cu_k = nullptr;
+    int64_t b = query.size(0), tq = query.size(0), tk = k_nope.size(0);
+    if (packed) {
+        for (const at::Tensor *cu : {&*cu_seqlens_q, &*cu_seqlens_k}) {
+            check_cuda(*cu, "cu_seqlens");
+            TORCH_CHECK(cu->device() == query.device() && cu->scalar_type() == at::kInt && cu->dim() == 1 &&
+                            cu->size(0) >= 1 && cu->size(0) == cu_seqlens_q->size(0),
+                        "mla_prefill: cu_seqlens must be int32 [B + 1] on the query's device");
+        }
+        b = cu_seqlens_q->size(0) - 1;
+        cu_q = cu_seqlens_q->data_ptr<int32_t>();
+        cu_k = cu_seqlens_k->data_ptr<int32_t>();
+        auto longest = [&](const at::Tensor &cu) {
+            return b > 0 ? std::max<int64_t>((cu.slice(0, 1) - cu.slice(0, 0, b)).max().item<int64_t>(), 0) : 0;
+        };
+        if (max_seq_len_q < 0) max_seq_len_q = longest(*cu_seqlens_q);
+        if (max_seq_len_k < 0) max_seq_len_k = longest(*cu_seqlens_k);
+    } else {
+        max_seq_len_q = query.size(1);
+        max_seq_len_k = k_nope.size(1);
+        tq = b * max_seq_len_q;
+        tk = b * max_seq_len_k;
+    }
+    TORCH_CHECK(max_seq_len_q <= INT32_MAX && max_seq_len_k <= INT32_MAX && b <= INT32_MAX && nh <= INT32_MAX,
+                "mla_prefill: sizes out of range");
+    auto shape = query.sizes().vec();
+    shape.back() = MLA_B200_HEAD_DIM;
+    // (rows outside every sequence of a packed batch are left as they are allocated)
+    at::Tensor out = at::empty(shape, query.options());
+    shape.pop_back();
+    if (!return_lse) shape[0] = 0;
+    at::Tensor lse = at::empty(shape, query.options().dtype(at::kFloat));
+    at::Tensor w;
+    size_t ws = 0;
+    if (packed && b > 1) {
+        ws = mla_b200_workspace_size_prefill((int)b, tq);
+        w = workspace(query, ws);
+    }
+    auto *fn = bf16 ? mla_b200_prefill_bf16 : mla_b200_prefill_f16;
+    const int64_t d = lead - 1;
+    check_status(fn(query.data_ptr(), query.stride(d), query.stride(d + 1), k_nope.data_ptr(), k_nope.stride(d),
+                    k_nope.stride(d + 1), k_rope.data_ptr(), k_rope.stride(d), v.data_ptr(), v.stride(d),
+                    v.stride(d + 1), cu_q, cu_k, (int)b, (int)nh, tq, tk, (int)max_seq_len_q, (int)max_seq_len_k,
+                    causal ? 1 : 0, (float)softmax_scale, out.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
+                    ws > 0 ? w.data_ptr() : nullptr, ws, stream_ptr()),
+                 "mla_prefill");
+    return {out, lse};
+}
+
 // Pages and slots for a step's new tokens (no reference counterpart); block_table is
 // written in place.  Returns (slots int64 [num_tokens], positions int32
 // [num_tokens], cu_new int32 [B + 1], new seq_lens int32 [B], new free_head int32 [1]).
@@ -537,6 +627,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("tree_mask") = py::none(), py::arg("max_seq_len") = -1,
           py::arg("softmax_scale") = 0.07216878364870322, py::arg("num_splits") = -1,
           py::arg("return_lse") = false, py::arg("out_fp32") = false);
+    m.def("mla_prefill", &mla_prefill, "attention over prompts in expanded form", py::arg("query"),
+          py::arg("k_nope"), py::arg("k_rope"), py::arg("v"), py::arg("cu_seqlens_q") = py::none(),
+          py::arg("cu_seqlens_k") = py::none(), py::arg("max_seq_len_q") = -1, py::arg("max_seq_len_k") = -1,
+          py::arg("softmax_scale") = 0.07216878364870322, py::arg("causal") = true, py::arg("return_lse") = false);
     m.def("mla_build_slots", &mla_build_slots, "pages and slots for a step's new tokens", py::arg("seq_lens"),
           py::arg("new_lens"), py::arg("block_table"), py::arg("free_pages"), py::arg("page_size"),
           py::arg("num_tokens"), py::arg("free_head") = py::none());

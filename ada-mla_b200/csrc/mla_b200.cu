@@ -17,6 +17,7 @@
 #include "mla_b200.h"
 #include "mla_combine.cuh"
 #include "mla_fp8.cuh"
+#include "mla_prefill.cuh"
 #include "mla_common.cuh"
 #include "mla_exchange.cuh"
 #include "mla_proj.cuh"
@@ -38,6 +39,7 @@ struct DevInfo {
     int major = 0;
     bool simt_attr_set = false;
     bool proj_attr_set = false;
+    bool prefill_attr_set = false;
     int tc_clusters = 0;  // co-resident 2-CTA clusters of the tcgen05 decode kernel
 };
 
@@ -97,6 +99,19 @@ int current_device(int *dev_out, DevInfo *info_out) {
                                  proj::kSmemBudget + 4096) != cudaSuccess)
             return cuda_failure(cudaGetLastError());
         d.proj_attr_set = true;
+    }
+    if (!d.prefill_attr_set) {
+        for (const void *k : {reinterpret_cast<const void *>(&prefill::prefill_kernel<false>),
+                              reinterpret_cast<const void *>(&prefill::prefill_kernel<true>)}) {
+            if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, prefill::kSmemBytes) != cudaSuccess)
+                return cuda_failure(cudaGetLastError());
+            // the softmax warps' larger register share comes out of what the block was
+            // launched with: a kernel compiled to fewer would wait for it without end
+            cudaFuncAttributes a;
+            if (cudaFuncGetAttributes(&a, k) != cudaSuccess) return cuda_failure(cudaGetLastError());
+            if (a.numRegs < prefill::kRegsLaunch) return MLA_B200_ERR_UNSUPPORTED;
+        }
+        d.prefill_attr_set = true;
     }
     if (d.tc_clusters == 0) {
         if (!set_tc_smem<false, false>() || !set_tc_smem<true, false>() ||
@@ -977,6 +992,120 @@ int run_proj(const void *x, const void *w, const void *rope, void *out, int batc
 }  // namespace
 
 namespace {
+// One operand of the prompt attention: `rows` tokens of `heads` rows of `width`
+// elements, strides in elements.
+struct Operand {
+    const void *base;
+    long long rows;
+    int heads, width;
+    long long row_stride, head_stride;
+};
+
+bool operand_ok(const Operand &o) {
+    return aligned(o.base, 16) && o.row_stride >= 0 && o.head_stride >= 0 && (o.rows <= 1 || o.row_stride % 8 == 0) &&
+           (o.heads <= 1 || o.head_stride % 8 == 0);
+}
+
+// (width, heads, rows) in boxes of 64 columns x 1 head x box_rows
+int make_tmap_operand(CUtensorMap *map, const Operand &o, int box_rows, bool bf16, const void *some) {
+    const long long rows = std::max(o.rows, 1LL);
+    const cuuint64_t dims[3] = {(cuuint64_t)o.width, (cuuint64_t)o.heads, (cuuint64_t)rows};
+    const long long hs = o.heads > 1 ? o.head_stride : o.width, rs = rows > 1 ? o.row_stride : (long long)o.width * o.heads;
+    const cuuint64_t strides[2] = {(cuuint64_t)hs * 2, (cuuint64_t)rs * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows};
+    return encode_tmap(map, o.rows > 0 ? o.base : some, 3, dims, strides, box, bf16);
+}
+
+struct PrefillWs {
+    int2 *pairs;
+    int *num_pairs;
+    long long cap;
+    size_t bytes;
+};
+
+PrefillWs prefill_ws(void *base, int batch, long long total_q) {
+    PrefillWs w;
+    w.cap = total_q / prefill::kItemQ + batch;
+    w.num_pairs = static_cast<int *>(base);
+    w.pairs = reinterpret_cast<int2 *>(static_cast<char *>(base) + 256);
+    w.bytes = 256 + (size_t)w.cap * sizeof(int2);
+    return w;
+}
+
+// Bytes of keys and values whose heads are walked together: what stays in L2 (126 MB)
+// next to the queries and outputs that stream through it.
+constexpr long long kPrefillL2 = 48LL << 20;
+
+template <bool kBf16>
+int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Operand &v, const int32_t *cu_q,
+                const int32_t *cu_k, int batch, int max_q, int max_k, int causal, float scale, void *out,
+                float *out_lse, void *workspace, size_t workspace_bytes, cudaStream_t stream) {
+    const int heads = q.heads;
+    if (batch < 0 || heads <= 0 || q.rows < 0 || kn.rows < 0 || max_q < 0 || max_k < 0) return MLA_B200_ERR_INVALID_ARG;
+    if (q.rows > 0 && (q.base == nullptr || out == nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if (kn.rows > 0 && (kn.base == nullptr || kr.base == nullptr || v.base == nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if ((cu_q == nullptr) != (cu_k == nullptr)) return MLA_B200_ERR_INVALID_ARG;
+    if (cu_q == nullptr && ((long long)batch * max_q != q.rows || (long long)batch * max_k != kn.rows))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (!(scale > 0.f) || !isfinite(scale)) return MLA_B200_ERR_INVALID_ARG;
+    if (!operand_ok(q) || !operand_ok(kn) || !operand_ok(kr) || !operand_ok(v) || !aligned(out, 32) ||
+        !aligned(out_lse, 4) || !aligned(cu_q, 4) || !aligned(cu_k, 4))
+        return MLA_B200_ERR_INVALID_ARG;
+    if (q.rows >= (1LL << 31) || kn.rows >= (1LL << 31)) return MLA_B200_ERR_UNSUPPORTED;
+    const PrefillWs ws = prefill_ws(workspace, batch, q.rows);
+    const int blocks = (int)cdiv(max_q, prefill::kItemQ);
+    const bool planned = cu_q != nullptr && batch > 1;
+    const long long pairs = planned ? ws.cap : (long long)batch * blocks;
+    if (pairs * heads >= (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
+    int dev;
+    DevInfo info;
+    int st = current_device(&dev, &info);
+    if (st != MLA_B200_OK) return st;
+    if (batch == 0 || q.rows == 0 || max_q == 0) return MLA_B200_OK;
+    if (planned && (workspace == nullptr || workspace_bytes < ws.bytes)) return MLA_B200_ERR_WORKSPACE;
+    if (planned && !aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
+    CUtensorMap qm, km, rm, vm;
+    st = make_tmap_operand(&qm, q, prefill::kTileQ, kBf16, q.base);
+    if (st == MLA_B200_OK) st = make_tmap_operand(&km, kn, prefill::kTileK, kBf16, q.base);
+    if (st == MLA_B200_OK) st = make_tmap_operand(&vm, v, prefill::kVHalf, kBf16, q.base);
+    if (st == MLA_B200_OK) {
+        const cuuint64_t dims[2] = {MLA_B200_HEAD_DIM_ROPE, (cuuint64_t)std::max(kr.rows, 1LL)};
+        const cuuint64_t strides[1] = {(cuuint64_t)(kr.rows > 1 ? kr.row_stride : MLA_B200_HEAD_DIM_ROPE) * 2};
+        const cuuint32_t box[2] = {64, (cuuint32_t)prefill::kTileK};
+        st = encode_tmap(&rm, kr.rows > 0 ? kr.base : q.base, 2, dims, strides, box, kBf16);
+    }
+    if (st != MLA_B200_OK) return st;
+    prefill::PrefillParams p{};
+    p.cu_q = cu_q;
+    p.cu_k = cu_k;
+    p.batch = batch;
+    p.heads = heads;
+    p.max_q = max_q;
+    p.max_k = max_k;
+    p.total_q = (int)q.rows;
+    p.total_k = (int)kn.rows;
+    p.causal = causal;
+    p.scale_log2 = scale * kLog2e;
+    p.dense_blocks = blocks;
+    const long long head_bytes = std::max(1LL, kn.rows * (MLA_B200_HEAD_DIM + prefill::kV) * 2);
+    p.head_group = (int)std::max(1LL, std::min((long long)heads, kPrefillL2 / head_bytes));
+    p.out = out;
+    p.out_lse = out_lse;
+    if (planned) {
+        prefill::plan_kernel<<<1, 1024, 0, stream>>>(p, (int)ws.cap, ws.pairs, ws.num_pairs);
+        p.pairs = ws.pairs;
+        p.num_pairs = ws.num_pairs;
+    }
+    const int grid = (int)std::min<long long>(pairs * heads, info.sms);
+    timing_mark(t_ev_start, stream);
+    launch_dependent(prefill::prefill_kernel<kBf16>, dim3(grid), dim3(prefill::kThreads), prefill::kSmemBytes, stream,
+                     planned, qm, km, rm, vm, p);
+    timing_mark(t_ev_stop, stream);
+    return launch_status();
+}
+}  // namespace
+
+namespace {
 template <typename InT, typename OutT>
 void launch_write(const write::WriteParams &p, bool vec, cudaStream_t stream) {
     const unsigned grid = (unsigned)cdiv(p.num_tokens, write::kWarps);
@@ -1088,6 +1217,38 @@ int mla_b200_plan(int batch, int num_heads, long long total_tokens, int max_seq_
     if (chunk_tokens) *chunk_tokens = chunk;
     if (num_splits) *num_splits = max_seq_len > 0 ? (int)cdiv(max_seq_len, chunk) : 0;
     return MLA_B200_OK;
+}
+
+size_t mla_b200_workspace_size_prefill(int batch, long long total_q) {
+    return batch < 0 || total_q < 0 ? 0 : prefill_ws(nullptr, batch, total_q).bytes;
+}
+
+int mla_b200_prefill_f16(const void *query, long long query_stride, long long query_head_stride, const void *k_nope,
+                         long long k_stride, long long k_head_stride, const void *k_rope, long long rope_stride,
+                         const void *v, long long v_stride, long long v_head_stride, const int32_t *cu_seqlens_q,
+                         const int32_t *cu_seqlens_k, int batch, int num_heads, long long total_q, long long total_k,
+                         int max_seq_len_q, int max_seq_len_k, int causal, float softmax_scale, void *out,
+                         float *out_lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return run_prefill<false>({query, total_q, num_heads, prefill::kQK, query_stride, query_head_stride},
+                              {k_nope, total_k, num_heads, MLA_B200_HEAD_DIM, k_stride, k_head_stride},
+                              {k_rope, total_k, 1, MLA_B200_HEAD_DIM_ROPE, rope_stride, 0},
+                              {v, total_k, num_heads, prefill::kV, v_stride, v_head_stride}, cu_seqlens_q,
+                              cu_seqlens_k, batch, max_seq_len_q, max_seq_len_k, causal, softmax_scale, out, out_lse,
+                              workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int mla_b200_prefill_bf16(const void *query, long long query_stride, long long query_head_stride, const void *k_nope,
+                         long long k_stride, long long k_head_stride, const void *k_rope, long long rope_stride,
+                         const void *v, long long v_stride, long long v_head_stride, const int32_t *cu_seqlens_q,
+                         const int32_t *cu_seqlens_k, int batch, int num_heads, long long total_q, long long total_k,
+                         int max_seq_len_q, int max_seq_len_k, int causal, float softmax_scale, void *out,
+                         float *out_lse, void *workspace, size_t workspace_bytes, void *stream) {
+    return run_prefill<true>({query, total_q, num_heads, prefill::kQK, query_stride, query_head_stride},
+                              {k_nope, total_k, num_heads, MLA_B200_HEAD_DIM, k_stride, k_head_stride},
+                              {k_rope, total_k, 1, MLA_B200_HEAD_DIM_ROPE, rope_stride, 0},
+                              {v, total_k, num_heads, prefill::kV, v_stride, v_head_stride}, cu_seqlens_q,
+                              cu_seqlens_k, batch, max_seq_len_q, max_seq_len_k, causal, softmax_scale, out, out_lse,
+                              workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 namespace {

@@ -1,0 +1,634 @@
+// mla_prefill.cuh -- attention over prompts in expanded form, tcgen05:
+//
+//   s[h, i, j] = scale (q_nope[i, h] . k_nope[j, h] + q_rope[i, h] . k_rope[j])
+//   o[i, h]    = softmax_j(s) v[j, h]          (j <= i + Lk - Lq when causal)
+//
+// q [.., 128 + 64], k_nope and v 128 wide per head, k_rope ONE 64-wide vector per
+// token shared by all heads: its tile is loaded straight into the third K-block of
+// the key tile, so the 192-wide keys never exist in memory.
+//
+// A work item is 256 query rows of one (sequence, head), two tiles of 128, on one
+// persistent CTA per SM.  Both tiles read each key / value tile of 128 tokens once.
+// While the tensor core works on one tile, the other tile's softmax runs:
+//
+//   MMA thread:  PV0(j)  QK0(j+1)  PV1(j)  QK1(j+1)  PV0(j+1) ...
+//   softmax 0:           [ tile 0, j+1 ......... ]
+//   softmax 1:                              [ tile 1, j+1 ......... ]
+//
+// TMEM (512 columns): S0 S1 [128 x 128] fp32, O0 O1 [128 x 128] fp32; P (16-bit)
+// overwrites the first half of its S and is PV's A operand.  A tile of the pair costs
+// 768 cycles of QK (K = 192) and 512 of PV at the tensor rate, against 1024 cycles of
+// exponentials (16 per cycle and SM), so the tensor core can be the bound.
+//
+// Shared memory: Q0 Q1 (2 x 48 KB) and a ring of eight 16 KB slots, a slot being one
+// 64-column block of 128 keys or 64 tokens of V: K(0) V(0) K(1) V(1) .. in 3 + 2
+// slots each.  Slots of one size let the two kinds share 128 KB (1.6 tiles).
+//
+// Roles (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 TMEM owner and
+// V tail, warps 4-7 softmax of tile 0, warps 8-11 of tile 1 (a thread per row: no
+// shuffles).  The softmax warps rescale O themselves, rarely: the running maximum is
+// only raised when it grew by more than 2^8.  Every wait is bounded.
+#pragma once
+
+#include "mla_tc.cuh"
+
+namespace mla {
+namespace prefill {
+
+constexpr int kQK = MLA_B200_HEAD_DIM + MLA_B200_HEAD_DIM_ROPE;  // 192
+constexpr int kV = MLA_B200_HEAD_DIM;                            // 128
+constexpr int kTileQ = 128;
+constexpr int kItemQ = 2 * kTileQ;
+constexpr int kTileK = 128;
+constexpr int kKBlk = kQK / 64;                 // 3
+constexpr int kBox = kTileQ * 128;              // 16 KB: 128 rows x 64 columns
+constexpr int kQBytes = kKBlk * kBox;           // 48 KB
+constexpr int kVHalf = kTileK / 2;              // tokens of a V slot
+constexpr int kVBox = kVHalf * 128;             // 8 KB: 64 tokens x 64 columns
+constexpr int kSlots = 8;
+constexpr int kSlotsPerTile = kKBlk + 2;        // 5
+constexpr int kThreads = 384;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kTmemO = 256;
+constexpr int kOffRing = 2 * kQBytes;
+constexpr int kOffBar = kOffRing + kSlots * kBox;
+enum : int {
+    kBarFull = 0,
+    kBarEmpty = kSlots,
+    kBarQFull = 2 * kSlots,      // [2] Q tile landed
+    kBarQEmpty = kBarQFull + 2,  // [2] last QK of the item done
+    kBarS = kBarQEmpty + 2,      // [2] S tile complete
+    kBarP = kBarS + 2,           // [2] P tile written, O corrected (128 threads)
+    kBarO = kBarP + 2,           // [2] PV done
+    kBarTail = kBarO + 2,        // [2] a sequence's last V tile landed, rows past its end not yet zeroed
+    kBarDrain = kBarTail + 2,
+    kNumBars = kBarDrain + 1
+};
+constexpr int kOffSlot = kOffBar + kNumBars * 8;
+constexpr int kOffAbort = kOffSlot + 4;
+constexpr int kSmemBytes = kOffAbort + 4 + 1024;  // + 1024 alignment slack
+static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
+// 384 threads x 168 registers at launch = 64512; the softmax warpgroups take 200
+// each and the first one keeps 104: 2 x 128 x 200 + 128 x 104 = 64512.
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
+static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
+constexpr float kRescaleLog2 = 8.f;
+constexpr int kPlanBuckets = 1024;
+constexpr uint32_t kMaxIdle = 100000000;  // tries of 200 ns and more: 20 s and more
+
+struct PrefillParams {
+    const int32_t *cu_q, *cu_k;  // null: dense
+    int batch, heads, max_q, max_k;
+    int total_q, total_k;
+    int causal;
+    float scale_log2;
+    const int2 *pairs;      // {sequence, first query row}, longest first; null: one sequence or a dense batch
+    const int *num_pairs;
+    int dense_blocks;       // without pairs: 256-row blocks per sequence
+    int head_group;         // heads walked together
+    void *out;              // [total_q, heads, 128]
+    float *out_lse;         // [total_q, heads] or null
+};
+
+struct Seq {
+    int q0, k0;  // first rows (all rows are below 2^31)
+    int lq, lk;
+};
+
+__device__ __forceinline__ Seq seq_of(const PrefillParams &p, int b) {
+    Seq s;
+    if (p.cu_q == nullptr) {
+        s.q0 = b * p.max_q;
+        s.k0 = b * p.max_k;
+        s.lq = p.max_q;
+        s.lk = p.max_k;
+    } else {
+        s.q0 = min(max(p.cu_q[b], 0), p.total_q);
+        s.k0 = min(max(p.cu_k[b], 0), p.total_k);
+        s.lq = min(p.max_q, max(0, min(p.cu_q[b + 1], p.total_q) - s.q0));
+        s.lk = min(p.max_k, max(0, min(p.cu_k[b + 1], p.total_k) - s.k0));
+    }
+    return s;
+}
+
+// Key tiles that rows [row, row + 128) of a sequence see.
+__device__ __forceinline__ int tiles_of(const PrefillParams &p, const Seq &s, int row) {
+    if (row >= s.lq) return 0;
+    int end = s.lk;
+    if (p.causal) end = min(end, min(row + kTileQ, s.lq) + s.lk - s.lq);
+    return end > 0 ? (end + kTileK - 1) / kTileK : 0;
+}
+
+struct Item {
+    Seq s;
+    int h, row;   // head, first query row of the item in its sequence
+    int n[2];     // key tiles of its two query tiles (n[0] <= n[1] unless tile 1 has no rows)
+    int nmax;
+};
+
+// Walks this CTA's items.  Items are laid out by head group (so that the keys and
+// values of the heads in flight stay in L2), within a group by pair (longest first),
+// and dealt to the CTAs back and forth (a CTA that got a long item in one round
+// gets a short one in the next).
+struct Cursor {
+    int round = 0;
+    int pairs, total;
+    __device__ __forceinline__ void init(const PrefillParams &p) {
+        pairs = p.pairs != nullptr ? *p.num_pairs : p.batch * p.dense_blocks;
+        total = pairs * p.heads;
+    }
+    __device__ __forceinline__ bool next(const PrefillParams &p, Item &it) {
+        const int g = gridDim.x, c = blockIdx.x;
+        const int u = round * g + ((round & 1) ? g - 1 - c : c);
+        if (round * g >= total) return false;
+        ++round;
+        it.nmax = -1;  // no item in this round
+        if (u >= total) return true;
+        const int per = pairs * p.head_group;
+        const int grp = u / per, r = u - grp * per;
+        const int heads = min(p.head_group, p.heads - grp * p.head_group);
+        const int pair = r / heads;
+        it.h = grp * p.head_group + (r - pair * heads);
+        int b;
+        if (p.pairs != nullptr) {
+            const int2 pr = p.pairs[pair];
+            b = pr.x;
+            it.row = pr.y;
+        } else {  // last blocks first
+            const int lvl = pair / p.batch;
+            b = pair - lvl * p.batch;
+            it.row = (p.dense_blocks - 1 - lvl) * kItemQ;
+        }
+        it.s = seq_of(p, b);
+        if (it.row >= it.s.lq) return true;
+        it.n[0] = tiles_of(p, it.s, it.row);
+        it.n[1] = tiles_of(p, it.s, it.row + kTileQ);
+        it.nmax = max(it.n[0], it.n[1]);
+        return true;
+    }
+};
+
+// {sequence, first row} of every 256-row block, most key tiles first (a counting
+// sort; blocks of one bucket come in any order, which no result depends on).  One
+// block, a warp per sequence.
+__global__ void __launch_bounds__(1024) plan_kernel(const PrefillParams p, int cap, int2 *__restrict__ pairs,
+                                                    int *__restrict__ num_pairs) {
+    __shared__ int count[kPlanBuckets];
+    __shared__ int warp_tot[32];
+    griddep_launch();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    count[tid] = 0;
+    __syncthreads();
+    const int most = (p.max_k + kTileK - 1) / kTileK + 1;
+    auto bucket = [&](const Seq &s, int row) {
+        const int n = max(tiles_of(p, s, row), tiles_of(p, s, row + kTileQ));
+        return kPlanBuckets - 1 - (int)((long long)n * kPlanBuckets / (most + 1));
+    };
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int b = warp; b < p.batch; b += 32) {
+            const Seq s = seq_of(p, b);
+            for (int row = lane * kItemQ; row < s.lq; row += 32 * kItemQ) {
+                const int at = atomicAdd(&count[bucket(s, row)], 1);
+                if (pass == 1 && at < cap) pairs[at] = make_int2(b, row);
+            }
+        }
+        __syncthreads();
+        if (pass == 0) {  // counts -> starts
+            const int own = count[tid];
+            int v = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            if (lane == 31) warp_tot[warp] = v;
+            __syncthreads();
+            if (warp == 0) {
+                int w = warp_tot[lane];
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, w, o);
+                    if (lane >= o) w += u;
+                }
+                warp_tot[lane] = w;
+            }
+            __syncthreads();
+            count[tid] = (warp > 0 ? warp_tot[warp - 1] : 0) + v - own;
+            if (tid == 1023) *num_pairs = min(warp_tot[31], cap);
+            __syncthreads();
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Packed fp32 pairs.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+        "add.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// Bounded wait without a pause between tries (try_wait itself suspends for a while).
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int err) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t n = 1;; ++n) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((n & 63) == 0) {
+            const uint64_t t = globaltimer_ns();
+            if (t0 == 0) {
+                t0 = t;
+            } else if (t - t0 > kWaitLimitNs) {
+                set_device_error(err);
+                return false;
+            }
+        }
+    }
+}
+
+// The V tail warp may have nothing to do for the whole of a long item: its limit
+// starts anew while the other roles are at work, and an abort ends it.
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
+    for (uint32_t n = 0; n < kMaxIdle; ++n) {
+        if (*abort_flag) return false;
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        __nanosleep(200);
+    }
+    set_device_error(kErrWaitFull);
+    return false;
+}
+
+__device__ __forceinline__ void store32(void *dst, const uint32_t (&v)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// qmap: q as (192, heads, rows), box (64, 1, 128); kmap: k_nope as (128, heads,
+// rows), box (64, 1, 128); rmap: k_rope as (64, rows), box (64, 128); vmap: v as
+// (128, heads, rows), box (64, 1, 64).  128-byte swizzle.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                   const __grid_constant__ CUtensorMap rmap, const __grid_constant__ CUtensorMap vmap,
+                   const PrefillParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = ptx::smem_u32(smem);
+    auto bar = [&](int id) -> uint32_t { return sbase + kOffBar + 8u * id; };
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + kOffAbort);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < kNumBars; ++i) ptx::mbar_init(bar(i), i == kBarP || i == kBarP + 1 ? 128 : 1);
+        *abort_flag = 0;
+        ptx::fence_mbarrier_init_cluster();
+    }
+    if (tid == 32) {
+        ptx::tma_prefetch_desc(&qmap);
+        ptx::tma_prefetch_desc(&kmap);
+        ptx::tma_prefetch_desc(&rmap);
+        ptx::tma_prefetch_desc(&vmap);
+    }
+    if (warp == 2) {
+        ptx::tmem_alloc(sbase + kOffSlot, kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + kOffSlot);
+    griddep_launch();
+    griddep_wait();
+
+    Cursor cur;
+    cur.init(p);
+    Item it{};
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (warp == 0) {
+            // ------------------------------------------------------ TMA producer
+            if (lane == 0) {
+                uint32_t at = 0;           // slots filled so far
+                uint32_t qn[2] = {0, 0};   // Q tiles loaded so far
+                uint32_t tails = 0;        // V tiles handed to the V tail warp so far
+                bool ok = true;
+                auto acquire = [&](uint32_t &full, bool tail = false) -> uint32_t {  // next slot's address, its full barrier
+                    const uint32_t s = at % kSlots;
+                    if (!ok || *abort_flag || !wait_bar(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty)) {
+                        ok = false;
+                        return 0;
+                    }
+                    ++at;
+                    full = bar(tail ? kBarTail + (tails & 1) : kBarFull + s);
+                    if (!tail) ptx::mbar_arrive_expect_tx(full, kBox);
+                    return sbase + kOffRing + s * kBox;
+                };
+                auto load_q = [&](int t) {
+                    if (!ok || *abort_flag || !wait_bar(bar(kBarQEmpty + t), (qn[t] & 1) ^ 1, kErrWaitEmpty)) {
+                        ok = false;
+                        return;
+                    }
+                    ++qn[t];
+                    ptx::mbar_arrive_expect_tx(bar(kBarQFull + t), kQBytes);
+                    const int row = it.s.q0 + it.row + t * kTileQ;
+                    for (int c = 0; c < kKBlk; ++c)
+                        ptx::tma_load_3d(sbase + t * kQBytes + c * kBox, &qmap, c * 64, it.h, row, bar(kBarQFull + t));
+                };
+                auto load_k = [&](int j) {
+                    const int row = it.s.k0 + j * kTileK;
+                    uint32_t full = 0;
+                    for (int c = 0; c < kKBlk; ++c) {
+                        const uint32_t dst = acquire(full);
+                        if (!ok) return;
+                        if (c < 2) ptx::tma_load_3d(dst, &kmap, c * 64, it.h, row, full);
+                        else ptx::tma_load_2d(dst, &rmap, 0, row, full);
+                    }
+                };
+                auto load_v = [&](int j) {
+                    const int row = it.s.k0 + j * kTileK;
+                    const bool tail = (j + 1) * kTileK > it.s.lk;
+                    uint32_t full = 0;
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t dst = acquire(full, tail);
+                        if (!ok) return;
+                        if (tail && c == 0) ptx::mbar_arrive_expect_tx(full, 2 * kBox);
+                        ptx::tma_load_3d(dst, &vmap, 0, it.h, row + c * kVHalf, full);
+                        ptx::tma_load_3d(dst + kVBox, &vmap, 64, it.h, row + c * kVHalf, full);
+                    }
+                    if (tail) ++tails;
+                };
+                while (ok && cur.next(p, it)) {
+                    if (it.nmax <= 0) continue;
+                    if (it.n[0] > 0) load_q(0);
+                    load_k(0);
+                    if (it.n[1] > 0) load_q(1);
+                    for (int j = 0; ok && j < it.nmax; ++j) {
+                        load_v(j);
+                        if (j + 1 < it.nmax) load_k(j + 1);
+                    }
+                }
+                if (!ok) *abort_flag = 1;
+                // every load has landed before this CTA's shared memory goes
+                for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
+                    ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
+                for (uint32_t k = tails > 2 ? tails - 2 : 0; k < tails; ++k)
+                    ptx::mbar_wait(bar(kBarTail + (k & 1)), (k >> 1) & 1, kErrWaitFull);
+                for (int t = 0; t < 2; ++t)
+                    if (qn[t] > 0) ptx::mbar_wait(bar(kBarQFull + t), (qn[t] - 1) & 1, kErrWaitFull);
+            }
+        } else if (warp == 1) {
+            // ------------------------------------------------------ MMA issuer
+            if (lane == 0) {
+                const uint32_t idesc_qk = ptx::idesc_f16_f32(kTileQ, kTileK, 0, 0, kBf16);
+                const uint32_t idesc_pv = ptx::idesc_f16_f32(kTileQ, kV, 0, 1, kBf16);
+                uint32_t at = 0;  // ring slots of the items before this one
+                uint32_t qn[2] = {0, 0}, pn[2] = {0, 0};
+                bool ok = true;
+                auto full = [&](uint32_t k) {
+                    if (ok && !ptx::mbar_spin(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull)) ok = false;
+                };
+                // S_t = Q_t . K(j)^T; the last reader frees the slots
+                auto qk = [&](int t, int j, bool free_slots, bool last) {
+                    const uint32_t k0 = at + j * kSlotsPerTile;
+                    for (int c = 0; c < kKBlk; ++c) {
+                        full(k0 + c);
+                        if (!ok) return;
+                        const uint32_t slot = (k0 + c) % kSlots;
+                        const uint64_t a = ptx::sdesc_sw128(sbase + t * kQBytes + c * kBox, 16, 1024);
+                        const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, 16, 1024);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            ptx::mma_ss(tmem + t * kTileK, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
+                                        (c > 0 || k > 0) ? 1u : 0u);
+                        if (free_slots) ptx::mma_commit(bar(kBarEmpty + slot));
+                    }
+                    ptx::mma_commit(bar(kBarS + t));
+                    if (last) ptx::mma_commit(bar(kBarQEmpty + t));
+                };
+                // O_t += P_t . V(j)
+                auto pv = [&](int t, int j, bool free_slots) {
+                    if (!ptx::mbar_spin(bar(kBarP + t), pn[t] & 1, kErrWaitMma)) { ok = false; return; }
+                    ++pn[t];
+                    const uint32_t k0 = at + j * kSlotsPerTile + kKBlk;
+                    ptx::tc_fence_after();  // P (and a corrected O) were stored by other threads
+                    for (int c = 0; c < 2; ++c) {
+                        full(k0 + c);
+                        if (!ok) return;
+                        const uint32_t slot = (k0 + c) % kSlots;
+                        const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, kVBox, 1024);
+#pragma unroll
+                        for (int k = 0; k < kVHalf / 16; ++k)
+                            ptx::mma_ts(tmem + kTmemO + t * kV, tmem + t * kTileK + (c * 4 + k) * 8,
+                                        b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || c > 0 || k > 0) ? 1u : 0u);
+                        if (free_slots) ptx::mma_commit(bar(kBarEmpty + slot));
+                    }
+                    ptx::mma_commit(bar(kBarO + t));
+                };
+                while (ok && cur.next(p, it)) {
+                    if (it.nmax <= 0) continue;
+                    for (int t = 0; t < 2; ++t) {
+                        if (it.n[t] <= 0) continue;
+                        if (*abort_flag || !ptx::mbar_spin(bar(kBarQFull + t), qn[t] & 1, kErrWaitFull)) { ok = false; break; }
+                        ++qn[t];
+                        qk(t, 0, t == 1 || it.n[1] <= 0, it.n[t] == 1);
+                        if (!ok) break;
+                    }
+                    for (int j = 0; ok && j < it.nmax; ++j) {
+                        if (*abort_flag) { ok = false; break; }
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            if (j < it.n[t]) {
+                                // tile 1 reads last, where it reads at all
+                                pv(t, j, t == 1 || j >= it.n[1]);
+                                if (ok && j + 1 < it.n[t]) qk(t, j + 1, t == 1 || j + 1 >= it.n[1], j + 2 == it.n[t]);
+                            }
+                        }
+                    }
+                    at += it.nmax * kSlotsPerTile;
+                }
+                if (!ok) *abort_flag = 1;
+                // every MMA has retired before TMEM and shared memory go
+                ptx::mma_commit(bar(kBarDrain));
+                ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
+            }
+        } else if (warp == 2) {
+            // ------------------------------------------------------ V tail
+            // The rows of a sequence's last V tile past its end hold the next
+            // sequence's values, or none: P is 0 there, but 0 x NaN is not.  Such a
+            // tile lands on a barrier of this warp, which zeroes those rows and then
+            // completes the slots' own barriers.  Two barriers in turn: the producer
+            // may be one item ahead, but not two, as the ring does not hold the
+            // second's values before the first's are used.
+            uint32_t at = 0, tails = 0;
+            bool ok = true;
+            while (ok && cur.next(p, it)) {
+                if (it.nmax <= 0) continue;
+                const int left = it.s.lk - (it.nmax - 1) * kTileK;  // tokens in the last tile
+                if (left < kTileK) {
+                    const uint32_t k0 = at + (it.nmax - 1) * kSlotsPerTile + kKBlk;
+                    ok = wait_or_abort(bar(kBarTail + (tails & 1)), (tails >> 1) & 1, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    ++tails;
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        const int keep = min(max(left - c * kVHalf, 0), kVHalf);
+                        const uint32_t base = sbase + kOffRing + ((k0 + c) % kSlots) * kBox;
+                        // 16-byte pieces of rows keep.. of both 64-column boxes
+                        for (int q = lane; q < (kVHalf - keep) * 16; q += 32)
+                            ptx::st_shared_v4(base + ((q >> 3) & 1) * kVBox + (keep + (q >> 4)) * 128 + (q & 7) * 16, 0u, 0u, 0u, 0u);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane < 2) ptx::mbar_arrive(bar(kBarFull + (k0 + lane) % kSlots));
+                }
+                at += it.nmax * kSlotsPerTile;
+            }
+            if (!ok) *abort_flag = 1;
+        }
+    } else {
+        // ---------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        const int t = warp >= 8 ? 1 : 0;
+        const int r = tid - 128 - t * 128;  // row of the tile = TMEM lane
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + t * kTileK, o_addr = tmem + lanes + kTmemO + t * kV;
+        uint32_t sn = 0;  // S tiles so far (PV tile k completes phase k of kBarO)
+        bool ok = true;
+        const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+        while (ok && cur.next(p, it)) {
+            if (it.nmax < 0) continue;
+            const int row = it.row + t * kTileQ + r;
+            if (it.row + t * kTileQ >= it.s.lq) continue;
+            const int n = it.n[t];
+            // keys this row sees (rows past the sequence's end: like its last row)
+            int sees = it.s.lk;
+            if (p.causal) sees = min(sees, min(row, it.s.lq - 1) + 1 + it.s.lk - it.s.lq);
+            float m_used = -INFINITY, l_run = 0.f;
+            for (int j = 0; j < n; ++j, ++sn) {
+                ok = !*abort_flag && wait_bar(bar(kBarS + t), sn & 1, kErrWaitMma);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                uint32_t s[kTileK];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) ptx::tmem_ld_x32(s_addr + q * 32, *reinterpret_cast<uint32_t(*)[32]>(s + q * 32));
+                ptx::tmem_wait_ld();
+                const int valid = sees - j * kTileK;
+                if (valid < kTileK) {
+#pragma unroll
+                    for (int k = 0; k < kTileK; ++k)
+                        if (k >= valid) s[k] = tc::u32_of(-INFINITY);
+                }
+                float m8[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) m8[k] = tc::f32_of(s[k]);
+#pragma unroll
+                for (int k = 8; k < kTileK; ++k) m8[k & 7] = fmaxf(m8[k & 7], tc::f32_of(s[k]));
+                const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
+                float alpha = 1.f;
+                if (mx > m_used + kRescaleLog2) {
+                    alpha = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - mx);
+                    m_used = mx;
+                }
+                if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+                    ok = __all_sync(0xffffffffu, wait_bar(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < kV / 32; ++c) {
+                        uint32_t o[32];
+                        ptx::tmem_ld_x32(o_addr + c * 32, o);
+                        ptx::tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = tc::u32_of(tc::f32_of(o[k]) * alpha);
+                        ptx::tmem_st_x32(o_addr + c * 32, o);
+                    }
+                }
+                // (a row that has seen nothing keeps m_used = -inf: its weights are 0)
+                const float nm = m_used == -INFINITY ? 0.f : -m_used;
+                const float2 neg = make_float2(nm, nm);
+                float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        float2 x = make_float2(tc::f32_of(s[hf * 64 + 2 * k]), tc::f32_of(s[hf * 64 + 2 * k + 1]));
+                        x = fma2(x, sl2, neg);
+                        x.x = ptx::ex2(x.x);
+                        x.y = ptx::ex2(x.y);
+                        sum[k & 3] = add2(sum[k & 3], x);
+                        pk[k] = tc::pack2<kBf16>(x.x, x.y);
+                    }
+                    ptx::tmem_st_x32(s_addr + hf * 32, pk);
+                }
+                ptx::tmem_wait_st();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(bar(kBarP + t));
+                const float2 a = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                l_run = l_run * alpha + (a.x + a.y);
+            }
+            if (!ok) break;
+            // ------------------------------------------------------ epilogue
+            const bool real = row < it.s.lq;
+            const long long orow = (long long)(it.s.q0 + row) * p.heads + it.h;
+            uint8_t *dst = static_cast<uint8_t *>(p.out) + orow * (kV * 2);
+            const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+            if (n > 0) {
+                ok = __all_sync(0xffffffffu, wait_bar(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
+                if (!ok) break;
+                ptx::tc_fence_after();
+            }
+#pragma unroll 1
+            for (int c = 0; c < kV / 32; ++c) {
+                uint32_t o[32];
+                if (n > 0) {
+                    ptx::tmem_ld_x32(o_addr + c * 32, o);
+                    ptx::tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0u;
+                }
+                uint32_t w[2][8];
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                    w[k >> 3][k & 7] = tc::pack2<kBf16>(tc::f32_of(o[2 * k]) * inv, tc::f32_of(o[2 * k + 1]) * inv);
+                if (real) {
+                    store32(dst + c * 64, w[0]);
+                    store32(dst + c * 64 + 32, w[1]);
+                }
+            }
+            ptx::tc_fence_before();  // O is read before this thread's next P arrival lets a PV overwrite it
+            if (real && p.out_lse != nullptr)
+                p.out_lse[orow] = l_run > 0.f ? (m_used + __log2f(l_run)) * kLn2 : -INFINITY;
+        }
+        if (!ok) *abort_flag = 1;
+    }
+
+    ptx::tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (warp == 2) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+}  // namespace prefill
+}  // namespace mla

@@ -358,6 +358,47 @@ MLA_B200_API int mla_b200_decode_split_f16_noalloc(const void *query, const void
                                                    void *stream);
 
 /* ------------------------------------------------------------------------ */
+/* Attention over prompts, expanded form                                     */
+/* ------------------------------------------------------------------------ */
+
+/* Latent attention over prompts with the keys and values of each head at hand (no
+ * reference counterpart: it decodes one token):
+ *   s[h, i, j] = softmax_scale (q[i, h, 0:128] . k_nope[j, h] + q[i, h, 128:192] . k_rope[j])
+ *   out[i, h]  = softmax_j(s) v[j, h]
+ * query total_q tokens of [num_heads, 192]; k_nope and v total_k tokens of
+ * [num_heads, 128] (the two halves of one up-projection of the latent, by their
+ * strides); k_rope [total_k, 64], shared by the heads.  Strides are in elements, the
+ * innermost dimension is dense, and every base and stride a multiple of 16 bytes.
+ * Sequences are packed: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (device int32
+ * [batch + 1]; q and k alike or both NULL: dense, total = batch * max_seq_len).
+ * Lengths above max_seq_len_q / _k are cut to them.  causal != 0: query i of a
+ * sequence with Lq queries and Lk keys sees keys 0 .. i + Lk - Lq (the queries are the
+ * last Lq tokens: a chunk of a prompt sees what came before it).  Rows that see no
+ * key: out 0 and LSE -inf.  out [total_q, num_heads, 128] in the inputs' type, 32-byte
+ * aligned; out_lse [total_q, num_heads] fp32 natural log, or NULL.  Rows of query
+ * outside every sequence are not written.  Workspace (packed batches of two or more):
+ * mla_b200_workspace_size_prefill. */
+MLA_B200_API size_t mla_b200_workspace_size_prefill(int batch, long long total_q);
+MLA_B200_API int mla_b200_prefill_f16(const void *query, long long query_stride, long long query_head_stride,
+                                      const void *k_nope, long long k_stride, long long k_head_stride,
+                                      const void *k_rope, long long rope_stride, const void *v,
+                                      long long v_stride, long long v_head_stride,
+                                      const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
+                                      int num_heads, long long total_q, long long total_k,
+                                      int max_seq_len_q, int max_seq_len_k, int causal,
+                                      float softmax_scale, void *out, float *out_lse, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+MLA_B200_API int mla_b200_prefill_bf16(const void *query, long long query_stride, long long query_head_stride,
+                                      const void *k_nope, long long k_stride, long long k_head_stride,
+                                      const void *k_rope, long long rope_stride, const void *v,
+                                      long long v_stride, long long v_head_stride,
+                                      const int32_t *cu_seqlens_q, const int32_t *cu_seqlens_k, int batch,
+                                      int num_heads, long long total_q, long long total_k,
+                                      int max_seq_len_q, int max_seq_len_k, int causal,
+                                      float softmax_scale, void *out, float *out_lse, void *workspace,
+                                      size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Filling the paged latent cache                                            */
 /* ------------------------------------------------------------------------ */
 

@@ -70,3 +70,21 @@ def test_write_arguments():
         assert call(**bad) == capi.ERR_INVALID_ARG, bad
     if not torch.cuda.is_available():
         assert call() == capi.ERR_NO_DEVICE
+
+
+def test_prefill_arguments():
+    def call(**kw):
+        a = dict(q=16, qs=768, qh=192, k=16, ks=1024, kh=256, r=16, rs=64, v=16, vs=1024, vh=256, cuq=16, cuk=16, batch=2, heads=4, tq=100, tk=100,
+                 mq=64, mk=64, causal=1, scale=1.0, out=32, lse=None, ws=16, ws_bytes=1 << 20, stream=None)
+        a.update(kw)
+        return capi.lib().mla_b200_prefill_f16(*a.values())
+
+    for bad in [dict(q=None), dict(k=None), dict(r=None), dict(v=None), dict(out=None), dict(out=16), dict(q=24), dict(qs=764), dict(kh=4), dict(rs=60),
+                dict(vs=-8), dict(cuq=None), dict(cuk=None), dict(cuq=None, cuk=None), dict(batch=-1), dict(heads=0), dict(tq=-1), dict(tk=-1),
+                dict(mq=-1), dict(mk=-1), dict(scale=0.0), dict(scale=float("nan")), dict(lse=2)]:
+        assert call(**bad) == capi.ERR_INVALID_ARG, bad
+    assert call(tq=1 << 31) == capi.ERR_UNSUPPORTED and call(tk=1 << 31) == capi.ERR_UNSUPPORTED
+    if not torch.cuda.is_available():
+        assert call() == capi.ERR_NO_DEVICE
+    size = capi.lib().mla_b200_workspace_size_prefill
+    assert size(3, 1000) >= 8 * (1000 // 256 + 3) and size(-1, 5) == 0
