@@ -55,12 +55,20 @@ int cuda_failure(cudaError_t e) {
 
 // Opts a tensor-core kernel instantiation (both schedules) into its dynamic
 // shared memory.
-template <bool kBf16, bool kPaged, bool kFp8 = false, bool kMtp = false, bool kRows = false, bool kTree = false>
+template <bool kBf16, bool kPaged, bool kFp8 = false, bool kMtp = false, bool kRows = false>
 bool set_tc_smem() {
-    return cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedChunked, kBf16, kPaged, kFp8, kMtp, kRows, kTree>,
+    return cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedChunked, kBf16, kPaged, kFp8, kMtp, kRows>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSmemBytes) == cudaSuccess &&
-           cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedBalanced, kBf16, kPaged, kFp8, kMtp, kRows, kTree>,
+           cudaFuncSetAttribute(tc::tc_decode_kernel<kSchedBalanced, kBf16, kPaged, kFp8, kMtp, kRows>,
                                 cudaFuncAttributeMaxDynamicSharedMemorySize, tc::kSmemBytes) == cudaSuccess;
+}
+
+template <bool kBf16>
+bool set_tree_smem() {
+    return cudaFuncSetAttribute(tree::decode_kernel<kSchedChunked, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                tree::kSmemBytes) == cudaSuccess &&
+           cudaFuncSetAttribute(tree::decode_kernel<kSchedBalanced, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                tree::kSmemBytes) == cudaSuccess;
 }
 
 // Current device's properties (cached).  Returns a status.
@@ -119,8 +127,7 @@ int current_device(int *dev_out, DevInfo *info_out) {
             !set_tc_smem<false, false, true>() || !set_tc_smem<false, false, true, false, true>() ||
             !set_tc_smem<false, false, false, true>() ||
             !set_tc_smem<true, false, false, true>() ||
-            !set_tc_smem<false, true, false, false, false, true>() ||
-            !set_tc_smem<true, true, false, false, false, true>()) {
+            !set_tree_smem<false>() || !set_tree_smem<true>()) {
             return cuda_failure(cudaGetLastError());
         }
         cudaLaunchConfig_t cfg = {};
@@ -385,7 +392,7 @@ struct PagedArgs {
 
 // A tree of `drafts` draft tokens per sequence over a paged cache: `tiles` row tiles
 // of up to `tile_drafts` drafts of `heads` rows each per sequence, each tile a
-// sequence of the work list (tc::TcTreeParams).
+// sequence of the work list (tree::TreeParams).
 struct TreeArgs {
     const unsigned long long *mask;  // null: a chain
     int mask_stride;
@@ -425,13 +432,13 @@ void launch_tc(int clusters, const TcMaps &m, const tc::TcParams &tp, cudaStream
 }
 
 template <int kSched, bool kBf16>
-void launch_tc_tree(int clusters, const TcMaps &m, const tc::TcTreeParams &tp, cudaStream_t stream) {
-    launch_dependent(tc::tc_decode_kernel<kSched, kBf16, true, false, false, false, true>, dim3(2 * clusters),
-                     dim3(tc::kThreads), tc::kSmemBytes, stream, true, m.cmap_s, m.cmap_o, m.qmap, tp);
+void launch_tree(int clusters, const TcMaps &m, const tree::TreeParams &tp, cudaStream_t stream) {
+    launch_dependent(tree::decode_kernel<kSched, kBf16>, dim3(2 * clusters), dim3(tree::kThreads), tree::kSmemBytes,
+                     stream, true, m.cmap_s, m.cmap_o, m.qmap, tp);
 }
 
 template <typename OutT>
-void launch_tree_merge(const WsLayout &L, const WorkList &wl, const tc::TcTreeParams &tp, void *out, float *out_lse,
+void launch_tree_merge(const WsLayout &L, const WorkList &wl, const tree::TreeParams &tp, void *out, float *out_lse,
                        cudaStream_t stream, bool chain) {
     // a few tiles have many splits each: a block of 8 warps per row; many tiles have
     // one or two: a warp per row
@@ -503,7 +510,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
     if (max_items > (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
     WsLayout L = ws_layout(workspace, max_items, num_heads, batch, f8 != nullptr, tr != nullptr);
     if (workspace == nullptr || workspace_bytes < L.bytes) return MLA_B200_ERR_WORKSPACE;
-    if (!aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
+    if (!aligned(workspace, tr != nullptr ? 32 : 16)) return MLA_B200_ERR_INVALID_ARG;
     const int32_t *seq_lens = nullptr;
     if (pg != nullptr) {
         seq_lens = pg->seq_lens;
@@ -515,6 +522,19 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
     wl.chunk = balanced ? 0 : chunk;
     wl.item_cost = item_cost_for(num_heads);
     wl.group = group;
+    tree::TreeParams tree_p{};
+    TreePlan tree_plan{};
+    if (tr != nullptr) {
+        tree_p.num_heads = num_heads;
+        tree_p.mask = tr->mask;
+        tree_p.seen = L.tree_seen;
+        tree_p.mask_stride = tr->mask_stride;
+        tree_p.drafts = tr->drafts;
+        tree_p.heads = tr->heads;
+        tree_p.tiles = tr->tiles;
+        tree_p.tile_drafts = tr->tile_drafts;
+        tree_plan = {tr->mask, tr->mask_stride, tr->drafts, tr->tiles, tr->tile_drafts, L.tree_seen};
+    }
     const bool planned = cu_seqlens != nullptr || virt;  // a plan kernel precedes the decode
     int bal_clusters = 0;      // balanced: clusters to launch
     bool bal_split = true;     // balanced: some sequence has more than one item
@@ -544,8 +564,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             wl.nworkers = info.tc_clusters;
             bal_clusters = info.tc_clusters;
             plan_balanced_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, wl.item_cost, L.item_off, seq_lens,
-                                                         max_seq_len, L.cu_virtual, group, max_seq_len,
-                                                         tr != nullptr ? tr->tiles : 1);
+                                                         max_seq_len, L.cu_virtual, group, max_seq_len, tree_plan);
         }
     } else if (!planned) {
         wl.items = nullptr;
@@ -562,20 +581,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
         wl.cu_seqlens = cu_seqlens;  // read by the paged kernel
         plan_varlen_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, chunk, L.item_off, L.items,
                                                    (int)max_items, seq_lens, max_seq_len, L.cu_virtual,
-                                                   group, max_seq_len, tr != nullptr ? tr->tiles : 1);
-    }
-    tc::TcTreeParams tree_p{};
-    if (tr != nullptr) {
-        tree_p.num_heads = num_heads;
-        tree_p.mask = tr->mask;
-        tree_p.seen = L.tree_seen;
-        tree_p.mask_stride = tr->mask_stride;
-        tree_p.drafts = tr->drafts;
-        tree_p.heads = tr->heads;
-        tree_p.tiles = tr->tiles;
-        tree_p.tile_drafts = tr->tile_drafts;
-        tree::seen_kernel<<<(unsigned)cdiv(batch, 256), 256, 0, stream>>>(
-            tr->mask, tr->mask_stride, tr->drafts, tr->tiles, tr->tile_drafts, batch, L.tree_seen);
+                                                   group, max_seq_len, tree_plan);
     }
     bool tc_direct = false;  // the tcgen05 kernel wrote single-item sequences itself
     // A few long sequences chain decode -> merge -> next decode with programmatic
@@ -654,10 +660,20 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             const int clusters = balanced ? bal_clusters : std::min(info.tc_clusters, wl.max_items);
             timing_mark(t_ev_start, stream);
             if (tr != nullptr) {
-                static_cast<tc::TcParams &>(tree_p) = tp;
-                tree_p.part_kind = tc::kOutF32;  // tree::merge_kernel
-                if (balanced) launch_tc_tree<kSchedBalanced, kBf16>(clusters, maps, tree_p, stream);
-                else launch_tc_tree<kSchedChunked, kBf16>(clusters, maps, tree_p, stream);
+                tree_p.wl = wl;
+                tree_p.scale_log2 = tp.scale_log2;
+                tree_p.part_o = L.part_o;
+                tree_p.part_lse = L.part_lse;
+                tree_p.out = out;
+                tree_p.out_kind = tp.out_kind;
+                tree_p.out_lse = out_lse;
+                tree_p.chain = tp.chain;
+                tree_p.block_table = tp.block_table;
+                tree_p.max_blocks = tp.max_blocks;
+                tree_p.page_size = tp.page_size;
+                tree_p.num_pages = pg != nullptr ? (int)(pg->pool_rows / pg->page_size) : 0;
+                if (balanced) launch_tree<kSchedBalanced, kBf16>(clusters, maps, tree_p, stream);
+                else launch_tree<kSchedChunked, kBf16>(clusters, maps, tree_p, stream);
             } else if (mtp != nullptr) {
                 if (balanced) launch_tc<kSchedBalanced, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
                 else launch_tc<kSchedChunked, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
@@ -690,7 +706,6 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
         }
     }
     if (tr != nullptr) {
-        tree_p.num_heads = num_heads;
         if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(L, wl, tree_p, out, out_lse, stream, chain);
         else if constexpr (kBf16) launch_tree_merge<__nv_bfloat16>(L, wl, tree_p, out, out_lse, stream, chain);
         else if constexpr (!std::is_same<T, float>::value) launch_tree_merge<__half>(L, wl, tree_p, out, out_lse, stream, chain);
@@ -881,7 +896,7 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
               : (out_dtype != MLA_B200_OUT_F16 && out_dtype != MLA_B200_OUT_F32))
         return MLA_B200_ERR_INVALID_ARG;
     if (!(softmax_scale > 0.f) || !isfinite(softmax_scale)) return MLA_B200_ERR_INVALID_ARG;
-    if (!aligned(query, 16) || !aligned(kv_pages, 16) || !aligned(out, 16) || !aligned(out_lse, 4) ||
+    if (!aligned(query, 16) || !aligned(kv_pages, 16) || !aligned(out, 32) || !aligned(out_lse, 4) ||
         !aligned(block_table, 4) || !aligned(seq_lens, 4) || !aligned(mask, 8))
         return MLA_B200_ERR_INVALID_ARG;
     if (drafts > 64 || heads > 128 || page_size % tc::kTO != 0) return MLA_B200_ERR_UNSUPPORTED;

@@ -308,6 +308,26 @@ __device__ void lens_to_offsets(const int32_t *lens, int batch, int max_len, int
     __syncthreads();
 }
 
+// Draft trees: seen[v] = the drafts that some draft of row tile v sees (tc_decode_kernel,
+// TcTreeParams); mask null: a chain, draft i sees drafts 0..i.  `tiles` row tiles share
+// a sequence; tiles 0: no trees.
+struct TreePlan {
+    const unsigned long long *mask;
+    int mask_stride, drafts, tiles, tile_drafts;
+    unsigned long long *seen;
+};
+
+__device__ __forceinline__ void plan_tree(const TreePlan &t, int v) {
+    if (t.tiles == 0) return;
+    const int b = v / t.tiles, d0 = (v - b * t.tiles) * t.tile_drafts;
+    const int d1 = min(d0 + t.tile_drafts, t.drafts);
+    unsigned long long m = 0;
+    if (t.mask == nullptr) m = (2ull << (d1 - 1)) - 1;
+    else
+        for (int d = d0; d < d1; ++d) m |= t.mask[(long long)b * t.mask_stride + d];
+    t.seen[v] = t.drafts < 64 ? m & ((1ull << t.drafts) - 1) : m;
+}
+
 // Expands cu_seqlens[B+1] into item_off[B+1] (exclusive prefix of per-sequence
 // item counts) and items[] = {b, row_begin, row_end, token offset in the
 // sequence}.  One block.  With
@@ -322,13 +342,13 @@ __global__ void __launch_bounds__(1024) plan_varlen_kernel(const int32_t *cu_seq
                                                            int max_len = 0,
                                                            int32_t *cu_out = nullptr,
                                                            int group = 1, int dense_len = 0,
-                                                             int share = 1) {
+                                                             TreePlan tree = {}) {
     __shared__ int warp_tot[32];
     __shared__ int carry_s;
     griddep_launch();  // the decode kernel may start its set-up now
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (seq_lens != nullptr) {
-        lens_to_offsets(seq_lens, batch, max_len, cu_out, share);
+        lens_to_offsets(seq_lens, batch, max_len, cu_out, max(tree.tiles, 1));
         cu_seqlens = cu_out;
     }
     if (tid == 0) carry_s = 0;
@@ -337,6 +357,7 @@ __global__ void __launch_bounds__(1024) plan_varlen_kernel(const int32_t *cu_seq
         const int b = base + tid;
         int cnt = 0;
         if (b < batch) {
+            plan_tree(tree, b);
             const int len = seq_len_of(cu_seqlens, dense_len, group, b);
             cnt = len > 0 ? (len + chunk - 1) / chunk : 0;
         }
@@ -387,13 +408,13 @@ __global__ void __launch_bounds__(1024) plan_balanced_kernel(const int32_t *cu_s
                                                              int max_len = 0,
                                                              int32_t *cu_out = nullptr,
                                                              int group = 1, int dense_len = 0,
-                                                             int share = 1) {
+                                                             TreePlan tree = {}) {
     __shared__ int warp_tot[32];
     __shared__ int carry_s;
     griddep_launch();  // the decode kernel may start its set-up now
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (seq_lens != nullptr) {
-        lens_to_offsets(seq_lens, batch, max_len, cu_out, share);
+        lens_to_offsets(seq_lens, batch, max_len, cu_out, max(tree.tiles, 1));
         cu_seqlens = cu_out;
     }
     if (tid == 0) carry_s = 0;
@@ -402,6 +423,7 @@ __global__ void __launch_bounds__(1024) plan_balanced_kernel(const int32_t *cu_s
         const int b = base + tid;
         int cost = 0;
         if (b < batch) {
+            plan_tree(tree, b);
             const int len = seq_len_of(cu_seqlens, dense_len, group, b);
             cost = len > 0 ? (len + kTile - 1) / kTile + item_cost : 0;
         }

@@ -46,8 +46,6 @@
 // tensor work as 128.
 #pragma once
 
-#include <type_traits>
-
 #include "mla_tc_ptx.cuh"
 
 namespace mla {
@@ -210,45 +208,6 @@ struct TcParams {
     };
 };
 
-// Draft-tree decode (kTree): the drafts of a sequence fill one or more 128-row
-// tiles of whole drafts; "sequence" v of the work list is tile v % tiles of real
-// sequence v / tiles, `tile_drafts` drafts of `heads` rows each (the last tile may
-// hold fewer), and reads the real sequence's pages.
-struct TcTreeParams : TcParams {
-    const unsigned long long *mask;   // [batch or 1, drafts]: bit j of draft i's word = i sees draft j; null: a chain
-    const unsigned long long *seen;   // [batch * tiles]: the drafts that some draft of the tile sees
-    int mask_stride;                  // words from one sequence's masks to the next: drafts, or 0 (shared)
-    int drafts, heads, tiles, tile_drafts;
-};
-
-// Rows of query, output and LSE before tile v, and the rows it has.
-__device__ __forceinline__ void tree_rows(const TcTreeParams &p, int v, long long &row0, int &rows) {
-    const int b = v / p.tiles, d0 = (v - b * p.tiles) * p.tile_drafts;
-    row0 = ((long long)b * p.drafts + d0) * p.heads;
-    rows = min(p.tile_drafts, p.drafts - d0) * p.heads;
-}
-
-// Which of the 32 tokens [t, t + 32) a row sees whose drafts start at token
-// `start`: all before `start`, then the bits of `mask` (no bits at or past the
-// number of drafts), none after.
-__device__ __forceinline__ uint32_t tree_word(unsigned long long mask, int start, int t) {
-    const int s = start - t;
-    if (s >= 32) return 0xffffffffu;
-    if (s >= 0) return ((1u << s) - 1u) | (uint32_t)(mask << s);
-    return s > -64 ? (uint32_t)(mask >> -s) : 0u;
-}
-
-// Zeroes the rows of a landed [32 x 512] C tile whose bit of `keep` is clear (see
-// zero_tail).
-__device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t keep, int lane) {
-    for (int q = lane; q < kTO * kVBlocks * 8; q += 32) {
-        const int row = q >> 6;
-        if (!((keep >> row) & 1u))
-            ptx::st_shared_v4(tile + ((q >> 3) & (kVBlocks - 1)) * kBoxO + row * 128 + (q & 7) * 16, 0u, 0u, 0u, 0u);
-    }
-    ptx::fence_proxy_async_smem();
-}
-
 // Zeroes rows [tail, 32) of a landed [32 x 512] C tile (8 SW128 K-blocks of
 // 32 rows; whole 128-byte rows, so the swizzle does not matter), this lane's
 // share of a warp's work, and orders the stores before the tensor core's
@@ -396,13 +355,11 @@ struct Ring {
 // (hi plane, then lo plane), box 64 x 128, SW64.  kRows (with kFp8): one
 // dequantisation scale per cache row, p.kv_scales; a separate instantiation
 // because the per-row code slowed the per-tensor kernel by ~10 %.
-// kTree (with kPaged): draft trees, TcTreeParams.
-template <int kSched, bool kBf16, bool kPaged, bool kFp8, bool kMtp = false, bool kRows = false, bool kTree = false>
+template <int kSched, bool kBf16, bool kPaged, bool kFp8, bool kMtp = false, bool kRows = false>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tc_decode_kernel(const __grid_constant__ CUtensorMap cmap_s,
                      const __grid_constant__ CUtensorMap cmap_o,
-                     const __grid_constant__ CUtensorMap qmap,
-                     const std::conditional_t<kTree, TcTreeParams, TcParams> p) {
+                     const __grid_constant__ CUtensorMap qmap, const TcParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = ptx::smem_u32(smem);
@@ -480,13 +437,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 // of the next tile's, read a tile ahead so the block-table
                 // latency stays off the refill path (the first tile's overlaps
                 // the Q loads)
-                int last = 0, real_b = 0, pr[kOPerS], pn[kOPerS];
+                int last = 0, pr[kOPerS], pn[kOPerS];
                 if constexpr (kPaged) {
                     last = it.tok0 + it.len - 1;
-                    if constexpr (kTree) real_b = it.b / p.tiles;
-                    else real_b = it.b;
 #pragma unroll
-                    for (int c = 0; c < kOPerS; ++c) pr[c] = paged_row(p, real_b, it.tok0 + c * kTO, last);
+                    for (int c = 0; c < kOPerS; ++c) pr[c] = paged_row(p, it.b, it.tok0 + c * kTO, last);
                 }
                 if (kFp8 && role == 0 && it.b != prev_b) {
                     // Q8 of the new sequence: hi and lo boxes of one K-block per slot
@@ -502,13 +457,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     prev_b = it.b;
                 } else if (role == 0 && it.b != prev_b) {
                     // Q of the new sequence: two 128 x 64 boxes per ring slot
-                    int qrow = it.b * p.num_heads;
-                    if constexpr (kTree) {
-                        long long r0;
-                        int rows;
-                        tree_rows(p, it.b, r0, rows);
-                        qrow = (int)r0;
-                    }
+                    const int qrow = it.b * p.num_heads;
                     for (int kb = 0; kb < kKBlocks; kb += 2) {
                         if (!acquire()) { ok = false; break; }
                         const int nb = min(2, kKBlocks - kb);
@@ -524,7 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     const int row = (int)(it.row0 + t0);
                     if constexpr (kPaged) {
 #pragma unroll
-                        for (int c = 0; c < kOPerS; ++c) pn[c] = paged_row(p, real_b, it.tok0 + t0 + kTS + c * kTO, last);
+                        for (int c = 0; c < kOPerS; ++c) pn[c] = paged_row(p, it.b, it.tok0 + t0 + kTS + c * kTO, last);
                     }
                     if (role == 0) {
                         if constexpr (kPaged) {
@@ -707,25 +656,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 // boundaries, so this is a sequence's end; elsewhere it would
                                 // only zero rows whose P is 0.
                                 const int tail = (it.len - t0) % kTO;
-                                if constexpr (kTree) {
-                                    // the rows past the sequence's end, and those of drafts that no
-                                    // draft of this tile sees (a padded draft's row may be unwritten)
-                                    const int start = wl.cu_seqlens[it.b + 1] - wl.cu_seqlens[it.b] - p.drafts;
-                                    const int t = it.tok0 + t0 + ct * kTO;
-                                    if (t + kTO > start) {
-                                        const uint32_t keep = tree_word(p.seen[it.b], start, t);
-                                        if (keep != 0xffffffffu) {
-                                            volatile int *za = reinterpret_cast<volatile int *>(smem + kOffZArg);
-                                            const uint32_t tile = sbase + kOffRing + rg.slot * kSlotO;
-                                            za[0] = (int)tile;
-                                            za[1] = (int)keep;
-                                            __syncwarp();
-                                            zero_rows(tile, keep, 0);
-                                            __syncwarp();
-                                            ptx::tc_fence_after();
-                                        }
-                                    }
-                                } else if (ct == nct - 1 && t0 + kTS >= it.len && tail != 0) {
+                                if (ct == nct - 1 && t0 + kTS >= it.len && tail != 0) {
                                     volatile int *za = reinterpret_cast<volatile int *>(smem + kOffZArg);
                                     const uint32_t tile = sbase + kOffRing + rg.slot * kSlotO;
                                     za[0] = (int)tile;
@@ -791,8 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (;;) {
                 __syncwarp();
                 if (za[2] != 0) break;
-                if constexpr (kTree) zero_rows((uint32_t)za[0], (uint32_t)za[1], lane);
-                else zero_tail((uint32_t)za[0], za[1], lane);
+                zero_tail((uint32_t)za[0], za[1], lane);
                 __syncwarp();
             }
         }
@@ -835,16 +765,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     const int slen = wl.cu_seqlens != nullptr ? wl.cu_seqlens[it.b + 1] - wl.cu_seqlens[it.b]
                                                               : wl.seq_len;
                     lim = slen - (mk - 1 - tok) - it.tok0;
-                }
-                // draft tree: the drafts this row sees, and where they start in the item
-                unsigned long long tmask = 0;
-                int tstart = 0;
-                if constexpr (kTree) {
-                    const int b = it.b / p.tiles;
-                    const int d = min((it.b - b * p.tiles) * p.tile_drafts + h / p.heads, p.drafts - 1);
-                    tmask = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
-                    if (p.drafts < 64) tmask &= (1ull << p.drafts) - 1;
-                    tstart = wl.cu_seqlens[it.b + 1] - wl.cu_seqlens[it.b] - p.drafts - it.tok0;
                 }
                 for (int t0 = 0; t0 < it.len; t0 += kTS, ++jt) {
                     const uint32_t sb = jt & 1, use = jt >> 1;
@@ -897,17 +817,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             for (int k = 0; k < kTS; ++k)
                                 if (k >= valid) r[k] = u32_of(-INFINITY);
                         }
-                        if constexpr (kTree) {
-                            if (t0 + kTS > tstart) {  // the tile reaches into the drafts
-#pragma unroll
-                                for (int q = 0; q < kTS / 32; ++q) {
-                                    const uint32_t see = tree_word(tmask, tstart, t0 + q * 32);
-#pragma unroll
-                                    for (int k = 0; k < 32; ++k)
-                                        if (!((see >> k) & 1u)) r[q * 32 + k] = u32_of(-INFINITY);
-                                }
-                            }
-                        }
                         float m8[8];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) m8[j] = f32_of(r[j]);
@@ -921,7 +830,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         }
                         // p = 2^(s * scale_log2 - m_used): one FFMA + one EX2 per logit.
                         // (a row that has seen nothing yet keeps m_used = -inf: its p are 0)
-                        const float neg_m = ((kMtp || kTree) && m_used == -INFINITY) ? 0.f : -m_used;
+                        const float neg_m = (kMtp && m_used == -INFINITY) ? 0.f : -m_used;
                         float s4[4] = {0.f, 0.f, 0.f, 0.f};
                         if constexpr (kFp8) {
                             // the per-row branch outside the unrolled loops (two copies)
@@ -1074,12 +983,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         const size_t row_bytes = (size_t)kDV * (f16 ? 2 : 4);
                         uint8_t *dst = single ? static_cast<uint8_t *>(p.out) + (size_t)it.b * p.num_heads * row_bytes
                                               : static_cast<uint8_t *>(p.part_o) + (size_t)i * p.num_heads * row_bytes;
-                        int nrows = p.num_heads;
-                        long long lse_row = (long long)it.b * p.num_heads;
-                        if constexpr (kTree) {
-                            tree_rows(p, it.b, lse_row, nrows);
-                            if (single) dst = static_cast<uint8_t *>(p.out) + (size_t)lse_row * row_bytes;
-                        }
                         // Each pass moves a 128-byte segment of every row (64 fp16 or 32 fp32
                         // columns) through a per-warp swizzled 32-row staging tile, so that
                         // each store instruction covers 4 rows x 128 contiguous bytes.  (One
@@ -1125,13 +1028,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int k = 0; k < 8; ++k) {
                                 const int head = row0 + 4 * k + rr;
-                                if (head < nrows)
+                                if (head < p.num_heads)
                                     *reinterpret_cast<uint4 *>(dst + head * row_bytes + c * 128 + qq * 16) = v[k];
                             }
                         }
-                        if (h < nrows) {
+                        if (h < p.num_heads) {
                             if (single) {
-                                if (p.out_lse != nullptr) p.out_lse[lse_row + h] = lse;
+                                if (p.out_lse != nullptr) p.out_lse[(size_t)it.b * p.num_heads + h] = lse;
                             } else {
                                 p.part_lse[(size_t)i * p.num_heads + h] = lse;
                             }

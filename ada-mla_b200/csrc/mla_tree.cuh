@@ -1,5 +1,39 @@
-// mla_tree.cuh -- the kernels around the draft-tree decode (tc::tc_decode_kernel
-// with kTree): the drafts each row tile sees, and the merge of its split partials.
+// mla_tree.cuh -- attention of a tree of drafted tokens over the paged latent cache.
+//
+//   O[b, i, h] = softmax(scale Q*[b, i, h] . C_b^T + M[b, i]) . C_b[:, :512]
+//
+// for drafts i < k of sequence b, whose own rows are the last k of C_b: M hides draft
+// row j from draft i unless bit j of i's mask is set, and nothing else.
+//
+// (draft, head) rows fill tiles of 128 rows: as many whole drafts as fit, dealt
+// evenly over a sequence's tiles.  A tile is a "sequence" of the work list (WorkList:
+// split by cost over the clusters, partials merged below), and reads its sequence's
+// pages once.  Per cached token a tile needs 1152 bytes and 2 x 128 x (576 + 512)
+// flop, so one tile is bound by HBM (1152 B / 6.5 TB/s over 74 clusters = 13 ns) about
+// as much as by the tensor cores (12.6 ns); a sequence's further tiles find its rows in
+// L2.
+//
+// The two products do not fit one SM's TMEM (O alone is all of it), so a tile runs on
+// a cluster of two, as in the decode of one token per sequence (tc_decode_kernel): the
+// S-CTA keeps Q in TMEM, computes S = Q C^T for 96 tokens at a time and the softmax,
+// and sends P to the O-CTA, which accumulates O += P C_N.  Different here:
+//
+//   * the softmax of a tile is shared by two warpgroups, 48 columns each: with one,
+//     its 1.2 us a tile were longer than everything else on the S-CTA.  They exchange
+//     row maxima in shared memory; one barrier serves the exchange, the staging
+//     buffer and errors, a second one precedes the message;
+//   * the producer warp holds the block-table entries of ten tiles (30 pieces of 32
+//     rows), a lane each, and loads the next ten ahead;
+//   * rows of a C tile that no draft of the tile may see (past the sequence's end, or
+//     padded drafts that may never have been written) are zeroed by a warp of their own
+//     before GEMM2 (0 x NaN is not 0): such tiles land on that warp's barrier, which
+//     then completes the slot's.  No other tile pays for it;
+//   * partials are fp32: a 16-bit partial would add a third rounding of the size of
+//     the output's own.
+//
+// Roles (384 threads): warp 0 TMA producer, warps 1 and 3 MMA issuers (GEMM1 alternates
+// between them; GEMM2 has one), warp 2 TMEM owner and (O-CTA) row zeroing, warps 4-11
+// math: thread h of each warpgroup owns row h.  Every wait is bounded.
 #pragma once
 
 #include "mla_combine.cuh"
@@ -8,24 +42,623 @@
 namespace mla {
 namespace tree {
 
-constexpr int kMergeWarps = 8;  // warps of a merge block
+using tc::kBoxO;
+using tc::kBoxS;
+using tc::kKBlocks;
+using tc::kKbPerSlot;
+using tc::kOPerS;
+using tc::kPieceS;
+using tc::kQBoxBytes;
+using tc::kQSlots;
+using tc::kSlotO;
+using tc::kSlotS;
+using tc::kSlotsO;
+using tc::kSlotsPerTile;
+using tc::kSlotsS;
+using tc::kSubP;
+using tc::kTO;
+using tc::kTS;
+using tc::kVBlocks;
 
-// seen[v] = the drafts that some draft of row tile v sees (bits at and past
-// `drafts` clear); mask null: a chain, draft i sees drafts 0..i.  A thread per tile.
-__global__ void __launch_bounds__(256) seen_kernel(const unsigned long long *__restrict__ mask, int mask_stride,
-                                                   int drafts, int tiles, int tile_drafts, int ntiles,
-                                                   unsigned long long *__restrict__ seen) {
-    griddep_launch();
-    griddep_wait();
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= ntiles) return;
-    const int b = v / tiles, d0 = (v - b * tiles) * tile_drafts;
-    const int d1 = min(d0 + tile_drafts, drafts);
-    unsigned long long m = 0;
-    if (mask == nullptr) m = (2ull << (d1 - 1)) - 1;
-    else
-        for (int d = d0; d < d1; ++d) m |= mask[(long long)b * mask_stride + d];
-    seen[v] = drafts < 64 ? m & ((1ull << drafts) - 1) : m;
+constexpr int kThreads = 384;
+constexpr int kMath = 256;        // threads of the two math warpgroups
+constexpr int kHalf = kTS / 2;    // columns of one warpgroup
+constexpr int kRowTiles = 10;     // tiles whose block-table entries the producer warp holds
+constexpr int kMergeWarps = 8;    // warps of a merge block
+constexpr uint64_t kTailWaitNs = 20000000000ull;  // the zeroing warp waits through whole items
+
+// Message S-CTA -> O-CTA, one per S tile: P as three SW64 K-major sub-tiles of [128
+// rows x 32 tokens], then per row alpha, the two warpgroups' sums, m.
+constexpr int kMsgP = kOPerS * kSubP;          // 24576
+constexpr int kMsgAlpha = kMsgP;
+constexpr int kMsgL = kMsgP + 512;             // [2][128]
+constexpr int kMsgM = kMsgP + 1536;
+constexpr int kMsgBytes = kMsgP + 2048;        // 26624
+constexpr int kMsgSlots = 3;
+
+enum BarId {
+    kBarFull = 0,                       // ring slot landed (and its hidden rows zeroed)
+    kBarEmpty = kSlotsS,                // ring slot consumed
+    kBarSFull = 2 * kSlotsS,            // [2] S-CTA: S tile in TMEM
+    kBarSEmpty = kBarSFull + 2,         // [2] S-CTA: S tile read (256)
+    kBarQFree = kBarSEmpty + 2,         // [2] S-CTA: an issuer's GEMM1s reading Q done
+    kBarQReady = kBarQFree + 2,         //     S-CTA: a tile's Q copied into TMEM
+    kBarPFree = kBarQReady + 1,         // [3] GEMM2 done with a message slot (in both CTAs)
+    kBarPFull = kBarPFree + kMsgSlots,  // [3] O-CTA: message landed
+    kBarCorr = kBarPFull + kMsgSlots,   // [3] O-CTA: O ready for GEMM2 (256)
+    kBarMmaDone = kBarCorr + kMsgSlots, // [3] O-CTA: GEMM2 of a message done
+    kBarTail = kBarMmaDone + kMsgSlots, // [4] O-CTA: slot landed, hidden rows not yet zeroed
+    kBarDrain = kBarTail + kSlotsO,     // [2] an issuer's operations retired
+    kNumBars = kBarDrain + 2
+};
+static_assert(kSlotsS >= kSlotsO, "ring barriers");
+
+constexpr int kOffRing = 0;
+constexpr int kOffStg = kSlotsS * kSlotS;                   // S-CTA: message staging
+constexpr int kOffMsg = kSlotsO * kSlotO;                   // O-CTA: received messages [3]
+constexpr int kOffBar = kOffStg + kMsgBytes;
+static_assert(kOffMsg + kMsgSlots * kMsgBytes <= kOffBar, "O-CTA layout");
+static_assert(kMsgBytes % 1024 == 0, "swizzle atoms of the message slots");
+constexpr int kOffSlot = kOffBar + kNumBars * 8;
+constexpr int kOffAbort = kOffSlot + 4;
+constexpr int kOffMax = (kOffAbort + 4 + 15) / 16 * 16;     // S-CTA: row maxima [2 tiles][2 halves][128]
+constexpr int kSmemBytes = kOffMax + 2 * 2 * 128 * 4 + 1024;
+static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
+constexpr uint32_t kTmemCols = 512, kTmemQ = 0, kTmemS = 288;
+
+struct TreeParams {
+    WorkList wl;
+    int num_heads;     // rows of a full tile = rows between partials: tile_drafts * heads
+    float scale_log2;  // softmax scale * log2(e)
+    float *part_o;     // [items, num_heads, 512]
+    float *part_lse;   // [items, num_heads]
+    void *out;         // [batch, drafts, heads, 512]: written directly for tiles of one item
+    int out_kind;      // tc::OutKind
+    float *out_lse;    // [batch, drafts, heads] or null
+    int chain;         // the merge after this launch is a programmatic dependent
+    const int32_t *block_table;
+    int max_blocks, page_size, num_pages;
+    const unsigned long long *mask;   // [batch or 1, drafts]; null: a chain
+    const unsigned long long *seen;   // [tiles of all sequences] (TreePlan)
+    int mask_stride;                  // drafts, or 0 (one mask for all)
+    int drafts, heads, tiles, tile_drafts;
+};
+
+// Rows of query, output and LSE before tile v, and the rows it has.
+__device__ __forceinline__ void tree_rows(const TreeParams &p, int v, long long &row0, int &rows) {
+    const int b = v / p.tiles, d0 = (v - b * p.tiles) * p.tile_drafts;
+    row0 = ((long long)b * p.drafts + d0) * p.heads;
+    rows = min(p.tile_drafts, p.drafts - d0) * p.heads;
+}
+
+// Which of the 32 tokens [t, t + 32) a row sees whose drafts start at token `start`:
+// all before `start`, then the bits of `mask` (clear at and past the number of
+// drafts), so none past the sequence's end.
+__device__ __forceinline__ uint32_t tree_word(unsigned long long mask, int start, int t) {
+    const int s = start - t;
+    if (s >= 32) return 0xffffffffu;
+    if (s >= 0) return ((1u << s) - 1u) | (uint32_t)(mask << s);
+    return s > -64 ? (uint32_t)(mask >> -s) : 0u;
+}
+
+// First token of the drafts of tile v's sequence (below 0 when it is shorter).
+__device__ __forceinline__ int draft_start(const TreeParams &p, int v) {
+    return p.wl.cu_seqlens[v + 1] - p.wl.cu_seqlens[v] - p.drafts;
+}
+
+// Pool row of the 32-row piece at token t of sequence b; pieces past the item's last
+// token re-read its last piece (the softmax hides them).
+__device__ __forceinline__ int pool_row(const TreeParams &p, int b, int t, int last) {
+    const int tc = min(t, last & ~(kTO - 1));
+    const int blk = tc / p.page_size;
+    // (an entry that is no page: the row after the pool, which TMA reads as zeros)
+    const int pg = (int)min((unsigned)p.block_table[(long long)b * p.max_blocks + blk], (unsigned)p.num_pages);
+    return pg * p.page_size + (tc - blk * p.page_size);
+}
+
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void store32(void *dst, const uint32_t *v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
+                 "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
+// cmap_s: the pool as (64, 8 rows, 9 K-blocks, row groups), one box = 3 K-blocks x 32
+// rows, three boxes to a ring slot (its K-blocks interleaved per 8-row group); cmap_o:
+// the pool as (64, rows, 9), one box = 8 K-blocks x 32 rows; qmap: the queries
+// [batch * drafts * heads, 576], box 64 x 128.  128-byte swizzle.
+template <int kSched, bool kBf16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap cmap_s, const __grid_constant__ CUtensorMap cmap_o,
+                  const __grid_constant__ CUtensorMap qmap, const TreeParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = ptx::smem_u32(smem);
+    auto bar = [&](int id) -> uint32_t { return sbase + kOffBar + 8u * id; };
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + kOffAbort);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t role = ptx::cluster_ctarank();  // 0 = S-CTA, 1 = O-CTA
+    const int cid = (int)ptx::cluster_id_x(), ncl = (int)ptx::nclusters_x();
+
+    if (tid == 0) {
+        for (int i = 0; i < kNumBars; ++i) {
+            const bool math = (i >= kBarSEmpty && i < kBarSEmpty + 2) || (i >= kBarCorr && i < kBarCorr + kMsgSlots);
+            ptx::mbar_init(bar(i), math ? kMath : 1);
+        }
+        *abort_flag = 0;
+        ptx::fence_mbarrier_init_cluster();
+    }
+    if (warp == 0 && lane == 0) {
+        ptx::tma_prefetch_desc(role == 0 ? &cmap_s : &cmap_o);
+        if (role == 0) ptx::tma_prefetch_desc(&qmap);
+    }
+    if (warp == 2) {
+        ptx::tmem_alloc(sbase + kOffSlot, kTmemCols);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    ptx::cluster_sync();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + kOffSlot);
+    if (p.chain) griddep_launch();  // the chained merge may place its CTAs
+    griddep_wait();                 // the plan kernel's work list
+    const WorkList &wl = p.wl;
+    ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
+    Item it;
+    int id;
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA producer
+        // The whole warp walks the items; lane 0 loads.
+        const int nslots = role == 0 ? kSlotsS : kSlotsO;
+        tc::Ring rg;
+        int prev_b = -1;
+        bool ok = true;
+        auto acquire = [&]() -> bool {
+            return !*abort_flag && ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
+        };
+        while (ok && items_next<kSched>(wl, cur, it, id)) {
+            const int b = it.b / p.tiles, last = it.tok0 + it.len - 1;
+            auto rows_from = [&](int piece) -> int {  // this lane's piece of ten tiles
+                return pool_row(p, b, it.tok0 + (piece + min(lane, kRowTiles * kOPerS - 1)) * kTO, last);
+            };
+            int row = 0, row_next = rows_from(0);
+            const int start = draft_start(p, it.b);
+            const unsigned long long seen = role == 1 ? p.seen[it.b] : 0;
+            if (role == 0 && it.b != prev_b && lane == 0) {
+                // Q of the new tile: two 128 x 64 boxes per ring slot
+                long long r0;
+                int n;
+                tree_rows(p, it.b, r0, n);
+                for (int kb = 0; kb < kKBlocks; kb += 2) {
+                    if (!acquire()) { ok = false; break; }
+                    const int nb = min(2, kKBlocks - kb);
+                    const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
+                    ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), nb * kQBoxBytes);
+                    for (int j = 0; j < nb; ++j)
+                        ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)r0, bar(kBarFull + rg.slot));
+                    rg.next(nslots);
+                }
+            }
+            prev_b = it.b;
+            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            for (int t0 = 0; ok && t0 < it.len; t0 += kTS) {
+                const int piece = t0 / kTO, at = piece % (kRowTiles * kOPerS);
+                if (at == 0) {
+                    row = row_next;
+                    row_next = rows_from(piece + kRowTiles * kOPerS);
+                }
+                int pr[kOPerS];
+#pragma unroll
+                for (int c = 0; c < kOPerS; ++c) pr[c] = __shfl_sync(0xffffffffu, row, at + c);
+                if (lane == 0) {
+                    if (role == 0) {
+                        for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                            if (!acquire()) { ok = false; break; }
+                            const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
+                            ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kSlotS);
+#pragma unroll
+                            for (int c = 0; c < kOPerS; ++c)
+                                ptx::tma_load_4d(dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3,
+                                                 bar(kBarFull + rg.slot));
+                            rg.next(nslots);
+                        }
+                    } else {
+                        const int nct = (min(kTS, it.len - t0) + kTO - 1) / kTO;
+#pragma unroll
+                        for (int ct = 0; ct < kOPerS; ++ct) {
+                            if (ct >= nct || !ok) break;
+                            if (!acquire()) { ok = false; break; }
+                            const int t = it.tok0 + t0 + ct * kTO;
+                            const bool hidden = t + kTO > start && tree_word(seen, start, t) != 0xffffffffu;
+                            const uint32_t full = bar((hidden ? kBarTail : kBarFull) + rg.slot);
+                            ptx::mbar_arrive_expect_tx(full, kSlotO);
+                            ptx::tma_load_3d(sbase + kOffRing + rg.slot * kSlotO, &cmap_o, 0, pr[ct], 0, full);
+                            rg.next(nslots);
+                        }
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            }
+        }
+        if (lane == 0) {
+            if (!ok) *abort_flag = 1;
+            // drain: every issued load has been consumed (or the wait expires)
+            for (int k = 0; k < nslots; ++k, rg.next(nslots))
+                ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
+        }
+    } else if (warp == 1 && role == 1) {
+        // ------------------------------------------------------------ O-CTA: GEMM2
+        if (lane == 0) {
+            tc::Ring rg;
+            uint32_t jt = 0;
+            bool ok = true;
+            while (ok && items_next<kSched>(wl, cur, it, id)) {
+                for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
+                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                    if (*abort_flag || !ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer) ||
+                        !ptx::mbar_spin(bar(kBarCorr + ms), mu & 1, kErrWaitMma)) { ok = false; break; }
+                    const int nct = (min(kTS, it.len - t0) + kTO - 1) / kTO;
+                    ptx::tc_fence_after();  // the correction's TMEM stores to O come first
+                    const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsg + ms * kMsgBytes, 16, 512);
+                    for (int ct = 0; ct < nct; ++ct) {
+                        if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                        const uint32_t acc0 = (t0 > 0 || ct > 0) ? 1u : 0u;
+                        const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO, kBoxO, 1024);
+                        const uint64_t pa = p0 + (uint64_t)(ct * (kSubP >> 4));
+#pragma unroll
+                        for (int kk = 0; kk < kTO / 16; ++kk)
+#pragma unroll
+                            for (int nh = 0; nh < 2; ++nh)
+                                ptx::mma_ss(tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
+                                            c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), tc::idesc_o<kBf16>(),
+                                            kk > 0 ? 1u : acc0);
+                        ptx::mma_commit(bar(kBarEmpty + rg.slot));
+                        rg.next(kSlotsO);
+                    }
+                    if (!ok) break;
+                    ptx::mma_commit_mc(bar(kBarPFree + ms), 0x3);
+                    ptx::mma_commit(bar(kBarMmaDone + ms));
+                }
+            }
+            if (!ok) *abort_flag = 1;
+            ptx::mma_commit(bar(kBarDrain));
+            ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
+        }
+    } else if ((warp == 1 || warp == 3) && role == 0) {
+        // ------------------------------------------------------------ S-CTA: GEMM1
+        // Two threads take alternate S tiles (and S buffers).  At the first S tile of a
+        // row tile its issuer copies Q into TMEM once every GEMM1 of the previous one
+        // is done; the other waits for the copy before its next S tile.
+        if (lane == 0) {
+            const uint32_t me = warp == 1 ? 0u : 1u;
+            tc::Ring rg;
+            uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
+            int prev_b = -1;
+            bool ok = true;
+            while (ok && items_next<kSched>(wl, cur, it, id)) {
+                const bool new_seq = it.b != prev_b;
+                prev_b = it.b;
+                for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
+                    const bool mine = (jt & 1u) == me;
+                    if (new_seq && t0 == 0) {
+                        ++nseq;
+                        if (mine) {
+                            if (jt > 0) {
+                                // an MMA is not ordered before a later tcgen05.cp: every GEMM1
+                                // that reads the old Q completes first
+                                ptx::mma_commit(bar(kBarQFree + me));
+                                if (!ptx::mbar_spin(bar(kBarQFree + me), qphase, kErrWaitMma)) { ok = false; break; }
+                                qphase ^= 1;
+                                const uint32_t pj = jt - 1;  // the other issuer's last tile
+                                if (!ptx::mbar_spin(bar(kBarSFull + (pj & 1)), (pj >> 1) & 1, kErrWaitMma)) { ok = false; break; }
+                                ptx::tc_fence_after();
+                            }
+                            for (int kb = 0; ok && kb < kKBlocks; kb += 2) {
+                                if (*abort_flag || !ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                                const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
+                                const int nb = min(2, kKBlocks - kb);
+                                for (int j = 0; j < nb; ++j) {
+#pragma unroll
+                                    for (int c = 0; c < 4; ++c)
+                                        ptx::tmem_cp_128x256b(tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
+                                                              ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
+                                }
+                                ptx::mma_commit(bar(kBarEmpty + rg.slot));
+                                rg.next(kSlotsS);
+                            }
+                            if (!ok) break;
+                            ptx::mma_commit(bar(kBarQReady));
+                            qready_seq = nseq;
+                        } else {
+                            for (int q = 0; q < kQSlots; ++q) rg.next(kSlotsS);
+                        }
+                    }
+                    if (!mine) {
+                        for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(kSlotsS);
+                        continue;
+                    }
+                    if (qready_seq != nseq) {  // the other issuer copied this tile's Q
+                        if (!ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma)) { ok = false; break; }
+                        qready_seq = nseq;
+                    }
+                    const uint32_t sb = jt & 1, use = jt >> 1;
+                    if (*abort_flag || !ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma)) { ok = false; break; }
+                    ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
+                    const uint32_t d = tmem + kTmemS + sb * kTS;
+                    for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                        if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                        const uint32_t acc0 = sl > 0 ? 1u : 0u;
+                        // the slot's K-blocks interleave per 8-row group: groups 3 KB apart
+                        const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kKbPerSlot * 1024);
+                        const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 32);
+#pragma unroll
+                        for (int k = 0; k < kKbPerSlot * 4; ++k)
+                            ptx::mma_ts(d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * 1024 + (k & 3) * 32) >> 4),
+                                        tc::idesc_s<kBf16>(), k > 0 ? 1u : acc0);
+                        ptx::mma_commit(bar(kBarEmpty + rg.slot));
+                        rg.next(kSlotsS);
+                    }
+                    if (!ok) break;
+                    ptx::mma_commit(bar(kBarSFull + sb));
+                }
+            }
+            if (!ok) *abort_flag = 1;
+            ptx::mma_commit(bar(kBarDrain + me));
+            ptx::mbar_wait(bar(kBarDrain + me), 0, kErrWaitMma);
+        }
+    } else if (warp == 2 && role == 1) {
+        // ------------------------------------------------------------ O-CTA: hidden rows
+        uint32_t at = 0;        // ring slots of the items before this one
+        uint32_t uses = 0;      // per slot: parity of its next hidden tile
+        bool ok = true;
+        while (ok && items_next<kSched>(wl, cur, it, id)) {
+            const int start = draft_start(p, it.b);
+            const int pieces = (it.len + kTO - 1) / kTO;
+            if (it.tok0 + it.len > start) {
+                const unsigned long long seen = p.seen[it.b];
+                for (int q = max(0, (start - it.tok0) / kTO - 1); ok && q < pieces; ++q) {
+                    const int t = it.tok0 + q * kTO;
+                    if (t + kTO <= start) continue;
+                    const uint32_t keep = tree_word(seen, start, t);
+                    if (keep == 0xffffffffu) continue;
+                    const uint32_t slot = (at + q) % kSlotsO;
+                    ok = !*abort_flag && ptx::mbar_wait(bar(kBarTail + slot), (uses >> slot) & 1, kErrWaitFull, kTailWaitNs);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    uses ^= 1u << slot;
+                    const uint32_t tile = sbase + kOffRing + slot * kSlotO;
+                    for (int i = lane; i < kTO * kVBlocks * 8; i += 32) {  // 16-byte pieces, 64 a row
+                        const int row = i >> 6;
+                        if (!((keep >> row) & 1u))
+                            ptx::st_shared_v4(tile + ((i >> 3) & (kVBlocks - 1)) * kBoxO + row * 128 + (i & 7) * 16, 0u, 0u, 0u, 0u);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(bar(kBarFull + slot));
+                }
+            }
+            at += pieces;
+        }
+        if (!ok) *abort_flag = 1;
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ math warpgroups
+        const int h = (tid - 128) & 127;            // row = TMEM lane
+        const int half = (tid - 128) >> 7;
+        const uint32_t trow = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        uint32_t jt = 0;
+        bool ok = true;
+        if (role == 0) {
+            // ------------------------------------------------ S-CTA: softmax
+            const uint32_t peer_pfull0 = ptx::mapa(bar(kBarPFull), 1);
+            const uint32_t peer_msg0 = ptx::mapa(sbase + kOffMsg, 1);
+            const bool sender = tid == 128;
+            float *maxima = reinterpret_cast<float *>(smem + kOffMax);
+            const float sl2 = p.scale_log2;
+            while (ok && items_next<kSched>(wl, cur, it, id)) {
+                float m_used = -INFINITY, l_run = 0.f;
+                // the drafts this row sees, and where they start from this warpgroup's column 0
+                const int b = it.b / p.tiles;
+                const int d = min((it.b - b * p.tiles) * p.tile_drafts + h / p.heads, p.drafts - 1);
+                unsigned long long mask = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
+                if (p.drafts < 64) mask &= (1ull << p.drafts) - 1;
+                const int start = draft_start(p, it.b) - it.tok0 - half * kHalf;
+                for (int t0 = 0; t0 < it.len; t0 += kTS, ++jt) {
+                    const uint32_t sb = jt & 1, use = jt >> 1;
+                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                    const bool last = t0 + kTS >= it.len;
+                    // Every decision is uniform over the warpgroups (bar.red below), so an
+                    // expired wait never splits a warp at a .sync.aligned instruction.
+                    bool w = !*abort_flag && ptx::mbar_wait(bar(kBarSFull + sb), use & 1, kErrWaitMma);
+                    w = __all_sync(0xffffffffu, w);
+                    uint32_t r[kHalf];
+                    float own = -INFINITY;
+                    if (w) {
+                        ptx::tc_fence_after();
+                        const uint32_t s_addr = trow + kTmemS + sb * kTS + half * kHalf;
+                        ptx::tmem_ld_x32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(r));
+                        tmem_ld_x16(s_addr + 32, *reinterpret_cast<uint32_t(*)[16]>(r + 32));
+                        ptx::tmem_wait_ld();
+                        ptx::tc_fence_before();
+                        ptx::mbar_arrive(bar(kBarSEmpty + sb));
+                        if (t0 + kHalf > start) {  // the columns reach into the drafts
+                            const uint32_t w0 = tree_word(mask, start, t0), w1 = tree_word(mask, start, t0 + 32);
+#pragma unroll
+                            for (int k = 0; k < kHalf; ++k)
+                                if (!(((k < 32 ? w0 : w1) >> (k & 31)) & 1u)) r[k] = tc::u32_of(-INFINITY);
+                        }
+                        float m4[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) m4[k] = tc::f32_of(r[k]);
+#pragma unroll
+                        for (int k = 4; k < kHalf; ++k) m4[k & 3] = fmaxf(m4[k & 3], tc::f32_of(r[k]));
+                        own = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+                        maxima[(sb * 2 + half) * 128 + h] = own;
+                    }
+                    // the previous message has left the staging buffer, both maxima are there
+                    if (sender) ptx::bulk_wait_group_read<0>();
+                    if (!ptx::named_barrier_and(1, kMath, w)) { ok = false; break; }
+                    const float mx = fmaxf(own, maxima[(sb * 2 + (half ^ 1)) * 128 + h]) * sl2;
+                    float alpha = 1.f;
+                    if (mx > m_used + tc::kRescaleLog2) {
+                        alpha = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - mx);
+                        m_used = mx;
+                    }
+                    // (a row that has seen nothing keeps m_used = -inf: its weights are 0)
+                    const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+                    float s4[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t pk[kHalf / 2];
+#pragma unroll
+                    for (int k = 0; k < kHalf; k += 2) {
+                        const float p0 = ptx::ex2(fmaf(tc::f32_of(r[k]), sl2, neg_m));
+                        const float p1 = ptx::ex2(fmaf(tc::f32_of(r[k + 1]), sl2, neg_m));
+                        s4[(k >> 1) & 3] += p0 + p1;
+                        pk[k >> 1] = tc::pack2<kBf16>(p0, p1);
+                    }
+                    l_run = l_run * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+                    uint8_t *msg = smem + kOffStg;
+#pragma unroll
+                    for (int q = 0; q < kHalf / 8; ++q) {  // 16-byte pieces of 8 tokens
+                        const int c = half * (kHalf / 8) + q, st = c >> 2, c4 = c & 3;
+                        reinterpret_cast<uint4 *>(msg + st * kSubP + h * 64)[c4 ^ ((h >> 1) & 3)] =
+                            make_uint4(pk[4 * q], pk[4 * q + 1], pk[4 * q + 2], pk[4 * q + 3]);
+                    }
+                    if (half == 0) reinterpret_cast<float *>(msg + kMsgAlpha)[h] = alpha;
+                    if (last) {
+                        reinterpret_cast<float *>(msg + kMsgL)[half * 128 + h] = l_run;
+                        if (half == 0) reinterpret_cast<float *>(msg + kMsgM)[h] = m_used;
+                    }
+                    ptx::fence_proxy_async_smem();
+                    ptx::named_barrier(1, kMath);
+                    if (sender) {
+                        // the O-CTA's slot is free once GEMM2 of S tile jt - 3 finished
+                        if (ptx::mbar_wait<true>(bar(kBarPFree + ms), (mu & 1) ^ 1, kErrWaitPeer)) {
+                            const uint32_t rbar = peer_pfull0 + 8u * ms;
+                            ptx::mbar_remote_arrive_expect_tx(rbar, kMsgBytes);
+                            ptx::bulk_copy_s2cluster(peer_msg0 + ms * kMsgBytes, sbase + kOffStg, kMsgBytes, rbar);
+                            ptx::bulk_commit_group();
+                        } else {
+                            *abort_flag = 1;  // everyone leaves at the next tile's barrier, or below
+                        }
+                    }
+                }
+            }
+            if (!ok) *abort_flag = 1;
+            // The last messages were consumed by the peer's GEMM2 (so no remote arrival
+            // is still in flight towards this CTA).
+            for (uint32_t k = (jt >= (uint32_t)kMsgSlots ? jt - kMsgSlots : 0); k < jt; ++k)
+                ptx::mbar_wait<true>(bar(kBarPFree + (k % kMsgSlots)), (k / kMsgSlots) & 1, kErrWaitPeer);
+            if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        } else {
+            // ------------------------------------------------ O-CTA: correction + epilogue
+            // (each warpgroup its half of O's columns)
+            const uint32_t o_addr = trow + half * (kDV / 2);
+            auto gemm2_done = [&](uint32_t x) -> bool {
+                return ptx::mbar_wait(bar(kBarMmaDone + x % kMsgSlots), (x / kMsgSlots) & 1, kErrWaitMma);
+            };
+            while (ok && items_next<kSched>(wl, cur, it, id)) {
+                for (int t0 = 0; t0 < it.len; t0 += kTS, ++jt) {
+                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                    bool w = !*abort_flag && ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer);
+                    const uint8_t *msg = smem + kOffMsg + ms * kMsgBytes;
+                    const bool last = t0 + kTS >= it.len;
+                    float alpha = 1.f, l_fin = 0.f, m_fin = 0.f;
+                    if (w) {
+                        alpha = reinterpret_cast<const float *>(msg + kMsgAlpha)[h];
+                        if (last) {
+                            l_fin = reinterpret_cast<const float *>(msg + kMsgL)[h] +
+                                    reinterpret_cast<const float *>(msg + kMsgL)[128 + h];
+                            m_fin = reinterpret_cast<const float *>(msg + kMsgM)[h];
+                        }
+                    } else {
+                        *abort_flag = 1;
+                    }
+                    // one barrier: does any row need its O corrected, or did any wait fail?
+                    if (ptx::named_barrier_or(2, kMath, !w || (t0 > 0 && alpha != 1.f))) {
+                        w = !*abort_flag && gemm2_done(jt - 1);
+                        if (!ptx::named_barrier_and(2, kMath, w)) { ok = false; break; }
+                        ptx::tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < kDV / 64; ++c) {
+                            uint32_t r[32];
+                            ptx::tmem_ld_x32(o_addr + c * 32, r);
+                            ptx::tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) r[k] = tc::u32_of(tc::f32_of(r[k]) * alpha);
+                            ptx::tmem_st_x32(o_addr + c * 32, r);
+                        }
+                        ptx::tmem_wait_st();
+                    }
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(bar(kBarCorr + ms));
+                    if (last) {
+                        w = gemm2_done(jt);
+                        if (!ptx::named_barrier_and(2, kMath, w)) { ok = false; break; }
+                        ptx::tc_fence_after();
+                        // A tile of one item gets its final output here, else its partial
+                        // goes to the workspace.  32 bytes (a whole sector) a store.
+                        int i0, i1, nrows;
+                        item_range<kSched>(wl, it.b, i0, i1);
+                        const bool single = i1 - i0 == 1;
+                        long long row0;
+                        tree_rows(p, it.b, row0, nrows);
+                        const float inv_l = l_fin > 0.f ? 1.f / l_fin : 0.f;
+                        const bool f32 = !single || p.out_kind == tc::kOutF32;
+                        const size_t row = single ? (size_t)row0 + h : (size_t)id * p.num_heads + h;
+                        uint8_t *dst = (single ? static_cast<uint8_t *>(p.out) : reinterpret_cast<uint8_t *>(p.part_o)) +
+                                       (row * kDV + half * (kDV / 2)) * (f32 ? 4 : 2);
+#pragma unroll 1
+                        for (int c = 0; c < kDV / 64; ++c) {
+                            uint32_t r[32];
+                            ptx::tmem_ld_x32(o_addr + c * 32, r);
+                            ptx::tmem_wait_ld();
+                            if (f32) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) r[k] = tc::u32_of(tc::f32_of(r[k]) * inv_l);
+                                if (h < nrows) {
+#pragma unroll
+                                    for (int k = 0; k < 4; ++k) store32(dst + c * 128 + k * 32, r + 8 * k);
+                                }
+                            } else {
+                                uint32_t o[16];
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    o[k] = tc::pack2<kBf16>(tc::f32_of(r[2 * k]) * inv_l, tc::f32_of(r[2 * k + 1]) * inv_l);
+                                if (h < nrows) {
+                                    store32(dst + c * 64, o);
+                                    store32(dst + c * 64 + 32, o + 8);
+                                }
+                            }
+                        }
+                        if (half == 0 && h < nrows) {
+                            const float lse = l_fin > 0.f ? (m_fin + __log2f(l_fin)) * kLn2 : -INFINITY;
+                            if (!single) p.part_lse[row] = lse;
+                            else if (p.out_lse != nullptr) p.out_lse[row] = lse;
+                        }
+                        ptx::tc_fence_before();
+                    }
+                }
+            }
+            if (!ok) *abort_flag = 1;
+        }
+    }
+
+    // ---------------------------------------------------------------- teardown
+    ptx::tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    ptx::cluster_sync();  // neither CTA leaves while its partner may still target it
+    if (warp == 2) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, kTmemCols);
+    }
 }
 
 // O = sum_i e^(lse_i - M) O_i / sum_i e^(lse_i - M), M = max_i lse_i, over the
@@ -37,7 +670,7 @@ __global__ void __launch_bounds__(256) seen_kernel(const unsigned long long *__r
 template <typename OutT, int kRowWarps>
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__restrict__ part_o,
                                                                  const float *__restrict__ part_lse, WorkList wl,
-                                                                 tc::TcTreeParams p, OutT *__restrict__ out,
+                                                                 TreeParams p, OutT *__restrict__ out,
                                                                  float *__restrict__ out_lse) {
     constexpr int kRows = kMergeWarps / kRowWarps;  // rows per block
     __shared__ __align__(16) float acc_s[kRowWarps > 1 ? kRowWarps - 1 : 1][kDV];
@@ -49,7 +682,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
     const int r = blockIdx.x * kRows + warp / kRowWarps, g = warp % kRowWarps;
     long long row0;
     int rows;
-    tc::tree_rows(p, v, row0, rows);
+    tree_rows(p, v, row0, rows);
     int i0, i1;
     item_range(wl, v, i0, i1);
     if (i1 - i0 == 1) return;               // the same for the whole block

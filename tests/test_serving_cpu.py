@@ -19,13 +19,13 @@ def test_tree_mask_from_parents():
 
 def tree(**kw):
     a = dict(q=16, kv=16, bt=16, sl=16, mask=16, shared=0, batch=1, drafts=4, heads=16, pages=4, page=64, blocks=4, longest=64, scale=1.0,
-             splits=0, out=16, dtype=capi.OUT_F16, lse=None, ws=None, ws_bytes=0, stream=None)
+             splits=0, out=32, dtype=capi.OUT_F16, lse=None, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return capi.lib().mla_b200_decode_tree_f16(*a.values())
 
 
 def test_tree_arguments():
-    for bad in [dict(q=None), dict(kv=None), dict(bt=None), dict(sl=None), dict(out=None), dict(q=18), dict(kv=24), dict(mask=12), dict(lse=2),
+    for bad in [dict(q=None), dict(kv=None), dict(bt=None), dict(sl=None), dict(out=None), dict(out=16), dict(q=18), dict(kv=24), dict(mask=12), dict(lse=2),
                 dict(batch=-1), dict(drafts=0), dict(heads=0), dict(page=0), dict(longest=-1), dict(longest=257), dict(scale=0.0),
                 dict(scale=float("inf")), dict(dtype=capi.OUT_BF16), dict(dtype=9)]:
         assert tree(**bad) == capi.ERR_INVALID_ARG, bad
