@@ -383,6 +383,52 @@ __device__ __forceinline__ void mma_commit_mc(uint32_t bar, uint16_t mask) {
         : "memory");
 }
 
+// The same behind a predicate, for whole warps with one elected lane (lane_on != 0 in
+// that lane alone): without a branch around them, the descriptors of a run of MMAs can
+// stay in uniform registers.
+__device__ __forceinline__ void mma_ss_if(uint32_t lane_on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_ts_if(uint32_t lane_on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_cp_128x256b_if(uint32_t lane_on, uint32_t d_tmem, uint64_t s_desc) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.128x256b [%0], %1;\n\t}" ::"r"(
+            d_tmem),
+        "l"(s_desc), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_commit_if(uint32_t lane_on, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_commit_mc_if(uint32_t lane_on, uint32_t bar, uint16_t mask) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
+            bar),
+        "h"(mask), "r"(lane_on)
+        : "memory");
+}
+
 #define MLA_TMEM_LD_X32(taddr, r)                                                               \
     asm volatile(                                                                               \
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13," \

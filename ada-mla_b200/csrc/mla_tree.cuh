@@ -296,124 +296,131 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
     } else if (warp == 1 && role == 1) {
         // ------------------------------------------------------------ O-CTA: GEMM2
-        if (lane == 0) {
-            tc::Ring rg;
-            uint32_t jt = 0;
-            bool ok = true;
-            while (ok && items_next<kSched>(wl, cur, it, id)) {
-                for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
-                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
-                    if (*abort_flag || !ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer) ||
-                        !ptx::mbar_spin(bar(kBarCorr + ms), mu & 1, kErrWaitMma)) { ok = false; break; }
-                    const int nct = (min(kTS, it.len - t0) + kTO - 1) / kTO;
-                    ptx::tc_fence_after();  // the correction's TMEM stores to O come first
-                    const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsg + ms * kMsgBytes, 16, 512);
-                    for (int ct = 0; ct < nct; ++ct) {
-                        if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
-                        const uint32_t acc0 = (t0 > 0 || ct > 0) ? 1u : 0u;
-                        const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO, kBoxO, 1024);
-                        const uint64_t pa = p0 + (uint64_t)(ct * (kSubP >> 4));
+        // (The issuing warps run as whole warps with uniform control flow and one elected
+        // lane behind each instruction, so that descriptors stay in uniform registers: 48
+        // cycles an MMA of N = 96 against 53 from a branch of lane 0, and ~100 there when
+        // math warps share the scheduler.  So a wait that runs out does not branch off
+        // either: the tile is finished on whatever the buffers hold and then given up.)
+        const uint32_t e = ptx::elect_one();
+        tc::Ring rg;
+        uint32_t jt = 0;
+        bool ok = true;
+        while (ok && items_next<kSched>(wl, cur, it, id)) {
+            const int len = __shfl_sync(0xffffffffu, it.len, 0);
+            for (int t0 = 0; t0 < len; t0 += kTS, ++jt) {
+                const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                ok = !*abort_flag && ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer);
+                ok = ok && ptx::mbar_spin(bar(kBarCorr + ms), mu & 1, kErrWaitMma);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                const int nct = (min(kTS, len - t0) + kTO - 1) / kTO;
+                ptx::tc_fence_after();  // the correction's TMEM stores to O come first
+                const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsg + ms * kMsgBytes, 16, 512);
+                for (int ct = 0; ct < nct; ++ct) {
+                    ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                    const uint32_t acc0 = (t0 > 0 || ct > 0) ? 1u : 0u;
+                    const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO, kBoxO, 1024);
+                    const uint64_t pa = p0 + (uint64_t)(ct * (kSubP >> 4));
 #pragma unroll
-                        for (int kk = 0; kk < kTO / 16; ++kk)
+                    for (int kk = 0; kk < kTO / 16; ++kk)
 #pragma unroll
-                            for (int nh = 0; nh < 2; ++nh)
-                                ptx::mma_ss(tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
-                                            c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), tc::idesc_o<kBf16>(),
-                                            kk > 0 ? 1u : acc0);
-                        ptx::mma_commit(bar(kBarEmpty + rg.slot));
-                        rg.next(kSlotsO);
-                    }
-                    if (!ok) break;
-                    ptx::mma_commit_mc(bar(kBarPFree + ms), 0x3);
-                    ptx::mma_commit(bar(kBarMmaDone + ms));
+                        for (int nh = 0; nh < 2; ++nh)
+                            ptx::mma_ss_if(e, tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
+                                           c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), tc::idesc_o<kBf16>(),
+                                           kk > 0 ? 1u : acc0);
+                    ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                    rg.next(kSlotsO);
                 }
+                ptx::mma_commit_mc_if(e, bar(kBarPFree + ms), 0x3);
+                ptx::mma_commit_if(e, bar(kBarMmaDone + ms));
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             }
-            if (!ok) *abort_flag = 1;
-            ptx::mma_commit(bar(kBarDrain));
-            ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
         }
+        if (!ok) *abort_flag = 1;
+        ptx::mma_commit_if(e, bar(kBarDrain));
+        ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
     } else if ((warp == 1 || warp == 3) && role == 0) {
         // ------------------------------------------------------------ S-CTA: GEMM1
-        // Two threads take alternate S tiles (and S buffers).  At the first S tile of a
+        // Two warps take alternate S tiles (and S buffers).  At the first S tile of a
         // row tile its issuer copies Q into TMEM once every GEMM1 of the previous one
         // is done; the other waits for the copy before its next S tile.
-        if (lane == 0) {
-            const uint32_t me = warp == 1 ? 0u : 1u;
-            tc::Ring rg;
-            uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
-            int prev_b = -1;
-            bool ok = true;
-            while (ok && items_next<kSched>(wl, cur, it, id)) {
-                const bool new_seq = it.b != prev_b;
-                prev_b = it.b;
-                for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
-                    const bool mine = (jt & 1u) == me;
-                    if (new_seq && t0 == 0) {
-                        ++nseq;
-                        if (mine) {
-                            if (jt > 0) {
-                                // an MMA is not ordered before a later tcgen05.cp: every GEMM1
-                                // that reads the old Q completes first
-                                ptx::mma_commit(bar(kBarQFree + me));
-                                if (!ptx::mbar_spin(bar(kBarQFree + me), qphase, kErrWaitMma)) { ok = false; break; }
-                                qphase ^= 1;
-                                const uint32_t pj = jt - 1;  // the other issuer's last tile
-                                if (!ptx::mbar_spin(bar(kBarSFull + (pj & 1)), (pj >> 1) & 1, kErrWaitMma)) { ok = false; break; }
-                                ptx::tc_fence_after();
-                            }
-                            for (int kb = 0; ok && kb < kKBlocks; kb += 2) {
-                                if (*abort_flag || !ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
-                                const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
-                                const int nb = min(2, kKBlocks - kb);
-                                for (int j = 0; j < nb; ++j) {
-#pragma unroll
-                                    for (int c = 0; c < 4; ++c)
-                                        ptx::tmem_cp_128x256b(tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
-                                                              ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
-                                }
-                                ptx::mma_commit(bar(kBarEmpty + rg.slot));
-                                rg.next(kSlotsS);
-                            }
-                            if (!ok) break;
-                            ptx::mma_commit(bar(kBarQReady));
-                            qready_seq = nseq;
-                        } else {
-                            for (int q = 0; q < kQSlots; ++q) rg.next(kSlotsS);
+        const uint32_t e = ptx::elect_one();
+        const uint32_t me = warp == 1 ? 0u : 1u;
+        tc::Ring rg;
+        uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
+        int prev_b = -1;
+        bool ok = true;
+        while (ok && items_next<kSched>(wl, cur, it, id)) {
+            const int len = __shfl_sync(0xffffffffu, it.len, 0), v = __shfl_sync(0xffffffffu, it.b, 0);
+            const bool new_seq = v != prev_b;
+            prev_b = v;
+            for (int t0 = 0; t0 < len; t0 += kTS, ++jt) {
+                const bool mine = (jt & 1u) == me;
+                if (new_seq && t0 == 0) {
+                    ++nseq;
+                    if (mine) {
+                        if (jt > 0) {
+                            // an MMA is not ordered before a later tcgen05.cp: every GEMM1
+                            // that reads the old Q completes first
+                            ptx::mma_commit_if(e, bar(kBarQFree + me));
+                            ok = ptx::mbar_spin(bar(kBarQFree + me), qphase, kErrWaitMma);
+                            qphase ^= 1;
+                            const uint32_t pj = jt - 1;  // the other issuer's last tile
+                            ok = ok && ptx::mbar_spin(bar(kBarSFull + (pj & 1)), (pj >> 1) & 1, kErrWaitMma);
+                            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                            ptx::tc_fence_after();
                         }
-                    }
-                    if (!mine) {
-                        for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(kSlotsS);
-                        continue;
-                    }
-                    if (qready_seq != nseq) {  // the other issuer copied this tile's Q
-                        if (!ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma)) { ok = false; break; }
-                        qready_seq = nseq;
-                    }
-                    const uint32_t sb = jt & 1, use = jt >> 1;
-                    if (*abort_flag || !ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma)) { ok = false; break; }
-                    ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
-                    const uint32_t d = tmem + kTmemS + sb * kTS;
-                    for (int sl = 0; sl < kSlotsPerTile; ++sl) {
-                        if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
-                        const uint32_t acc0 = sl > 0 ? 1u : 0u;
-                        // the slot's K-blocks interleave per 8-row group: groups 3 KB apart
-                        const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kKbPerSlot * 1024);
-                        const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 32);
+                        for (int kb = 0; kb < kKBlocks; kb += 2) {
+                            ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                            const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
+                            const int nb = min(2, kKBlocks - kb);
+                            for (int j = 0; j < nb; ++j) {
 #pragma unroll
-                        for (int k = 0; k < kKbPerSlot * 4; ++k)
-                            ptx::mma_ts(d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * 1024 + (k & 3) * 32) >> 4),
-                                        tc::idesc_s<kBf16>(), k > 0 ? 1u : acc0);
-                        ptx::mma_commit(bar(kBarEmpty + rg.slot));
-                        rg.next(kSlotsS);
+                                for (int c = 0; c < 4; ++c)
+                                    ptx::tmem_cp_128x256b_if(e, tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
+                                                             ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
+                            }
+                            ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                            rg.next(kSlotsS);
+                        }
+                        ptx::mma_commit_if(e, bar(kBarQReady));
+                        qready_seq = nseq;
+                    } else {
+                        for (int q = 0; q < kQSlots; ++q) rg.next(kSlotsS);
                     }
-                    if (!ok) break;
-                    ptx::mma_commit(bar(kBarSFull + sb));
                 }
+                if (!mine) {
+                    for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(kSlotsS);
+                    continue;
+                }
+                if (qready_seq != nseq) {  // the other issuer copied this tile's Q
+                    ok &= ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma);
+                    qready_seq = nseq;
+                }
+                const uint32_t sb = jt & 1, use = jt >> 1;
+                ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
+                const uint32_t d = tmem + kTmemS + sb * kTS;
+                for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                    ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                    const uint32_t acc0 = sl > 0 ? 1u : 0u;
+                    // the slot's K-blocks interleave per 8-row group: groups 3 KB apart
+                    const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kKbPerSlot * 1024);
+                    const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 32);
+#pragma unroll
+                    for (int k = 0; k < kKbPerSlot * 4; ++k)
+                        ptx::mma_ts_if(e, d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * 1024 + (k & 3) * 32) >> 4),
+                                       tc::idesc_s<kBf16>(), k > 0 ? 1u : acc0);
+                    ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                    rg.next(kSlotsS);
+                }
+                ptx::mma_commit_if(e, bar(kBarSFull + sb));
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             }
-            if (!ok) *abort_flag = 1;
-            ptx::mma_commit(bar(kBarDrain + me));
-            ptx::mbar_wait(bar(kBarDrain + me), 0, kErrWaitMma);
         }
+        if (!ok) *abort_flag = 1;
+        ptx::mma_commit_if(e, bar(kBarDrain + me));
+        ptx::mbar_wait(bar(kBarDrain + me), 0, kErrWaitMma);
     } else if (warp == 2 && role == 1) {
         // ------------------------------------------------------------ O-CTA: hidden rows
         uint32_t at = 0;        // ring slots of the items before this one
