@@ -390,15 +390,6 @@ struct PagedArgs {
     long long pool_rows;
 };
 
-// A tree of `drafts` draft tokens per sequence over a paged cache: `tiles` row tiles
-// of up to `tile_drafts` drafts of `heads` rows each per sequence, each tile a
-// sequence of the work list (tree::TreeParams).
-struct TreeArgs {
-    const unsigned long long *mask;  // null: a chain
-    int mask_stride;
-    int drafts, heads, tiles, tile_drafts;
-};
-
 // Launch, with programmatic stream serialization when `dependent`: the kernel
 // may then start while its predecessor in the stream runs (the predecessor
 // allows it with griddep_launch) and waits for it (griddep_wait) before
@@ -431,27 +422,6 @@ void launch_tc(int clusters, const TcMaps &m, const tc::TcParams &tp, cudaStream
                      dim3(tc::kThreads), tc::kSmemBytes, stream, after_plan, m.cmap_s, m.cmap_o, m.qmap, tp);
 }
 
-template <int kSched, bool kBf16>
-void launch_tree(int clusters, const TcMaps &m, const tree::TreeParams &tp, cudaStream_t stream) {
-    launch_dependent(tree::decode_kernel<kSched, kBf16>, dim3(2 * clusters), dim3(tree::kThreads), tree::kSmemBytes,
-                     stream, true, m.cmap_s, m.cmap_o, m.qmap, tp);
-}
-
-template <typename OutT>
-void launch_tree_merge(const WsLayout &L, const WorkList &wl, const tree::TreeParams &tp, void *out, float *out_lse,
-                       cudaStream_t stream, bool chain) {
-    // a few tiles have many splits each: a block of 8 warps per row; many tiles have
-    // one or two: a warp per row
-    const dim3 block(32 * tree::kMergeWarps);
-    if (wl.batch < 8)
-        launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3((unsigned)tp.num_heads, (unsigned)wl.batch),
-                         block, 0, stream, chain, L.part_o, L.part_lse, wl, tp, static_cast<OutT *>(out), out_lse);
-    else
-        launch_dependent(tree::merge_kernel<OutT, 1>,
-                         dim3((unsigned)cdiv(tp.num_heads, tree::kMergeWarps), (unsigned)wl.batch), block, 0, stream,
-                         chain, L.part_o, L.part_lse, wl, tp, static_cast<OutT *>(out), out_lse);
-}
-
 // Shared driver of the split-KV paths: plan -> partial kernel -> combine.
 // pg (tensor-core path only): the cache is a page pool; cu_seqlens is ignored
 // and the sequences' offsets on a virtual packed axis are built from
@@ -462,7 +432,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
                      int num_splits, void *out, int out_dtype, float *out_lse, void *workspace,
                      size_t workspace_bytes, cudaStream_t stream, const PagedArgs *pg = nullptr,
                      const Fp8Args *f8 = nullptr, const MtpArgs *mtp = nullptr, int group = 1,
-                     const XchgArgs *xa = nullptr, const TreeArgs *tr = nullptr) {
+                     const XchgArgs *xa = nullptr) {
     int dev;
     DevInfo info;
     int st = current_device(&dev, &info);
@@ -508,9 +478,9 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
     const long long max_items = balanced ? (long long)batch + info.tc_clusters
                                          : max_items_for(batch, plan_total, chunk);
     if (max_items > (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
-    WsLayout L = ws_layout(workspace, max_items, num_heads, batch, f8 != nullptr, tr != nullptr);
+    WsLayout L = ws_layout(workspace, max_items, num_heads, batch, f8 != nullptr);
     if (workspace == nullptr || workspace_bytes < L.bytes) return MLA_B200_ERR_WORKSPACE;
-    if (!aligned(workspace, tr != nullptr ? 32 : 16)) return MLA_B200_ERR_INVALID_ARG;
+    if (!aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
     const int32_t *seq_lens = nullptr;
     if (pg != nullptr) {
         seq_lens = pg->seq_lens;
@@ -522,19 +492,6 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
     wl.chunk = balanced ? 0 : chunk;
     wl.item_cost = item_cost_for(num_heads);
     wl.group = group;
-    tree::TreeParams tree_p{};
-    TreePlan tree_plan{};
-    if (tr != nullptr) {
-        tree_p.num_heads = num_heads;
-        tree_p.mask = tr->mask;
-        tree_p.seen = L.tree_seen;
-        tree_p.mask_stride = tr->mask_stride;
-        tree_p.drafts = tr->drafts;
-        tree_p.heads = tr->heads;
-        tree_p.tiles = tr->tiles;
-        tree_p.tile_drafts = tr->tile_drafts;
-        tree_plan = {tr->mask, tr->mask_stride, tr->drafts, tr->tiles, tr->tile_drafts, L.tree_seen};
-    }
     const bool planned = cu_seqlens != nullptr || virt;  // a plan kernel precedes the decode
     int bal_clusters = 0;      // balanced: clusters to launch
     bool bal_split = true;     // balanced: some sequence has more than one item
@@ -564,7 +521,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             wl.nworkers = info.tc_clusters;
             bal_clusters = info.tc_clusters;
             plan_balanced_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, wl.item_cost, L.item_off, seq_lens,
-                                                         max_seq_len, L.cu_virtual, group, max_seq_len, tree_plan);
+                                                         max_seq_len, L.cu_virtual, group, max_seq_len);
         }
     } else if (!planned) {
         wl.items = nullptr;
@@ -581,7 +538,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
         wl.cu_seqlens = cu_seqlens;  // read by the paged kernel
         plan_varlen_kernel<<<1, 1024, 0, stream>>>(cu_seqlens, batch, chunk, L.item_off, L.items,
                                                    (int)max_items, seq_lens, max_seq_len, L.cu_virtual,
-                                                   group, max_seq_len, tree_plan);
+                                                   group, max_seq_len);
     }
     bool tc_direct = false;  // the tcgen05 kernel wrote single-item sequences itself
     // A few long sequences chain decode -> merge -> next decode with programmatic
@@ -598,8 +555,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             // S-CTA: one box per ring slot (3 K-blocks x 96 rows); paged, one per
             // 32-row piece and slot.  O-CTA: one box per 32-row C tile (8 K-blocks).
             const long long map_rows = pg != nullptr ? pg->pool_rows : total_tokens;
-            const long long qrows = tr != nullptr ? (long long)(batch / tr->tiles) * tr->drafts * tr->heads
-                                                  : (long long)batch * num_heads;
+            const long long qrows = (long long)batch * num_heads;
             if (f8 != nullptr) {
                 st = make_tmap_fp8_s(&cmap_s, f8->cache8, map_rows);
                 if (st == MLA_B200_OK) st = make_tmap_fp8_o(&cmap_o, f8->cache8, map_rows);
@@ -659,22 +615,7 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
             tc_direct = true;
             const int clusters = balanced ? bal_clusters : std::min(info.tc_clusters, wl.max_items);
             timing_mark(t_ev_start, stream);
-            if (tr != nullptr) {
-                tree_p.wl = wl;
-                tree_p.scale_log2 = tp.scale_log2;
-                tree_p.part_o = L.part_o;
-                tree_p.part_lse = L.part_lse;
-                tree_p.out = out;
-                tree_p.out_kind = tp.out_kind;
-                tree_p.out_lse = out_lse;
-                tree_p.chain = tp.chain;
-                tree_p.block_table = tp.block_table;
-                tree_p.max_blocks = tp.max_blocks;
-                tree_p.page_size = tp.page_size;
-                tree_p.num_pages = pg != nullptr ? (int)(pg->pool_rows / pg->page_size) : 0;
-                if (balanced) launch_tree<kSchedBalanced, kBf16>(clusters, maps, tree_p, stream);
-                else launch_tree<kSchedChunked, kBf16>(clusters, maps, tree_p, stream);
-            } else if (mtp != nullptr) {
+            if (mtp != nullptr) {
                 if (balanced) launch_tc<kSchedBalanced, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
                 else launch_tc<kSchedChunked, kBf16, false, false, true>(clusters, maps, tp, stream, planned || chain);
             } else if (f8 != nullptr) {
@@ -704,12 +645,6 @@ int run_split_decode(const T *q, const T *cache, const int32_t *cu_seqlens, int 
                 q, cache, wl, num_heads, scale * kLog2e, L.part_o, L.part_lse);
             timing_mark(t_ev_stop, stream);
         }
-    }
-    if (tr != nullptr) {
-        if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(L, wl, tree_p, out, out_lse, stream, chain);
-        else if constexpr (kBf16) launch_tree_merge<__nv_bfloat16>(L, wl, tree_p, out, out_lse, stream, chain);
-        else if constexpr (!std::is_same<T, float>::value) launch_tree_merge<__half>(L, wl, tree_p, out, out_lse, stream, chain);
-        return launch_status();
     }
     const long long rows = (long long)batch * num_heads;
     if (xa != nullptr) {
@@ -881,6 +816,20 @@ TreeTiles tree_tiles(int drafts, int heads) {
     return {tiles, (int)cdiv(drafts, tiles)};
 }
 
+template <typename OutT>
+void launch_tree_merge(const WsLayout &L, const tree::TreeParams &p, cudaStream_t stream, bool chain) {
+    // a few tiles have many splits each: a block of 8 warps per row; many tiles have one
+    // or two: a warp per row
+    const dim3 block(32 * tree::kMergeWarps);
+    const unsigned rows = (unsigned)p.num_heads, tiles = (unsigned)p.wl.batch;
+    if (tiles < 8)
+        launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(rows, tiles), block, 0, stream, chain,
+                         L.part_o, L.part_lse, p.wl, p, static_cast<OutT *>(p.out), p.out_lse);
+    else
+        launch_dependent(tree::merge_kernel<OutT, 1>, dim3((unsigned)cdiv(rows, tree::kMergeWarps), tiles), block, 0,
+                         stream, chain, L.part_o, L.part_lse, p.wl, p, static_cast<OutT *>(p.out), p.out_lse);
+}
+
 template <typename T>
 int decode_tree(const void *query, const void *kv_pages, const int32_t *block_table, const int32_t *seq_lens,
                 const uint64_t *mask, int shared_mask, int batch, int drafts, int heads, int num_pages, int page_size,
@@ -908,16 +857,99 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
         (long long)batch * drafts * heads >= (1LL << 31))
         return MLA_B200_ERR_UNSUPPORTED;
     if (batch == 0) return MLA_B200_OK;
-    TreeArgs tr{reinterpret_cast<const unsigned long long *>(mask), shared_mask ? 0 : drafts, drafts, heads, tt.tiles,
-                tt.tile_drafts};
-    PagedArgs pg{block_table, seq_lens, max_blocks, page_size, pool_rows};
-    // (no pages or no tokens: every row's O is 0 and its LSE -inf, through the merge of no partials)
-    const bool empty = num_pages == 0 || max_seq_len == 0;
-    return run_split_decode<T>(static_cast<const T *>(query), static_cast<const T *>(kv_pages), nullptr, (int)tiles,
-                               tt.tile_drafts * heads, empty ? 0 : tiles * max_seq_len, empty ? 0 : max_seq_len,
-                               softmax_scale, num_splits, out, out_dtype, out_lse, workspace, workspace_bytes,
-                               static_cast<cudaStream_t>(stream), empty ? nullptr : &pg, nullptr, nullptr, 1, nullptr,
-                               &tr);
+    int dev;
+    DevInfo info;
+    int st = current_device(&dev, &info);
+    if (st != MLA_B200_OK) return st;
+    const int rows = tt.tile_drafts * heads;
+    const bool empty = num_pages == 0 || max_seq_len == 0;  // every row's O is 0 and its LSE -inf
+    const int longest = empty ? 0 : max_seq_len;
+    // Automatic split: the balanced schedule, planned inside the decode kernel while its
+    // tables fit there; an explicit one: fixed chunks (whole S tiles), by a plan kernel.
+    const bool balanced = num_splits <= 0;
+    const bool planned_here = balanced && tiles <= tree::kPlanMax;
+    const int chunk = balanced ? 0 : (int)std::min<long long>(std::max(1LL, cdiv(cdiv(longest, num_splits), kTile)) * kTile, 1 << 30);
+    const long long max_items = balanced ? tiles + info.tc_clusters : max_items_for((int)tiles, tiles * longest, chunk);
+    if (max_items > (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
+    const WsLayout L = ws_layout(workspace, max_items, rows, (int)tiles, false, true);
+    if (workspace == nullptr || workspace_bytes < L.bytes) return MLA_B200_ERR_WORKSPACE;
+    if (!aligned(workspace, 32)) return MLA_B200_ERR_INVALID_ARG;
+    const long long cost_most = tiles * (cdiv(longest, kTile) + item_cost_for(rows));
+    const int clusters = (int)std::max(1LL, std::min<long long>(info.tc_clusters, balanced ? cost_most : max_items));
+    WorkList wl{};
+    wl.batch = (int)tiles;
+    wl.chunk = chunk;
+    wl.item_cost = item_cost_for(rows);
+    wl.group = 1;
+    wl.max_items = (int)max_items;
+    wl.seq_len = longest;
+    wl.item_off = L.item_off;
+    wl.items = L.items;
+    wl.cu_seqlens = L.cu_virtual;
+    wl.cost_off = L.item_off;
+    wl.nworkers = clusters;
+    tree::TreeParams p{};
+    p.num_heads = rows;
+    p.scale_log2 = softmax_scale * kLog2e;
+    p.part_o = L.part_o;
+    p.part_lse = L.part_lse;
+    p.out = out;
+    p.out_kind = out_dtype == MLA_B200_OUT_F16 ? tc::kOutF16 : out_dtype == MLA_B200_OUT_BF16 ? tc::kOutBF16 : tc::kOutF32;
+    p.out_lse = out_lse;
+    p.block_table = block_table;
+    p.max_blocks = max_blocks;
+    p.page_size = page_size;
+    p.num_pages = num_pages;
+    p.mask = reinterpret_cast<const unsigned long long *>(mask);
+    p.mask_stride = shared_mask ? 0 : drafts;
+    p.seen = L.tree_seen;
+    p.drafts = drafts;
+    p.heads = heads;
+    p.tiles = tt.tiles;
+    p.tile_drafts = tt.tile_drafts;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // a few tiles chain decode -> merge -> next decode (see run_split_decode)
+    const bool chain = tiles < 8;
+    p.chain = chain ? 1 : 0;
+    if (empty) {
+        wl.cost_off = nullptr;  // no items: the merge of nothing
+        wl.chunk = 0;
+        wl.seq_len = 0;
+    } else {
+        TcMaps maps;
+        st = make_tmap_pool_groups(&maps.cmap_s, kv_pages, pool_rows, kBf16);
+        if (st == MLA_B200_OK) st = make_tmap_blocks(&maps.cmap_o, kv_pages, pool_rows, tc::kTO, tc::kVBlocks, kBf16);
+        if (st == MLA_B200_OK) st = make_tmap_576(&maps.qmap, query, (long long)batch * drafts * heads, 128, kBf16);
+        if (st != MLA_B200_OK) return st;
+        if (planned_here) {
+            p.seq_lens = seq_lens;
+            p.max_seq_len = longest;
+            p.plan_cost = L.item_off;
+            p.plan_cu = L.cu_virtual;
+        } else {
+            const TreePlan plan = {p.mask, p.mask_stride, drafts, tt.tiles, tt.tile_drafts, L.tree_seen};
+            if (balanced)
+                plan_balanced_kernel<<<1, 1024, 0, s>>>(nullptr, (int)tiles, wl.item_cost, L.item_off, seq_lens, longest,
+                                                        L.cu_virtual, 1, longest, plan);
+            else
+                plan_varlen_kernel<<<1, 1024, 0, s>>>(nullptr, (int)tiles, chunk, L.item_off, L.items, (int)max_items,
+                                                      seq_lens, longest, L.cu_virtual, 1, longest, plan);
+        }
+        p.wl = wl;
+        timing_mark(t_ev_start, s);
+        const dim3 grid(2 * clusters), block(tree::kThreads);
+        if (balanced)
+            launch_dependent(tree::decode_kernel<kSchedBalanced, kBf16>, grid, block, tree::kSmemBytes, s,
+                             !planned_here || chain, maps.cmap_s, maps.cmap_o, maps.qmap, p);
+        else
+            launch_dependent(tree::decode_kernel<kSchedChunked, kBf16>, grid, block, tree::kSmemBytes, s, true,
+                             maps.cmap_s, maps.cmap_o, maps.qmap, p);
+        timing_mark(t_ev_stop, s);
+    }
+    p.wl = wl;
+    if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(L, p, s, chain);
+    else launch_tree_merge<T>(L, p, s, chain);
+    return launch_status();
 }
 }  // namespace
 

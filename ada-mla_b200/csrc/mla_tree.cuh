@@ -20,8 +20,8 @@
 //
 //   * the softmax of a tile is shared by two warpgroups, 48 columns each: with one,
 //     its 1.2 us a tile were longer than everything else on the S-CTA.  They exchange
-//     row maxima in shared memory; one barrier serves the exchange, the staging
-//     buffer and errors, a second one precedes the message;
+//     row maxima in shared memory behind one barrier; a warp of its own sends the
+//     messages, so that nobody else waits for the O-CTA;
 //   * the producer warp holds the block-table entries of ten tiles (30 pieces of 32
 //     rows), a lane each, and loads the next ten ahead;
 //   * rows of a C tile that no draft of the tile may see (past the sequence's end, or
@@ -31,9 +31,12 @@
 //   * partials are fp32: a 16-bit partial would add a third rounding of the size of
 //     the output's own.
 //
+//   * the schedule is made inside the kernel (plan_here).
+//
 // Roles (384 threads): warp 0 TMA producer, warps 1 and 3 MMA issuers (GEMM1 alternates
-// between them; GEMM2 has one), warp 2 TMEM owner and (O-CTA) row zeroing, warps 4-11
-// math: thread h of each warpgroup owns row h.  Every wait is bounded.
+// between them; GEMM2 has one), warp 2 TMEM owner and message sender (S-CTA) or row
+// zeroing (O-CTA), warps 4-11 math: thread h of each warpgroup owns row h.  Every wait
+// is bounded.
 #pragma once
 
 #include "mla_combine.cuh"
@@ -89,7 +92,9 @@ enum BarId {
     kBarMmaDone = kBarCorr + kMsgSlots, // [3] O-CTA: GEMM2 of a message done
     kBarTail = kBarMmaDone + kMsgSlots, // [4] O-CTA: slot landed, hidden rows not yet zeroed
     kBarDrain = kBarTail + kSlotsO,     // [2] an issuer's operations retired
-    kNumBars = kBarDrain + 2
+    kBarStaged = kBarDrain + 2,         //     S-CTA: a message is in the staging buffer (256)
+    kBarStgFree = kBarStaged + 1,       //     S-CTA: it has left it
+    kNumBars = kBarStgFree + 1
 };
 static_assert(kSlotsS >= kSlotsO, "ring barriers");
 
@@ -102,7 +107,13 @@ static_assert(kMsgBytes % 1024 == 0, "swizzle atoms of the message slots");
 constexpr int kOffSlot = kOffBar + kNumBars * 8;
 constexpr int kOffAbort = kOffSlot + 4;
 constexpr int kOffMax = (kOffAbort + 4 + 15) / 16 * 16;     // S-CTA: row maxima [2 tiles][2 halves][128]
-constexpr int kSmemBytes = kOffMax + 2 * 2 * 128 * 4 + 1024;
+// The plan of up to kPlanMax row tiles, made by every CTA for itself: offsets of the
+// tiles' sequences on a virtual packed axis, places on the cost line, drafts seen.
+constexpr int kPlanMax = 960;
+constexpr int kOffSeen = kOffMax + 2 * 2 * 128 * 4;
+constexpr int kOffCu = kOffSeen + kPlanMax * 8;
+constexpr int kOffCost = kOffCu + (kPlanMax + 4) * 4;
+constexpr int kSmemBytes = kOffCost + (kPlanMax + 4) * 4 + 1024;
 static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
 constexpr uint32_t kTmemCols = 512, kTmemQ = 0, kTmemS = 288;
 
@@ -119,7 +130,10 @@ struct TreeParams {
     const int32_t *block_table;
     int max_blocks, page_size, num_pages;
     const unsigned long long *mask;   // [batch or 1, drafts]; null: a chain
-    const unsigned long long *seen;   // [tiles of all sequences] (TreePlan)
+    const unsigned long long *seen;   // [tiles of all sequences], made by a plan kernel; or, with
+    const int32_t *seq_lens;          // seq_lens, made in the kernel (null: by a plan kernel)
+    int max_seq_len;
+    int *plan_cost, *plan_cu;         // with seq_lens: cost line and offsets for the merge kernel
     int mask_stride;                  // drafts, or 0 (one mask for all)
     int drafts, heads, tiles, tile_drafts;
 };
@@ -142,9 +156,65 @@ __device__ __forceinline__ uint32_t tree_word(unsigned long long mask, int start
 }
 
 // First token of the drafts of tile v's sequence (below 0 when it is shorter).
-__device__ __forceinline__ int draft_start(const TreeParams &p, int v) {
-    return p.wl.cu_seqlens[v + 1] - p.wl.cu_seqlens[v] - p.drafts;
+__device__ __forceinline__ int draft_start(const WorkList &wl, const TreeParams &p, int v) {
+    return wl.cu_seqlens[v + 1] - wl.cu_seqlens[v] - p.drafts;
 }
+
+// The balanced schedule's tables (lens_to_offsets, plan_balanced_kernel and plan_tree in
+// one) in this CTA's shared memory, by all its threads: a scan over up to kPlanMax
+// tiles takes about a microsecond, a plan kernel before this one cost four and a launch.
+__device__ void plan_here(const TreeParams &p, int ntiles, int item_cost, int *cu, int *cost,
+                          unsigned long long *seen) {
+    constexpr int kPer = (kPlanMax + kThreads - 1) / kThreads;
+    __shared__ int2 warp_tot[kThreads / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const TreePlan tp = {p.mask, p.mask_stride, p.drafts, p.tiles, p.tile_drafts, seen};
+    int2 own[kPer], sum = make_int2(0, 0);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int v = tid * kPer + k;
+        own[k] = make_int2(0, 0);
+        if (v < ntiles) {
+            const int len = min(max(p.seq_lens[v / p.tiles], 0), p.max_seq_len);
+            own[k] = make_int2(len, len > 0 ? (len + kTile - 1) / kTile + item_cost : 0);
+            plan_tree(tp, v);
+        }
+        sum.x += own[k].x;
+        sum.y += own[k].y;
+    }
+    int2 v2 = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, v2.x, o), y = __shfl_up_sync(0xffffffffu, v2.y, o);
+        if (lane >= o) {
+            v2.x += x;
+            v2.y += y;
+        }
+    }
+    if (lane == 31) warp_tot[warp] = v2;
+    __syncthreads();
+    int2 at = make_int2(v2.x - sum.x, v2.y - sum.y);
+    for (int k = 0; k < warp; ++k) {
+        at.x += warp_tot[k].x;
+        at.y += warp_tot[k].y;
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int v = tid * kPer + k;
+        if (v <= ntiles) {  // the entry after the last tile is the total
+            cu[v] = at.x;
+            cost[v] = at.y;
+            if (blockIdx.x == 0) {
+                p.plan_cu[v] = at.x;
+                p.plan_cost[v] = at.y;
+            }
+        }
+        at.x += own[k].x;
+        at.y += own[k].y;
+    }
+    __syncthreads();
+}
+static_assert(((kPlanMax + kThreads - 1) / kThreads) * kThreads > kPlanMax, "a thread for the total's entry");
 
 // Pool row of the 32-row piece at token t of sequence b; pieces past the item's last
 // token re-read its last piece (the softmax hides them).
@@ -189,7 +259,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i) {
-            const bool math = (i >= kBarSEmpty && i < kBarSEmpty + 2) || (i >= kBarCorr && i < kBarCorr + kMsgSlots);
+            const bool math = (i >= kBarSEmpty && i < kBarSEmpty + 2) || (i >= kBarCorr && i < kBarCorr + kMsgSlots) ||
+                              i == kBarStaged;
             ptx::mbar_init(bar(i), math ? kMath : 1);
         }
         *abort_flag = 0;
@@ -209,7 +280,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + kOffSlot);
     if (p.chain) griddep_launch();  // the chained merge may place its CTAs
     griddep_wait();                 // the plan kernel's work list
-    const WorkList &wl = p.wl;
+    WorkList wl = p.wl;
+    const unsigned long long *seen_of = p.seen;
+    if (kSched == kSchedBalanced && p.seq_lens != nullptr) {
+        int *cu = reinterpret_cast<int *>(smem + kOffCu), *cost = reinterpret_cast<int *>(smem + kOffCost);
+        unsigned long long *seen = reinterpret_cast<unsigned long long *>(smem + kOffSeen);
+        plan_here(p, wl.batch, wl.item_cost, cu, cost, seen);
+        wl.cu_seqlens = cu;
+        wl.cost_off = cost;
+        seen_of = seen;
+    }
     ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
     Item it;
     int id;
@@ -230,8 +310,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 return pool_row(p, b, it.tok0 + (piece + min(lane, kRowTiles * kOPerS - 1)) * kTO, last);
             };
             int row = 0, row_next = rows_from(0);
-            const int start = draft_start(p, it.b);
-            const unsigned long long seen = role == 1 ? p.seen[it.b] : 0;
+            const int start = draft_start(wl, p, it.b);
+            const unsigned long long seen = role == 1 ? seen_of[it.b] : 0;
             if (role == 0 && it.b != prev_b && lane == 0) {
                 // Q of the new tile: two 128 x 64 boxes per ring slot
                 long long r0;
@@ -427,10 +507,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         uint32_t uses = 0;      // per slot: parity of its next hidden tile
         bool ok = true;
         while (ok && items_next<kSched>(wl, cur, it, id)) {
-            const int start = draft_start(p, it.b);
+            const int start = draft_start(wl, p, it.b);
             const int pieces = (it.len + kTO - 1) / kTO;
             if (it.tok0 + it.len > start) {
-                const unsigned long long seen = p.seen[it.b];
+                const unsigned long long seen = seen_of[it.b];
                 for (int q = max(0, (start - it.tok0) / kTO - 1); ok && q < pieces; ++q) {
                     const int t = it.tok0 + q * kTO;
                     if (t + kTO <= start) continue;
@@ -455,6 +535,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             at += pieces;
         }
         if (!ok) *abort_flag = 1;
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ S-CTA: message sender
+        if (lane == 0) {
+            const uint32_t peer_pfull0 = ptx::mapa(bar(kBarPFull), 1);
+            const uint32_t peer_msg0 = ptx::mapa(sbase + kOffMsg, 1);
+            uint32_t jt = 0;
+            bool ok = true;
+            while (ok && items_next<kSched>(wl, cur, it, id)) {
+                for (int t0 = 0; t0 < it.len; t0 += kTS, ++jt) {
+                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                    // the O-CTA's slot is free once GEMM2 of S tile jt - 3 finished
+                    ok = !*abort_flag && ptx::mbar_wait<true>(bar(kBarPFree + ms), (mu & 1) ^ 1, kErrWaitPeer) &&
+                         ptx::mbar_wait(bar(kBarStaged), jt & 1, kErrWaitMma);
+                    if (!ok) break;
+                    const uint32_t rbar = peer_pfull0 + 8u * ms;
+                    ptx::mbar_remote_arrive_expect_tx(rbar, kMsgBytes);
+                    ptx::bulk_copy_s2cluster(peer_msg0 + ms * kMsgBytes, sbase + kOffStg, kMsgBytes, rbar);
+                    ptx::bulk_commit_group();
+                    ptx::bulk_wait_group_read<0>();
+                    ptx::mbar_arrive(bar(kBarStgFree));
+                }
+            }
+            if (!ok) *abort_flag = 1;
+            // The last messages were consumed by the peer's GEMM2 (so no remote arrival is
+            // still in flight towards this CTA).
+            for (uint32_t k = (jt >= (uint32_t)kMsgSlots ? jt - kMsgSlots : 0); k < jt; ++k)
+                ptx::mbar_wait<true>(bar(kBarPFree + (k % kMsgSlots)), (k / kMsgSlots) & 1, kErrWaitPeer);
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ math warpgroups
         const int h = (tid - 128) & 127;            // row = TMEM lane
@@ -464,9 +573,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bool ok = true;
         if (role == 0) {
             // ------------------------------------------------ S-CTA: softmax
-            const uint32_t peer_pfull0 = ptx::mapa(bar(kBarPFull), 1);
-            const uint32_t peer_msg0 = ptx::mapa(sbase + kOffMsg, 1);
-            const bool sender = tid == 128;
             float *maxima = reinterpret_cast<float *>(smem + kOffMax);
             const float sl2 = p.scale_log2;
             while (ok && items_next<kSched>(wl, cur, it, id)) {
@@ -476,10 +582,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 const int d = min((it.b - b * p.tiles) * p.tile_drafts + h / p.heads, p.drafts - 1);
                 unsigned long long mask = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
                 if (p.drafts < 64) mask &= (1ull << p.drafts) - 1;
-                const int start = draft_start(p, it.b) - it.tok0 - half * kHalf;
+                const int start = draft_start(wl, p, it.b) - it.tok0 - half * kHalf;
                 for (int t0 = 0; t0 < it.len; t0 += kTS, ++jt) {
                     const uint32_t sb = jt & 1, use = jt >> 1;
-                    const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
                     const bool last = t0 + kTS >= it.len;
                     // Every decision is uniform over the warpgroups (bar.red below), so an
                     // expired wait never splits a warp at a .sync.aligned instruction.
@@ -509,8 +614,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         own = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
                         maxima[(sb * 2 + half) * 128 + h] = own;
                     }
-                    // the previous message has left the staging buffer, both maxima are there
-                    if (sender) ptx::bulk_wait_group_read<0>();
                     if (!ptx::named_barrier_and(1, kMath, w)) { ok = false; break; }
                     const float mx = fmaxf(own, maxima[(sb * 2 + (half ^ 1)) * 128 + h]) * sl2;
                     float alpha = 1.f;
@@ -530,6 +633,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         pk[k >> 1] = tc::pack2<kBf16>(p0, p1);
                     }
                     l_run = l_run * alpha + ((s4[0] + s4[1]) + (s4[2] + s4[3]));
+                    // the previous message has left the staging buffer (a wait that runs out
+                    // is noticed at the next tile's barrier)
+                    if (!ptx::mbar_wait(bar(kBarStgFree), (jt & 1) ^ 1, kErrWaitPeer)) *abort_flag = 1;
                     uint8_t *msg = smem + kOffStg;
 #pragma unroll
                     for (int q = 0; q < kHalf / 8; ++q) {  // 16-byte pieces of 8 tokens
@@ -543,26 +649,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         if (half == 0) reinterpret_cast<float *>(msg + kMsgM)[h] = m_used;
                     }
                     ptx::fence_proxy_async_smem();
-                    ptx::named_barrier(1, kMath);
-                    if (sender) {
-                        // the O-CTA's slot is free once GEMM2 of S tile jt - 3 finished
-                        if (ptx::mbar_wait<true>(bar(kBarPFree + ms), (mu & 1) ^ 1, kErrWaitPeer)) {
-                            const uint32_t rbar = peer_pfull0 + 8u * ms;
-                            ptx::mbar_remote_arrive_expect_tx(rbar, kMsgBytes);
-                            ptx::bulk_copy_s2cluster(peer_msg0 + ms * kMsgBytes, sbase + kOffStg, kMsgBytes, rbar);
-                            ptx::bulk_commit_group();
-                        } else {
-                            *abort_flag = 1;  // everyone leaves at the next tile's barrier, or below
-                        }
-                    }
+                    ptx::mbar_arrive(bar(kBarStaged));
                 }
             }
             if (!ok) *abort_flag = 1;
-            // The last messages were consumed by the peer's GEMM2 (so no remote arrival
-            // is still in flight towards this CTA).
-            for (uint32_t k = (jt >= (uint32_t)kMsgSlots ? jt - kMsgSlots : 0); k < jt; ++k)
-                ptx::mbar_wait<true>(bar(kBarPFree + (k % kMsgSlots)), (k / kMsgSlots) & 1, kErrWaitPeer);
-            if (sender) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         } else {
             // ------------------------------------------------ O-CTA: correction + epilogue
             // (each warpgroup its half of O's columns)
@@ -696,6 +786,22 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
     if (r >= rows) return;                  // (with kRowWarps > 1 a block has one row)
     const int n = i1 - i0;
     const float *lse0 = part_lse + (size_t)i0 * p.num_heads + r;
+    const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)i0 * p.num_heads + r) * kDV) + lane;
+    const size_t step = (size_t)p.num_heads * (kDV / 4);
+    // the first splits' partials are on their way before the weights are known
+    constexpr int kAhead = 4;
+    float4 u[kAhead][4];
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int sj = s + j * kRowWarps;
+            if (sj < n) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) u[j][q] = __ldg(src + (size_t)sj * step + q * 32);
+            }
+        }
+    };
+    fetch(g);
     float mx = -INFINITY;
     for (int s = lane; s < n; s += 32) mx = fmaxf(mx, lse0[(size_t)s * p.num_heads]);
     mx = warp_max(mx);
@@ -704,32 +810,20 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
     float wsum = 0.f;
     if (mx != -INFINITY) {
-        const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)i0 * p.num_heads + r) * kDV) + lane;
-        const size_t step = (size_t)p.num_heads * (kDV / 4);
-        constexpr int kAhead = 4;
         for (int s = g; s < n; s += kRowWarps * kAhead) {
-            float4 u[kAhead][4];
-            float w[kAhead];
+            if (s != g) fetch(s);
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const int sj = s + j * kRowWarps;
-                w[j] = 0.f;
-                if (sj < n) {
-                    w[j] = __expf(lse0[(size_t)sj * p.num_heads] - mx);  // exp(-inf) = 0
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) u[j][q] = __ldg(src + (size_t)sj * step + q * 32);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                if (w[j] > 0.f) {  // (a split that saw nothing holds zeros)
-                    wsum += w[j];
+                const float w = sj < n ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;  // exp(-inf) = 0
+                if (w > 0.f) {  // (a split that saw nothing holds zeros)
+                    wsum += w;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        acc[4 * q] = fmaf(w[j], u[j][q].x, acc[4 * q]);
-                        acc[4 * q + 1] = fmaf(w[j], u[j][q].y, acc[4 * q + 1]);
-                        acc[4 * q + 2] = fmaf(w[j], u[j][q].z, acc[4 * q + 2]);
-                        acc[4 * q + 3] = fmaf(w[j], u[j][q].w, acc[4 * q + 3]);
+                        acc[4 * q] = fmaf(w, u[j][q].x, acc[4 * q]);
+                        acc[4 * q + 1] = fmaf(w, u[j][q].y, acc[4 * q + 1]);
+                        acc[4 * q + 2] = fmaf(w, u[j][q].z, acc[4 * q + 2]);
+                        acc[4 * q + 3] = fmaf(w, u[j][q].w, acc[4 * q + 3]);
                     }
                 }
             }
