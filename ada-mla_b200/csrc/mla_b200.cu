@@ -817,17 +817,17 @@ TreeTiles tree_tiles(int drafts, int heads) {
 }
 
 template <typename OutT>
-void launch_tree_merge(const WsLayout &L, const tree::TreeParams &p, cudaStream_t stream, bool chain) {
+void launch_tree_merge(const tree::TreeParams &p, cudaStream_t stream, bool chain) {
     // a few tiles have many splits each: a block of 8 warps per row; many tiles have one
     // or two: a warp per row
     const dim3 block(32 * tree::kMergeWarps);
     const unsigned rows = (unsigned)p.num_heads, tiles = (unsigned)p.wl.batch;
     if (tiles < 8)
         launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(rows, tiles), block, 0, stream, chain,
-                         L.part_o, L.part_lse, p.wl, p, static_cast<OutT *>(p.out), p.out_lse);
+                         p);
     else
         launch_dependent(tree::merge_kernel<OutT, 1>, dim3((unsigned)cdiv(rows, tree::kMergeWarps), tiles), block, 0,
-                         stream, chain, L.part_o, L.part_lse, p.wl, p, static_cast<OutT *>(p.out), p.out_lse);
+                         stream, chain, p);
 }
 
 template <typename T>
@@ -891,7 +891,9 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     tree::TreeParams p{};
     p.num_heads = rows;
     p.scale_log2 = softmax_scale * kLog2e;
-    p.part_o = L.part_o;
+    // (the workspace has room for fp32 partials: the 16-bit ones, then their scales)
+    p.part_o = reinterpret_cast<uint8_t *>(L.part_o);
+    p.part_scale = reinterpret_cast<float *>(p.part_o + align_up((size_t)max_items * rows * kDV * 2, 256));
     p.part_lse = L.part_lse;
     p.out = out;
     p.out_kind = out_dtype == MLA_B200_OUT_F16 ? tc::kOutF16 : out_dtype == MLA_B200_OUT_BF16 ? tc::kOutBF16 : tc::kOutF32;
@@ -924,8 +926,7 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
         if (planned_here) {
             p.seq_lens = seq_lens;
             p.max_seq_len = longest;
-            p.plan_cost = L.item_off;
-            p.plan_cu = L.cu_virtual;
+            p.plan_range = reinterpret_cast<int2 *>(L.items);  // (no chunk table here)
         } else {
             const TreePlan plan = {p.mask, p.mask_stride, drafts, tt.tiles, tt.tile_drafts, L.tree_seen};
             if (balanced)
@@ -947,8 +948,8 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
         timing_mark(t_ev_stop, s);
     }
     p.wl = wl;
-    if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(L, p, s, chain);
-    else launch_tree_merge<T>(L, p, s, chain);
+    if (out_dtype == MLA_B200_OUT_F32) launch_tree_merge<float>(p, s, chain);
+    else launch_tree_merge<T>(p, s, chain);
     return launch_status();
 }
 }  // namespace

@@ -589,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool real = row < it.s.lq;
             const long long orow = (long long)(it.s.q0 + row) * p.heads + it.h;
             uint8_t *dst = static_cast<uint8_t *>(p.out) + orow * (kV * 2);
-            const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+            const float inv = l_run != 0.f ? 1.f / l_run : 0.f;  // (NaN stays NaN)
             if (n > 0) {
                 ok = __all_sync(0xffffffffu, wait_bar(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
                 if (!ok) break;
@@ -616,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             ptx::tc_fence_before();  // O is read before this thread's next P arrival lets a PV overwrite it
             if (real && p.out_lse != nullptr)
-                p.out_lse[orow] = l_run > 0.f ? (m_used + __log2f(l_run)) * kLn2 : -INFINITY;
+                p.out_lse[orow] = l_run != 0.f ? (m_used + __log2f(l_run)) * kLn2 : -INFINITY;
         }
         if (!ok) *abort_flag = 1;
     }

@@ -28,8 +28,13 @@
 //     padded drafts that may never have been written) are zeroed by a warp of their own
 //     before GEMM2 (0 x NaN is not 0): such tiles land on that warp's barrier, which
 //     then completes the slot's.  No other tile pays for it;
-//   * partials are fp32: a 16-bit partial would add a third rounding of the size of
-//     the output's own.
+//   * partials are 16-bit whole numbers with an fp32 scale for every 32 columns of a row
+//     (its largest value / 32767): half the bytes of fp32, whose 256 KB an item took one SM
+//     8 us to store, and an error of 2^-16 of the largest of 32 neighbours (about 2e-5 of
+//     a typical value), where a 16-bit float's 2^-12 would add a third rounding of the
+//     size of the output's own.  They lie 32 bytes (16 columns) of all rows together, so a
+//     warp's store is one kilobyte in a row.  (A partial that is not finite makes its 32
+//     columns NaN.)
 //
 //   * the schedule is made inside the kernel (plan_here).
 //
@@ -121,7 +126,8 @@ struct TreeParams {
     WorkList wl;
     int num_heads;     // rows of a full tile = rows between partials: tile_drafts * heads
     float scale_log2;  // softmax scale * log2(e)
-    float *part_o;     // [items, num_heads, 512]
+    uint8_t *part_o;   // [items, 32 pieces, num_heads, 16] int16: see part_piece
+    float *part_scale; // [items, 16 chunks, num_heads]
     float *part_lse;   // [items, num_heads]
     void *out;         // [batch, drafts, heads, 512]: written directly for tiles of one item
     int out_kind;      // tc::OutKind
@@ -133,7 +139,7 @@ struct TreeParams {
     const unsigned long long *seen;   // [tiles of all sequences], made by a plan kernel; or, with
     const int32_t *seq_lens;          // seq_lens, made in the kernel (null: by a plan kernel)
     int max_seq_len;
-    int *plan_cost, *plan_cu;         // with seq_lens: cost line and offsets for the merge kernel
+    int2 *plan_range;                 // with seq_lens: every tile's items, for the merge kernel
     int mask_stride;                  // drafts, or 0 (one mask for all)
     int drafts, heads, tiles, tile_drafts;
 };
@@ -168,17 +174,28 @@ __device__ void plan_here(const TreeParams &p, int ntiles, int item_cost, int *c
     constexpr int kPer = (kPlanMax + kThreads - 1) / kThreads;
     __shared__ int2 warp_tot[kThreads / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const TreePlan tp = {p.mask, p.mask_stride, p.drafts, p.tiles, p.tile_drafts, seen};
     int2 own[kPer], sum = make_int2(0, 0);
+    int lens[kPer];
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
         const int v = tid * kPer + k;
-        own[k] = make_int2(0, 0);
-        if (v < ntiles) {
-            const int len = min(max(p.seq_lens[v / p.tiles], 0), p.max_seq_len);
-            own[k] = make_int2(len, len > 0 ? (len + kTile - 1) / kTile + item_cost : 0);
-            plan_tree(tp, v);
+        lens[k] = v < ntiles ? p.seq_lens[v / p.tiles] : 0;
+    }
+    // the drafts seen, a thread per (tile, draft): one round of loads, beside the lengths'
+    for (int v = tid; v < ntiles; v += kThreads) seen[v] = 0;
+    __syncthreads();
+    for (int i = tid; i < ntiles * p.tile_drafts; i += kThreads) {
+        const int v = i / p.tile_drafts, b = v / p.tiles;
+        const int d = (v - b * p.tiles) * p.tile_drafts + (i - v * p.tile_drafts);
+        if (d < p.drafts) {
+            const unsigned long long m = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
+            atomicOr(seen + v, p.drafts < 64 ? m & ((1ull << p.drafts) - 1) : m);
         }
+    }
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+        const int len = min(max(lens[k], 0), p.max_seq_len);
+        own[k] = make_int2(len, len > 0 ? (len + kTile - 1) / kTile + item_cost : 0);
         sum.x += own[k].x;
         sum.y += own[k].y;
     }
@@ -204,10 +221,6 @@ __device__ void plan_here(const TreeParams &p, int ntiles, int item_cost, int *c
         if (v <= ntiles) {  // the entry after the last tile is the total
             cu[v] = at.x;
             cost[v] = at.y;
-            if (blockIdx.x == 0) {
-                p.plan_cu[v] = at.x;
-                p.plan_cost[v] = at.y;
-            }
         }
         at.x += own[k].x;
         at.y += own[k].y;
@@ -224,6 +237,23 @@ __device__ __forceinline__ int pool_row(const TreeParams &p, int b, int t, int l
     // (an entry that is no page: the row after the pool, which TMA reads as zeros)
     const int pg = (int)min((unsigned)p.block_table[(long long)b * p.max_blocks + blk], (unsigned)p.num_pages);
     return pg * p.page_size + (tc - blk * p.page_size);
+}
+
+// Byte offset of 16 columns (16 piece ..) of row r of an item's partial.
+__device__ __forceinline__ size_t part_piece(const TreeParams &p, int item, int piece, int r) {
+    return (((size_t)item * (kDV / 16) + piece) * p.num_heads + r) * 32;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+
+// A 16-bit whole number as fp32, without the conversion instruction: its bits with the
+// sign flipped are the last of 2^23 + 2^15 + x.
+__device__ __forceinline__ float f32_of_i16(uint32_t x) {
+    return tc::f32_of((x & 0xffffu) ^ 0x4b008000u) - 8421376.f;
 }
 
 __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -289,6 +319,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         wl.cu_seqlens = cu;
         wl.cost_off = cost;
         seen_of = seen;
+        if (blockIdx.x == 0) {
+            for (int v = tid; v < wl.batch; v += kThreads) {
+                int i0, i1;
+                item_range<kSched>(wl, v, i0, i1);
+                p.plan_range[v] = make_int2(i0, i1);
+            }
+        }
     }
     ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
     Item it;
@@ -312,23 +349,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             int row = 0, row_next = rows_from(0);
             const int start = draft_start(wl, p, it.b);
             const unsigned long long seen = role == 1 ? seen_of[it.b] : 0;
-            if (role == 0 && it.b != prev_b && lane == 0) {
-                // Q of the new tile: two 128 x 64 boxes per ring slot
-                long long r0;
+            // Q of a new row tile goes through the ring too, two 128 x 64 boxes (K-blocks) to
+            // a slot, in front of the first S tile's slots that need them: Q01 Q23 C012 Q45
+            // C345 Q67 Q8 C678, so that the two come in together.
+            const bool new_q = role == 0 && it.b != prev_b;
+            prev_b = it.b;
+            long long q_row = 0;
+            if (new_q) {
                 int n;
-                tree_rows(p, it.b, r0, n);
-                for (int kb = 0; kb < kKBlocks; kb += 2) {
-                    if (!acquire()) { ok = false; break; }
+                tree_rows(p, it.b, q_row, n);
+            }
+            auto load_q = [&](int slots, int kb) {
+                for (int c = 0; c < slots; ++c, kb += 2) {
+                    if (!ok || !acquire()) { ok = false; return; }
                     const int nb = min(2, kKBlocks - kb);
                     const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
                     ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), nb * kQBoxBytes);
                     for (int j = 0; j < nb; ++j)
-                        ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)r0, bar(kBarFull + rg.slot));
+                        ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)q_row, bar(kBarFull + rg.slot));
                     rg.next(nslots);
                 }
-            }
-            prev_b = it.b;
-            ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+            };
             for (int t0 = 0; ok && t0 < it.len; t0 += kTS) {
                 const int piece = t0 / kTO, at = piece % (kRowTiles * kOPerS);
                 if (at == 0) {
@@ -341,7 +382,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (lane == 0) {
                     if (role == 0) {
                         for (int sl = 0; sl < kSlotsPerTile; ++sl) {
-                            if (!acquire()) { ok = false; break; }
+                            if (new_q && t0 == 0) load_q(sl == 1 ? 1 : 2, sl == 0 ? 0 : sl == 1 ? 4 : 6);
+                            if (!ok || !acquire()) { ok = false; break; }
                             const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
                             ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kSlotS);
 #pragma unroll
@@ -449,7 +491,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                             ptx::tc_fence_after();
                         }
-                        for (int kb = 0; kb < kKBlocks; kb += 2) {
+                        qready_seq = nseq;
+                    } else {
+                        for (int q = 0; q < kQSlots; ++q) rg.next(kSlotsS);
+                    }
+                }
+                if (!mine) {
+                    for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(kSlotsS);
+                    continue;
+                }
+                const bool copy_q = new_seq && t0 == 0;  // this issuer copies Q on the way
+                if (qready_seq != nseq) {  // the other issuer copied this tile's Q
+                    ok &= ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma);
+                    qready_seq = nseq;
+                }
+                const uint32_t sb = jt & 1, use = jt >> 1;
+                ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
+                const uint32_t d = tmem + kTmemS + sb * kTS;
+                for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                    if (copy_q) {  // K-blocks 0-3, 4-5, 6-8 of Q (see the producer)
+                        const int kb0 = sl == 0 ? 0 : sl == 1 ? 4 : 6, kb1 = sl == 0 ? 4 : sl == 1 ? 6 : kKBlocks;
+                        for (int kb = kb0; kb < kb1; kb += 2) {
                             ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
                             const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
                             const int nb = min(2, kKBlocks - kb);
@@ -462,26 +526,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
                             rg.next(kSlotsS);
                         }
-                        ptx::mma_commit_if(e, bar(kBarQReady));
-                        qready_seq = nseq;
-                    } else {
-                        for (int q = 0; q < kQSlots; ++q) rg.next(kSlotsS);
+                        if (sl == kSlotsPerTile - 1) ptx::mma_commit_if(e, bar(kBarQReady));
                     }
-                }
-                if (!mine) {
-                    for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(kSlotsS);
-                    continue;
-                }
-                if (qready_seq != nseq) {  // the other issuer copied this tile's Q
-                    ok &= ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma);
-                    qready_seq = nseq;
-                }
-                const uint32_t sb = jt & 1, use = jt >> 1;
-                ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
-                const uint32_t d = tmem + kTmemS + sb * kTS;
-                for (int sl = 0; sl < kSlotsPerTile; ++sl) {
                     ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
                     const uint32_t acc0 = sl > 0 ? 1u : 0u;
                     // the slot's K-blocks interleave per 8-row group: groups 3 KB apart
@@ -706,17 +752,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         const bool single = i1 - i0 == 1;
                         long long row0;
                         tree_rows(p, it.b, row0, nrows);
-                        const float inv_l = l_fin > 0.f ? 1.f / l_fin : 0.f;
-                        const bool f32 = !single || p.out_kind == tc::kOutF32;
+                        const float inv_l = l_fin != 0.f ? 1.f / l_fin : 0.f;  // (NaN stays NaN)
+                        const bool f32 = p.out_kind == tc::kOutF32;
                         const size_t row = single ? (size_t)row0 + h : (size_t)id * p.num_heads + h;
-                        uint8_t *dst = (single ? static_cast<uint8_t *>(p.out) : reinterpret_cast<uint8_t *>(p.part_o)) +
-                                       (row * kDV + half * (kDV / 2)) * (f32 ? 4 : 2);
+                        uint8_t *dst = static_cast<uint8_t *>(p.out) + (row * kDV + half * (kDV / 2)) * (f32 ? 4 : 2);
 #pragma unroll 1
                         for (int c = 0; c < kDV / 64; ++c) {
                             uint32_t r[32];
                             ptx::tmem_ld_x32(o_addr + c * 32, r);
                             ptx::tmem_wait_ld();
-                            if (f32) {
+                            if (!single) {
+                                float top[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) top[k & 3] = max_nan(top[k & 3], fabsf(tc::f32_of(r[k])));
+                                const float most = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
+                                const float up = most > 0.f ? 32767.f / most : 0.f;
+                                // round(x * up) by the addition of 1.5 * 2^23, whose low bits then
+                                // are the whole number (a conversion instruction has a quarter of
+                                // an addition's rate: 4096 cycles an item)
+                                uint32_t o[16];
+#pragma unroll
+                                for (int k = 0; k < 16; ++k)
+                                    o[k] = __byte_perm(tc::u32_of(fmaf(tc::f32_of(r[2 * k]), up, 12582912.f)),
+                                                       tc::u32_of(fmaf(tc::f32_of(r[2 * k + 1]), up, 12582912.f)), 0x5410);
+                                if (h < nrows) {
+                                    const int piece = half * (kDV / 32) + 2 * c;
+                                    store32(p.part_o + part_piece(p, id, piece, h), o);
+                                    store32(p.part_o + part_piece(p, id, piece + 1, h), o + 8);
+                                    p.part_scale[((size_t)id * (kDV / 32) + piece / 2) * p.num_heads + h] =
+                                        most * (1.f / 32767.f) * inv_l + most * 0.f;  // (infinite: NaN)
+                                }
+                            } else if (f32) {
 #pragma unroll
                                 for (int k = 0; k < 32; ++k) r[k] = tc::u32_of(tc::f32_of(r[k]) * inv_l);
                                 if (h < nrows) {
@@ -735,7 +801,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             }
                         }
                         if (half == 0 && h < nrows) {
-                            const float lse = l_fin > 0.f ? (m_fin + __log2f(l_fin)) * kLn2 : -INFINITY;
+                            const float lse = l_fin != 0.f ? (m_fin + __log2f(l_fin)) * kLn2 : -INFINITY;
                             if (!single) p.part_lse[row] = lse;
                             else if (p.out_lse != nullptr) p.out_lse[row] = lse;
                         }
@@ -758,22 +824,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 }
 
-// O = sum_i e^(lse_i - M) O_i / sum_i e^(lse_i - M), M = max_i lse_i, over the
-// items i of tile v that hold row r's partials (fp32: a 16-bit partial would add a
-// third rounding of the size of the output's own).  kRowWarps warps share a row
-// (each every kRowWarps-th split, joined in shared memory in a fixed order): 8
-// where a few tiles have many splits, else 1.  Rows of tiles that were one item are
-// complete already.  Bound by the partials' bytes, 2 KB a row and split.
+// O = sum_i e^(lse_i - M) O_i / sum_i e^(lse_i - M), M = max_i lse_i, over the items i
+// of tile v that hold row r's partials.  kRowWarps warps share a row (each every
+// kRowWarps-th split, joined in shared memory in a fixed order): 8 where a few tiles
+// have many splits, else 1.  Lane l owns columns 16 l .. 16 l + 15 (a piece).  Rows of
+// tiles that were one item are complete already.  Bound by the partials' bytes, 1 KB a
+// row and split, and by the latency of three dependent loads; the first splits' partials
+// are asked for before their weights are known.
 template <typename OutT, int kRowWarps>
-__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__restrict__ part_o,
-                                                                 const float *__restrict__ part_lse, WorkList wl,
-                                                                 TreeParams p, OutT *__restrict__ out,
-                                                                 float *__restrict__ out_lse) {
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParams p) {
     constexpr int kRows = kMergeWarps / kRowWarps;  // rows per block
-    __shared__ __align__(16) float acc_s[kRowWarps > 1 ? kRowWarps - 1 : 1][kDV];
+    __shared__ float acc_s[kRowWarps > 1 ? kRowWarps - 1 : 1][16][33];
     __shared__ float sum_s[kMergeWarps];
     griddep_launch();
     griddep_wait();
+    const WorkList &wl = p.wl;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int v = blockIdx.y;
     const int r = blockIdx.x * kRows + warp / kRowWarps, g = warp % kRowWarps;
@@ -781,30 +846,44 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
     int rows;
     tree_rows(p, v, row0, rows);
     int i0, i1;
-    item_range(wl, v, i0, i1);
+    if (p.plan_range != nullptr) {
+        const int2 range = p.plan_range[v];
+        i0 = range.x;
+        i1 = range.y;
+    } else {
+        item_range(wl, v, i0, i1);
+    }
     if (i1 - i0 == 1) return;               // the same for the whole block
     if (r >= rows) return;                  // (with kRowWarps > 1 a block has one row)
     const int n = i1 - i0;
-    const float *lse0 = part_lse + (size_t)i0 * p.num_heads + r;
-    const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)i0 * p.num_heads + r) * kDV) + lane;
-    const size_t step = (size_t)p.num_heads * (kDV / 4);
-    // the first splits' partials are on their way before the weights are known
+    const float *lse0 = p.part_lse + (size_t)i0 * p.num_heads + r;
+    const float *scale0 = p.part_scale + ((size_t)i0 * (kDV / 32) + lane / 2) * p.num_heads + r;
+    const uint8_t *src = p.part_o + part_piece(p, i0, lane, r);
+    const size_t step = (size_t)p.num_heads * kDV * 2;
     constexpr int kAhead = 4;
-    float4 u[kAhead][4];
+    uint4 u[kAhead][2];
+    float sc[kAhead];
     auto fetch = [&](int s) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int sj = s + j * kRowWarps;
             if (sj < n) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) u[j][q] = __ldg(src + (size_t)sj * step + q * 32);
+                const uint4 *at = reinterpret_cast<const uint4 *>(src + (size_t)sj * step);
+                u[j][0] = __ldg(at);
+                u[j][1] = __ldg(at + 1);
+                sc[j] = __ldg(scale0 + (size_t)sj * (kDV / 32) * p.num_heads);
             }
         }
     };
     fetch(g);
     float mx = -INFINITY;
-    for (int s = lane; s < n; s += 32) mx = fmaxf(mx, lse0[(size_t)s * p.num_heads]);
-    mx = warp_max(mx);
+    bool nan = false;
+    for (int s = lane; s < n; s += 32) {
+        const float l = lse0[(size_t)s * p.num_heads];
+        mx = fmaxf(mx, l);
+        nan |= l != l;
+    }
+    mx = __any_sync(0xffffffffu, nan) ? NAN : warp_max(mx);
     float acc[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -816,14 +895,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
             for (int j = 0; j < kAhead; ++j) {
                 const int sj = s + j * kRowWarps;
                 const float w = sj < n ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;  // exp(-inf) = 0
-                if (w > 0.f) {  // (a split that saw nothing holds zeros)
+                if (w != 0.f) {  // (a split that saw nothing holds zeros)
                     wsum += w;
+                    const float ws = w * sc[j];
+                    const uint32_t x[8] = {u[j][0].x, u[j][0].y, u[j][0].z, u[j][0].w,
+                                           u[j][1].x, u[j][1].y, u[j][1].z, u[j][1].w};
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        acc[4 * q] = fmaf(w, u[j][q].x, acc[4 * q]);
-                        acc[4 * q + 1] = fmaf(w, u[j][q].y, acc[4 * q + 1]);
-                        acc[4 * q + 2] = fmaf(w, u[j][q].z, acc[4 * q + 2]);
-                        acc[4 * q + 3] = fmaf(w, u[j][q].w, acc[4 * q + 3]);
+                    for (int k = 0; k < 8; ++k) {
+                        acc[2 * k] = fmaf(ws, f32_of_i16(x[k]), acc[2 * k]);
+                        acc[2 * k + 1] = fmaf(ws, f32_of_i16(x[k] >> 16), acc[2 * k + 1]);
                     }
                 }
             }
@@ -832,9 +912,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
     if constexpr (kRowWarps > 1) {
         if (g > 0) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                reinterpret_cast<float4 *>(acc_s[g - 1])[lane + q * 32] =
-                    make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
+            for (int e = 0; e < 16; ++e) acc_s[g - 1][e][lane] = acc[e];
             if (lane == 0) sum_s[g] = wsum;
         }
         __syncthreads();
@@ -843,26 +921,23 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const float *__
         for (int k = 1; k < kRowWarps; ++k) {
             wsum += sum_s[k];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const float4 a = reinterpret_cast<const float4 *>(acc_s[k - 1])[lane + q * 32];
-                acc[4 * q] += a.x;
-                acc[4 * q + 1] += a.y;
-                acc[4 * q + 2] += a.z;
-                acc[4 * q + 3] += a.w;
-            }
+            for (int e = 0; e < 16; ++e) acc[e] += acc_s[k - 1][e][lane];
         }
     }
-    const float inv = wsum > 0.f ? 1.f / wsum : 0.f;
-    OutT *dst = out + (row0 + r) * kDV + lane * 4;
+    const float inv = wsum != 0.f ? 1.f / wsum : 0.f;
+    OutT *dst = static_cast<OutT *>(p.out) + (row0 + r) * kDV + lane * 16;
+    uint32_t o[16];
+    if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const float a = acc[4 * q] * inv, b = acc[4 * q + 1] * inv, c = acc[4 * q + 2] * inv, d = acc[4 * q + 3] * inv;
-        if constexpr (sizeof(OutT) == 4)
-            *reinterpret_cast<float4 *>(dst + q * 128) = make_float4(a, b, c, d);
-        else
-            *reinterpret_cast<uint2 *>(dst + q * 128) = make_uint2(pack_out2<OutT>(a, b), pack_out2<OutT>(c, d));
+        for (int e = 0; e < 16; ++e) o[e] = tc::u32_of(acc[e] * inv);
+        store32(dst, o);
+        store32(dst + 8, o + 8);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = pack_out2<OutT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+        store32(dst, o);
     }
-    if (out_lse != nullptr && lane == 0) out_lse[row0 + r] = wsum > 0.f ? mx + __logf(wsum) : -INFINITY;
+    if (p.out_lse != nullptr && lane == 0) p.out_lse[row0 + r] = wsum != 0.f ? mx + __logf(wsum) : -INFINITY;
 }
 
 }  // namespace tree
