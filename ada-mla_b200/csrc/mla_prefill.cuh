@@ -241,24 +241,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
-// Bounded wait without a pause between tries (try_wait itself suspends for a while).
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, int err) {
-    if (ptx::mbar_try_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    for (uint32_t n = 1;; ++n) {
-        if (ptx::mbar_try_wait(bar, parity)) return true;
-        if ((n & 63) == 0) {
-            const uint64_t t = globaltimer_ns();
-            if (t0 == 0) {
-                t0 = t;
-            } else if (t - t0 > kWaitLimitNs) {
-                set_device_error(err);
-                return false;
-            }
-        }
-    }
-}
-
 // The V tail warp may have nothing to do for the whole of a long item: its limit
 // starts anew while the other roles are at work, and an abort ends it.
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
@@ -328,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool ok = true;
                 auto acquire = [&](uint32_t &full, bool tail = false) -> uint32_t {  // next slot's address, its full barrier
                     const uint32_t s = at % kSlots;
-                    if (!ok || *abort_flag || !wait_bar(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty)) {
+                    if (!ok || *abort_flag || !ptx::mbar_wait_now(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty)) {
                         ok = false;
                         return 0;
                     }
@@ -338,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return sbase + kOffRing + s * kBox;
                 };
                 auto load_q = [&](int t) {
-                    if (!ok || *abort_flag || !wait_bar(bar(kBarQEmpty + t), (qn[t] & 1) ^ 1, kErrWaitEmpty)) {
+                    if (!ok || *abort_flag || !ptx::mbar_wait_now(bar(kBarQEmpty + t), (qn[t] & 1) ^ 1, kErrWaitEmpty)) {
                         ok = false;
                         return;
                     }
@@ -520,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (p.causal) sees = min(sees, min(row, it.s.lq - 1) + 1 + it.s.lk - it.s.lq);
             float m_used = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n; ++j, ++sn) {
-                ok = !*abort_flag && wait_bar(bar(kBarS + t), sn & 1, kErrWaitMma);
+                ok = !*abort_flag && ptx::mbar_wait_now(bar(kBarS + t), sn & 1, kErrWaitMma);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 ptx::tc_fence_after();
@@ -547,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     m_used = mx;
                 }
                 if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                    ok = __all_sync(0xffffffffu, wait_bar(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait_now(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
                     if (!ok) break;
                     ptx::tc_fence_after();
 #pragma unroll 1
@@ -591,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint8_t *dst = static_cast<uint8_t *>(p.out) + orow * (kV * 2);
             const float inv = l_run != 0.f ? 1.f / l_run : 0.f;  // (NaN stays NaN)
             if (n > 0) {
-                ok = __all_sync(0xffffffffu, wait_bar(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
+                ok = __all_sync(0xffffffffu, ptx::mbar_wait_now(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
                 if (!ok) break;
                 ptx::tc_fence_after();
             }

@@ -268,6 +268,64 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
         : "memory");
 }
 
+// The same behind a predicate, for whole warps with one elected lane (see mma_ss_if).
+__device__ __forceinline__ void mbar_arrive_expect_tx_if(uint32_t lane_on, uint32_t bar, uint32_t bytes) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+        "r"(bytes), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_2d_if(uint32_t lane_on, uint32_t dst, const CUtensorMap *map, int x, int y,
+                                               uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d_if(uint32_t lane_on, uint32_t dst, const CUtensorMap *map, int x, int y,
+                                               int z, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d_if(uint32_t lane_on, uint32_t dst, const CUtensorMap *map, int x, int y,
+                                               int z, int w, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t}" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "r"(lane_on)
+        : "memory");
+}
+
+// Waits like mbar_wait, without the pause between tries: for roles on the critical path
+// that have their scheduler slot to themselves (try_wait itself suspends for a while).
+__device__ __forceinline__ bool mbar_wait_now(uint32_t bar, uint32_t parity, int err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    for (uint32_t n = 1;; ++n) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((n & 63) == 0) {
+            const uint64_t t = globaltimer_ns();
+            if (t0 == 0) {
+                t0 = t;
+            } else if (t - t0 > kWaitLimitNs) {
+                set_device_error(err);
+                return false;
+            }
+        }
+    }
+}
+
 // Bulk copy of `bytes` from this CTA's smem to another CTA's smem of the
 // cluster (dst and bar are shared::cluster addresses); completion is signalled
 // on the destination CTA's barrier.  Point to point: exactly one destination CTA.

@@ -333,44 +333,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
-        // The whole warp walks the items; lane 0 loads.
+        // (a whole warp with one elected lane, as the MMA issuers below)
+        const uint32_t e = ptx::elect_one();
         const int nslots = role == 0 ? kSlotsS : kSlotsO;
         tc::Ring rg;
         int prev_b = -1;
         bool ok = true;
-        auto acquire = [&]() -> bool {
-            return !*abort_flag && ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
+        auto acquire = [&]() {
+            ok = ok && !*abort_flag && ptx::mbar_wait_now(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
+            ok = __all_sync(0xffffffffu, ok);
         };
         while (ok && items_next<kSched>(wl, cur, it, id)) {
-            const int b = it.b / p.tiles, last = it.tok0 + it.len - 1;
+            const int len = __shfl_sync(0xffffffffu, it.len, 0), tok0 = __shfl_sync(0xffffffffu, it.tok0, 0);
+            const int v = __shfl_sync(0xffffffffu, it.b, 0), b = v / p.tiles, last = tok0 + len - 1;
             auto rows_from = [&](int piece) -> int {  // this lane's piece of ten tiles
-                return pool_row(p, b, it.tok0 + (piece + min(lane, kRowTiles * kOPerS - 1)) * kTO, last);
+                return pool_row(p, b, tok0 + (piece + min(lane, kRowTiles * kOPerS - 1)) * kTO, last);
             };
             int row = 0, row_next = rows_from(0);
-            const int start = draft_start(wl, p, it.b);
-            const unsigned long long seen = role == 1 ? seen_of[it.b] : 0;
+            const int start = draft_start(wl, p, v);
+            const unsigned long long seen = role == 1 ? seen_of[v] : 0;
             // Q of a new row tile goes through the ring too, two 128 x 64 boxes (K-blocks) to
             // a slot, in front of the first S tile's slots that need them: Q01 Q23 C012 Q45
             // C345 Q67 Q8 C678, so that the two come in together.
-            const bool new_q = role == 0 && it.b != prev_b;
-            prev_b = it.b;
+            const bool new_q = role == 0 && v != prev_b;
+            prev_b = v;
             long long q_row = 0;
             if (new_q) {
                 int n;
-                tree_rows(p, it.b, q_row, n);
+                tree_rows(p, v, q_row, n);
             }
-            auto load_q = [&](int slots, int kb) {
-                for (int c = 0; c < slots; ++c, kb += 2) {
-                    if (!ok || !acquire()) { ok = false; return; }
-                    const int nb = min(2, kKBlocks - kb);
-                    const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                    ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), nb * kQBoxBytes);
-                    for (int j = 0; j < nb; ++j)
-                        ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)q_row, bar(kBarFull + rg.slot));
-                    rg.next(nslots);
-                }
-            };
-            for (int t0 = 0; ok && t0 < it.len; t0 += kTS) {
+            for (int t0 = 0; ok && t0 < len; t0 += kTS) {
                 const int piece = t0 / kTO, at = piece % (kRowTiles * kOPerS);
                 if (at == 0) {
                     row = row_next;
@@ -379,43 +371,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 int pr[kOPerS];
 #pragma unroll
                 for (int c = 0; c < kOPerS; ++c) pr[c] = __shfl_sync(0xffffffffu, row, at + c);
-                if (lane == 0) {
-                    if (role == 0) {
-                        for (int sl = 0; sl < kSlotsPerTile; ++sl) {
-                            if (new_q && t0 == 0) load_q(sl == 1 ? 1 : 2, sl == 0 ? 0 : sl == 1 ? 4 : 6);
-                            if (!ok || !acquire()) { ok = false; break; }
-                            const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                            ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kSlotS);
-#pragma unroll
-                            for (int c = 0; c < kOPerS; ++c)
-                                ptx::tma_load_4d(dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3,
-                                                 bar(kBarFull + rg.slot));
-                            rg.next(nslots);
+                if (role == 0) {
+#pragma unroll 1
+                    for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                        if (new_q && t0 == 0) {
+                            int kb = sl == 0 ? 0 : sl == 1 ? 4 : 6;
+#pragma unroll 1
+                            for (int c = sl == 1 ? 1 : 0; c < 2 && ok; ++c, kb += 2) {
+                                acquire();
+                                if (!ok) break;
+                                const int nb = min(2, kKBlocks - kb);
+                                const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
+                                ptx::mbar_arrive_expect_tx_if(e, bar(kBarFull + rg.slot), nb * kQBoxBytes);
+                                for (int j = 0; j < nb; ++j)
+                                    ptx::tma_load_2d_if(e, dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)q_row,
+                                                        bar(kBarFull + rg.slot));
+                                rg.next(nslots);
+                            }
                         }
-                    } else {
-                        const int nct = (min(kTS, it.len - t0) + kTO - 1) / kTO;
+                        acquire();
+                        if (!ok) break;
+                        const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
+                        ptx::mbar_arrive_expect_tx_if(e, bar(kBarFull + rg.slot), kSlotS);
 #pragma unroll
-                        for (int ct = 0; ct < kOPerS; ++ct) {
-                            if (ct >= nct || !ok) break;
-                            if (!acquire()) { ok = false; break; }
-                            const int t = it.tok0 + t0 + ct * kTO;
-                            const bool hidden = t + kTO > start && tree_word(seen, start, t) != 0xffffffffu;
-                            const uint32_t full = bar((hidden ? kBarTail : kBarFull) + rg.slot);
-                            ptx::mbar_arrive_expect_tx(full, kSlotO);
-                            ptx::tma_load_3d(sbase + kOffRing + rg.slot * kSlotO, &cmap_o, 0, pr[ct], 0, full);
-                            rg.next(nslots);
-                        }
+                        for (int c = 0; c < kOPerS; ++c)
+                            ptx::tma_load_4d_if(e, dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3,
+                                                bar(kBarFull + rg.slot));
+                        rg.next(nslots);
+                    }
+                } else {
+                    const int nct = (min(kTS, len - t0) + kTO - 1) / kTO;
+#pragma unroll
+                    for (int ct = 0; ct < kOPerS; ++ct) {
+                        if (ct >= nct) break;
+                        acquire();
+                        if (!ok) break;
+                        const int t = tok0 + t0 + ct * kTO;
+                        const bool hidden = t + kTO > start && tree_word(seen, start, t) != 0xffffffffu;
+                        const uint32_t full = bar((hidden ? kBarTail : kBarFull) + rg.slot);
+                        ptx::mbar_arrive_expect_tx_if(e, full, kSlotO);
+                        ptx::tma_load_3d_if(e, sbase + kOffRing + rg.slot * kSlotO, &cmap_o, 0, pr[ct], 0, full);
+                        rg.next(nslots);
                     }
                 }
-                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
             }
         }
-        if (lane == 0) {
-            if (!ok) *abort_flag = 1;
-            // drain: every issued load has been consumed (or the wait expires)
-            for (int k = 0; k < nslots; ++k, rg.next(nslots))
-                ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
-        }
+        if (!ok) *abort_flag = 1;
+        // drain: every issued load has been consumed (or the wait expires)
+        for (int k = 0; k < nslots; ++k, rg.next(nslots))
+            ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
     } else if (warp == 1 && role == 1) {
         // ------------------------------------------------------------ O-CTA: GEMM2
         // (The issuing warps run as whole warps with uniform control flow and one elected
