@@ -7,6 +7,7 @@
 // the C ABI (include/mla_b200.h) on the current torch stream; a non-zero status
 // raises.  No torch types cross the C ABI.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -30,6 +31,32 @@ void check_cuda(const at::Tensor &t, const char *name) {
 }
 
 void *stream_ptr() { return static_cast<void *>(at::cuda::getCurrentCUDAStream().stream()); }
+
+// An uninitialised tensor straight from the caching allocator (at::empty without its
+// dispatch: about a microsecond less, which is what a step of small calls is made of).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor &like) {
+    return at::Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
+}
+
+// Tensors that share one allocation, each at a multiple of 16 bytes.
+class Carve {
+  public:
+    Carve(int64_t bytes, const at::Tensor &like) : base_(fresh({std::max<int64_t>(bytes, 16)}, at::kByte, like)) {}
+    static int64_t room(int64_t n, int64_t size) { return (n * size + 15) / 16 * 16; }
+    at::Tensor take(int64_t n, at::ScalarType dtype) {
+        const int64_t size = c10::elementSize(dtype);
+        auto t = c10::make_intrusive<c10::TensorImpl>(c10::Storage(base_.storage()), base_.key_set(),
+                                                      c10::scalarTypeToTypeMeta(dtype));
+        t->set_storage_offset(at_ / size);
+        t->set_sizes_contiguous({n});
+        at_ += room(n, size);
+        return at::Tensor(std::move(t));
+    }
+
+  private:
+    at::Tensor base_;
+    int64_t at_ = 0;
+};
 
 at::Tensor workspace(const at::Tensor &like, size_t bytes) {
     return at::empty({(int64_t)std::max<size_t>(bytes, 256)},
@@ -341,11 +368,11 @@ std::vector<at::Tensor> mla_decode_tree(const at::Tensor &query, const at::Tenso
     c10::cuda::CUDAGuard g(query.device());
     if (max_seq_len < 0) max_seq_len = b > 0 ? std::max<int64_t>(seq_lens.max().item<int64_t>(), 0) : 0;
     TORCH_CHECK(max_seq_len <= INT32_MAX, "mla_decode_tree: max_seq_len out of range");
-    at::Tensor out = at::empty({b, k, nh, MLA_B200_HEAD_DIM_V},
-                               query.options().dtype(out_fp32 ? at::kFloat : query.scalar_type()));
-    at::Tensor lse = at::empty({return_lse ? b : 0, k, nh}, query.options().dtype(at::kFloat));
-    at::Tensor w = workspace(query, mla_b200_workspace_size_tree((int)b, (int)k, (int)nh, (int)max_seq_len,
-                                                                 (int)num_splits));
+    at::Tensor out = fresh({b, k, nh, MLA_B200_HEAD_DIM_V}, out_fp32 ? at::kFloat : query.scalar_type(), query);
+    at::Tensor lse = fresh({return_lse ? b : 0, k, nh}, at::kFloat, query);
+    at::Tensor w = fresh({(int64_t)std::max<size_t>(mla_b200_workspace_size_tree((int)b, (int)k, (int)nh, (int)max_seq_len,
+                                                                                (int)num_splits), 256)},
+                         at::kByte, query);
     auto *fn = bf16 ? mla_b200_decode_tree_bf16 : mla_b200_decode_tree_f16;
     const int odt = out_fp32 ? MLA_B200_OUT_F32 : (bf16 ? MLA_B200_OUT_BF16 : MLA_B200_OUT_F16);
     check_status(fn(query.data_ptr(), kv_pages.data_ptr(), block_table.data_ptr<int32_t>(),
@@ -426,15 +453,15 @@ std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k
     auto shape = query.sizes().vec();
     shape.back() = MLA_B200_HEAD_DIM;
     // (rows outside every sequence of a packed batch are left as they are allocated)
-    at::Tensor out = at::empty(shape, query.options());
+    at::Tensor out = fresh(shape, query.scalar_type(), query);
     shape.pop_back();
     if (!return_lse) shape[0] = 0;
-    at::Tensor lse = at::empty(shape, query.options().dtype(at::kFloat));
+    at::Tensor lse = fresh(shape, at::kFloat, query);
     at::Tensor w;
     size_t ws = 0;
     if (packed && b > 1) {
         ws = mla_b200_workspace_size_prefill((int)b, tq);
-        w = workspace(query, ws);
+        w = fresh({(int64_t)ws}, at::kByte, query);
     }
     auto *fn = bf16 ? mla_b200_prefill_bf16 : mla_b200_prefill_f16;
     const int64_t d = lead - 1;
@@ -482,9 +509,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> mla_build
         head = free_head->data_ptr<int32_t>();
     }
     c10::cuda::CUDAGuard g(seq_lens.device());
-    const auto opt = seq_lens.options();
-    at::Tensor slots = at::empty({num_tokens}, opt.dtype(at::kLong)), positions = at::empty({num_tokens}, opt);
-    at::Tensor cu_new = at::empty({b + 1}, opt), lens = at::empty({b}, opt), new_head = at::empty({1}, opt);
+    Carve all(Carve::room(num_tokens, 8) + Carve::room(num_tokens, 4) + Carve::room(b + 1, 4) + Carve::room(b, 4) + 16,
+              seq_lens);
+    at::Tensor slots = all.take(num_tokens, at::kLong), positions = all.take(num_tokens, at::kInt);
+    at::Tensor cu_new = all.take(b + 1, at::kInt), lens = all.take(b, at::kInt), new_head = all.take(1, at::kInt);
     check_status(mla_b200_build_slots(seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
                                       block_table.data_ptr<int32_t>(),
                                       b > 1 ? block_table.stride(0) : block_table.size(1), (int)block_table.size(1),

@@ -47,13 +47,19 @@ struct Request {
     int len, add, have, need;
 };
 
+// ceil(n / page_size), at most `most`; the division in 32 bits where that holds n.
+__device__ __forceinline__ int pages_of(unsigned long long n, int page_size, int most) {
+    const unsigned long long up = n + (unsigned)(page_size - 1);
+    const unsigned long long q = up >> 32 ? up / (unsigned)page_size : (unsigned)up / (unsigned)page_size;
+    return (int)min(q, (unsigned long long)most);
+}
+
 __device__ __forceinline__ Request request_of(const SlotParams &p, int b) {
     Request r;
     r.len = max(p.seq_lens[b], 0);
     r.add = max(p.new_lens[b], 0);
-    const long long end = (long long)r.len + r.add;
-    r.have = (int)min((long long)p.max_blocks, ((long long)r.len + p.page_size - 1) / p.page_size);
-    r.need = (int)min((long long)p.max_blocks, (end + p.page_size - 1) / p.page_size) - r.have;
+    r.have = pages_of(r.len, p.page_size, p.max_blocks);
+    r.need = pages_of((unsigned long long)r.len + r.add, p.page_size, p.max_blocks) - r.have;
     return r;
 }
 
@@ -65,15 +71,18 @@ __global__ void __launch_bounds__(kThreads) build_slots_kernel(const SlotParams 
     __shared__ int mark[kThreads];           // 1 + index of the request record that starts at this token
     __shared__ long long rec_tok[kThreads];  // the request's first token ...
     __shared__ long long rec_page[kThreads]; // ... and its first new page's place in the free list
-    __shared__ int rec_b[kThreads];
+    __shared__ int rec_b[kThreads], rec_len[kThreads], rec_have[kThreads];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
     // the sums before this thread's requests
     const int per = (p.batch + kThreads - 1) / kThreads;
     const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+    const long long head = p.free_head != nullptr ? p.free_head[0] : 0;
     Sums own = {0, 0};
+    Request first = {0, 0, 0, 0};  // (kept: with up to 1024 requests it is the only one)
     for (int b = b0; b < b1; ++b) {
         const Request r = request_of(p, b);
+        if (b == b0) first = r;
         own = own + Sums{r.add, r.need};
     }
     Sums v = own;
@@ -97,13 +106,12 @@ __global__ void __launch_bounds__(kThreads) build_slots_kernel(const SlotParams 
     const long long total = warp_sum[31].tokens;
     Sums before = {v.tokens - own.tokens, v.pages - own.pages};
     if (warp > 0) before = before + warp_sum[warp - 1];
-    const long long head = p.free_head != nullptr ? p.free_head[0] : 0;
 
     // what is written once per request, dealt over the blocks
     if (tid % gridDim.x == blockIdx.x) {
         Sums s = before;
         for (int b = b0; b < b1; ++b) {
-            const Request r = request_of(p, b);
+            const Request r = b == b0 ? first : request_of(p, b);
             p.cu_new[b] = clamp_i32(s.tokens);
             p.new_seq_lens[b] = clamp_i32((long long)r.len + r.add);
             s = s + Sums{r.add, r.need};
@@ -122,13 +130,15 @@ __global__ void __launch_bounds__(kThreads) build_slots_kernel(const SlotParams 
         {
             Sums s = before;
             for (int b = b0; b < b1 && s.tokens < t0 + kThreads; ++b) {
-                const Request r = request_of(p, b);
+                const Request r = b == b0 ? first : request_of(p, b);
                 if (r.add > 0 && s.tokens + r.add > t0) {
                     const int at = (int)max(s.tokens - t0, 0ll);  // its own: requests do not overlap
                     mark[at] = at + 1;
                     rec_tok[at] = s.tokens;
                     rec_page[at] = head + s.pages;
                     rec_b[at] = b;
+                    rec_len[at] = r.len;
+                    rec_have[at] = r.have;
                 }
                 s = s + Sums{r.add, r.need};
             }
@@ -155,18 +165,17 @@ __global__ void __launch_bounds__(kThreads) build_slots_kernel(const SlotParams 
         if (warp > 0) m = max(m, warp_mark[warp - 1]);
         const long long t = t0 + tid;
         if (t < total) {
-            const int b = rec_b[m - 1];
-            const Request r = request_of(p, b);
-            const long long pos = r.len + (t - rec_tok[m - 1]);
-            const long long block = pos / p.page_size;
+            const int b = rec_b[m - 1], have = rec_have[m - 1];
+            const long long pos = rec_len[m - 1] + (t - rec_tok[m - 1]);
+            const long long block = pos >> 32 ? pos / p.page_size : (long long)((unsigned)pos / (unsigned)p.page_size);
             const int in_page = (int)(pos - block * p.page_size);
             int page = -1;
             if (block < p.max_blocks) {
                 int32_t *entry = p.table + (long long)b * p.table_stride + block;
-                if (block < r.have) {
+                if (block < have) {
                     page = *entry;  // not one that this call writes
                 } else {
-                    const long long i = rec_page[m - 1] + (block - r.have);
+                    const long long i = rec_page[m - 1] + (block - have);
                     if (i >= 0 && i < p.num_free) page = p.free_pages[i];
                     if (in_page == 0) *entry = page;
                 }

@@ -72,6 +72,19 @@ __device__ __forceinline__ void load8(const T *src, float (&v)[8]) {
     }
 }
 
+// Two consecutive elements at an even offset of a vector row.
+__device__ __forceinline__ void load2(const float *src, float &a, float &b) {
+    const float2 f = __ldg(reinterpret_cast<const float2 *>(src));
+    a = f.x;
+    b = f.y;
+}
+template <typename T>
+__device__ __forceinline__ void load2(const T *src, float &a, float &b) {
+    const float2 f = two_f32<T>(__ldg(reinterpret_cast<const uint32_t *>(src)));
+    a = f.x;
+    b = f.y;
+}
+
 __device__ __forceinline__ uint32_t pack2_to(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
@@ -90,20 +103,24 @@ __global__ void __launch_bounds__(32 * kWarps) cache_write_kernel(const WritePar
     const int lane = threadIdx.x & 31;
     const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (t >= p.num_tokens) return;
+    // every load that depends on no other goes out first: slot and position, the row
     const long long slot = __ldg(p.slots + t);
-    if (slot < 0 || slot >= p.cache_rows) return;  // a token without a page: nothing is written
-    int pos = 0;
-    if (p.positions != nullptr) {
-        pos = __ldg(p.positions + t);
-        if (pos < 0 || pos >= p.max_pos) return;  // no angle for it: nothing is written
-    }
+    const int pos = p.positions != nullptr ? __ldg(p.positions + t) : 0;
     const InT *row = static_cast<const InT *>(p.latent) + t * p.stride;
     float v[2][8];
     load8<InT, kVec>(row + 8 * lane, v[0]);
     load8<InT, kVec>(row + 256 + 8 * lane, v[1]);
     // this lane's rope pair
     const int ia = p.interleaved ? 2 * lane : lane, ib = p.interleaved ? 2 * lane + 1 : lane + 32;
-    float a = (float)row[kLat + ia], b = (float)row[kLat + ib];
+    float a, b;
+    if (kVec && p.interleaved) {
+        load2(row + kLat + ia, a, b);
+    } else {
+        a = (float)row[kLat + ia];
+        b = (float)row[kLat + ib];
+    }
+    if (slot < 0 || slot >= p.cache_rows) return;  // a token without a page: nothing is written
+    if (p.positions != nullptr && (pos < 0 || pos >= p.max_pos)) return;  // no angle for it: likewise
     if (p.positions != nullptr) {
         const float c = __ldg(p.cos_sin + (long long)pos * kRope + lane);
         const float s = __ldg(p.cos_sin + (long long)pos * kRope + 32 + lane);
