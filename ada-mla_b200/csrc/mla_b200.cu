@@ -1155,19 +1155,19 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
 
 namespace {
 template <typename InT, typename OutT>
-void launch_write(const write::WriteParams &p, bool vec, cudaStream_t stream) {
-    const unsigned grid = (unsigned)cdiv(p.num_tokens, write::kWarps);
+void launch_write(const write::WriteParams &p, bool vec, int sms, cudaStream_t stream) {
+    const unsigned grid = (unsigned)std::min<long long>(cdiv(p.num_tokens, write::kWarps), (long long)sms * write::kBlocksPerSm<OutT>);
     if (vec) write::cache_write_kernel<InT, OutT, true><<<grid, 32 * write::kWarps, 0, stream>>>(p);
     else write::cache_write_kernel<InT, OutT, false><<<grid, 32 * write::kWarps, 0, stream>>>(p);
 }
 
 template <typename InT>
-void launch_write_to(const write::WriteParams &p, int cache_dtype, cudaStream_t stream) {
+void launch_write_to(const write::WriteParams &p, int cache_dtype, int sms, cudaStream_t stream) {
     // 16-byte loads where every row and the weights start on 16 bytes
     const bool vec = aligned(p.latent, 16) && aligned(p.weight, 16) && p.stride * (long long)sizeof(InT) % 16 == 0;
-    if (cache_dtype == MLA_B200_DTYPE_F16) launch_write<InT, __half>(p, vec, stream);
-    else if (cache_dtype == MLA_B200_DTYPE_BF16) launch_write<InT, __nv_bfloat16>(p, vec, stream);
-    else launch_write<InT, __nv_fp8_storage_t>(p, vec, stream);
+    if (cache_dtype == MLA_B200_DTYPE_F16) launch_write<InT, __half>(p, vec, sms, stream);
+    else if (cache_dtype == MLA_B200_DTYPE_BF16) launch_write<InT, __nv_bfloat16>(p, vec, sms, stream);
+    else launch_write<InT, __nv_fp8_storage_t>(p, vec, sms, stream);
 }
 }  // namespace
 
@@ -1451,9 +1451,9 @@ int mla_b200_cache_write(const void *latent, int latent_dtype, long long latent_
     p.cache_rows = cache_rows;
     p.kv_scales = kv_scales;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (latent_dtype == MLA_B200_DTYPE_F16) launch_write_to<__half>(p, cache_dtype, s);
-    else if (latent_dtype == MLA_B200_DTYPE_BF16) launch_write_to<__nv_bfloat16>(p, cache_dtype, s);
-    else launch_write_to<float>(p, cache_dtype, s);
+    if (latent_dtype == MLA_B200_DTYPE_F16) launch_write_to<__half>(p, cache_dtype, info.sms, s);
+    else if (latent_dtype == MLA_B200_DTYPE_BF16) launch_write_to<__nv_bfloat16>(p, cache_dtype, info.sms, s);
+    else launch_write_to<float>(p, cache_dtype, info.sms, s);
     return launch_status();
 }
 

@@ -7,19 +7,26 @@
 //   cache[slot] = [y, rope], or e4m3([y, rope] / s) with s = max|row| / 448 kept in
 //   kv_scales[slot] (1 for a row of zeros).
 //
-// A warp per row: lane l holds latent columns 8l.. and 256 + 8l.. (or 4-column
-// pieces of fp32 input) and rope pair l, so a row is read once in 16-byte loads, its
-// sum of squares and its largest value are warp sums in registers, and the row is
-// written once.  All arithmetic is fp32.  Bound by memory: 576 * (in + out) bytes
-// a row.
+// A warp per row: lane l holds latent columns 8l.. and 256 + 8l.. and rope pair l, so
+// a row is read once in 16-byte loads, its sum of squares and its largest value are warp
+// reductions in registers, and the row is written once.  All arithmetic is fp32.  Bound
+// by memory: 576 * (in + out) bytes a row.  Each warp walks rows with the next one's
+// loads in flight (its position one further ahead, so that its angles are too) and
+// keeps its norm weights: a warp for one row alone left the memory 40 % idle.
 #pragma once
+
+#include <type_traits>
 
 #include "mla_common.cuh"
 
 namespace mla {
 namespace write {
 
-constexpr int kWarps = 8;  // rows per block
+constexpr int kWarps = 8;        // warps per block
+// Resident blocks per SM, which the rows are dealt to: 4 (64 registers) or, for e4m3, 3
+// (80).  32769 rows to bf16: 16.5 us with 4, 18.4 with 3, 21.7 with 5; 131072 rows to
+// e4m3: 52.5, 49.5, 66.7.
+template <typename OutT> constexpr int kBlocksPerSm = sizeof(OutT) == 1 ? 3 : 4;
 constexpr int kLat = kDV;
 constexpr int kRope = kDK - kDV;
 
@@ -47,43 +54,54 @@ template <> __device__ __forceinline__ float2 two_f32<__nv_bfloat16>(uint32_t u)
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u));
 }
 
-// Eight consecutive elements at `src`: 16-byte loads, or single ones where the row
-// does not start on 16 bytes.
+// This lane's part of a row as it was loaded: latent columns 8 lane .. and 256 + 8
+// lane .., and its rope pair.  16-byte loads, or single ones where rows do not start on
+// 16 bytes.
 template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T *src, float (&v)[8]) {
-    if constexpr (!kVec) {
+struct Raw {
+    static constexpr int kN = kVec ? (int)sizeof(T) : 16;  // 16-byte vectors (8 elements: sizeof(T) / 2), or elements
+    using V = std::conditional_t<kVec, uint4, T>;
+    V x[kN];
+    T a, b;
+
+    __device__ __forceinline__ void load(const T *row, int lane, int ia, int ib) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = (float)src[k];
-    } else if constexpr (sizeof(T) == 4) {
+        for (int h = 0; h < 2; ++h) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float4 u = __ldg(reinterpret_cast<const float4 *>(src) + k);
-            v[4 * k] = u.x; v[4 * k + 1] = u.y; v[4 * k + 2] = u.z; v[4 * k + 3] = u.w;
+            for (int k = 0; k < kN / 2; ++k)
+                x[h * (kN / 2) + k] = __ldg(reinterpret_cast<const V *>(row + 256 * h + 8 * lane) + k);
         }
-    } else {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        a = row[kLat + ia];
+        b = row[kLat + ib];
+    }
+
+    __device__ __forceinline__ void values(float (&v)[2][8]) const {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 f = two_f32<T>(w[k]);
-            v[2 * k] = f.x;
-            v[2 * k + 1] = f.y;
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (!kVec) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v[h][k] = (float)x[h * 8 + k];
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint4 u = x[h * 2 + k];
+                    v[h][4 * k] = __uint_as_float(u.x);
+                    v[h][4 * k + 1] = __uint_as_float(u.y);
+                    v[h][4 * k + 2] = __uint_as_float(u.z);
+                    v[h][4 * k + 3] = __uint_as_float(u.w);
+                }
+            } else {
+                const uint32_t w[4] = {x[h].x, x[h].y, x[h].z, x[h].w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 f = two_f32<T>(w[k]);
+                    v[h][2 * k] = f.x;
+                    v[h][2 * k + 1] = f.y;
+                }
+            }
         }
     }
-}
-
-// Two consecutive elements at an even offset of a vector row.
-__device__ __forceinline__ void load2(const float *src, float &a, float &b) {
-    const float2 f = __ldg(reinterpret_cast<const float2 *>(src));
-    a = f.x;
-    b = f.y;
-}
-template <typename T>
-__device__ __forceinline__ void load2(const T *src, float &a, float &b) {
-    const float2 f = two_f32<T>(__ldg(reinterpret_cast<const uint32_t *>(src)));
-    a = f.x;
-    b = f.y;
-}
+};
 
 __device__ __forceinline__ uint32_t pack2_to(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -98,96 +116,121 @@ __device__ __forceinline__ uint32_t pack2_e4m3(float a, float b) {
 }
 
 template <typename InT, typename OutT, bool kVec>
-__global__ void __launch_bounds__(32 * kWarps) cache_write_kernel(const WriteParams p) {
+__global__ void __launch_bounds__(32 * kWarps, kBlocksPerSm<OutT>) cache_write_kernel(const WriteParams p) {
     constexpr bool kFp8 = sizeof(OutT) == 1;
     const int lane = threadIdx.x & 31;
-    const long long t = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int warps = gridDim.x * kWarps;
+    int t = blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (t >= p.num_tokens) return;
-    // every load that depends on no other goes out first: slot and position, the row
-    const long long slot = __ldg(p.slots + t);
-    const int pos = p.positions != nullptr ? __ldg(p.positions + t) : 0;
-    const InT *row = static_cast<const InT *>(p.latent) + t * p.stride;
-    float v[2][8];
-    load8<InT, kVec>(row + 8 * lane, v[0]);
-    load8<InT, kVec>(row + 256 + 8 * lane, v[1]);
-    // this lane's rope pair
     const int ia = p.interleaved ? 2 * lane : lane, ib = p.interleaved ? 2 * lane + 1 : lane + 32;
-    float a, b;
-    if (kVec && p.interleaved) {
-        load2(row + kLat + ia, a, b);
-    } else {
-        a = (float)row[kLat + ia];
-        b = (float)row[kLat + ib];
-    }
-    if (slot < 0 || slot >= p.cache_rows) return;  // a token without a page: nothing is written
-    if (p.positions != nullptr && (pos < 0 || pos >= p.max_pos)) return;  // no angle for it: likewise
-    if (p.positions != nullptr) {
-        const float c = __ldg(p.cos_sin + (long long)pos * kRope + lane);
-        const float s = __ldg(p.cos_sin + (long long)pos * kRope + 32 + lane);
-        const float ra = a * c - b * s, rb = a * s + b * c;
-        a = ra;
-        b = rb;
-    }
-    if (p.weight != nullptr) {
-        float sq = 0.f;
+    const bool rope = p.positions != nullptr, norm = p.weight != nullptr;
+    const InT *base = static_cast<const InT *>(p.latent);
+    auto position = [&](int i) -> int { return rope && i < p.num_tokens ? __ldg(p.positions + i) : 0; };
+    auto angle = [&](int pos, float &c, float &s) {  // (no angle: the row is skipped below)
+        const bool ok = rope && pos >= 0 && pos < p.max_pos;
+        c = ok ? __ldg(p.cos_sin + (long long)pos * kRope + lane) : 0.f;
+        s = ok ? __ldg(p.cos_sin + (long long)pos * kRope + 32 + lane) : 0.f;
+    };
+    Raw<InT, kVec> raw, raw_next;
+    long long slot = __ldg(p.slots + t), slot_next = -1;
+    int pos = position(t), pos_next = position(t + warps);
+    raw.load(base + t * p.stride, lane, ia, ib);
+    float g[2][8];
+    if (norm) {
+        Raw<InT, kVec> w;
+        const InT *wp = static_cast<const InT *>(p.weight);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) sq = fmaf(v[h][k], v[h][k], sq);
-        sq = warp_sum(sq);
-        const float inv = rsqrtf(sq * (1.f / kLat) + p.eps);
-        const InT *w = static_cast<const InT *>(p.weight);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float g[8];
-            load8<InT, kVec>(w + 256 * h + 8 * lane, g);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[h][k] = v[h][k] * inv * g[k];
-        }
+            for (int k = 0; k < w.kN / 2; ++k)
+                w.x[h * (w.kN / 2) + k] = __ldg(reinterpret_cast<const typename Raw<InT, kVec>::V *>(wp + 256 * h + 8 * lane) + k);
+        w.values(g);
     }
-    if constexpr (kFp8) {
-        float mx = fmaxf(fabsf(a), fabsf(b));
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(v[h][k]));
-        mx = warp_max(mx);
-        // a positive normal scale, as the decode asks for, also for rows of zeros or
-        // of the smallest numbers
-        const float scale = mx > 0.f ? fmaxf(mx / 448.f, 1.17549435e-38f) : 1.f;
-        const float r = 1.f / scale;
-        uint8_t *dst = static_cast<uint8_t *>(p.cache) + slot * kDK;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            uint32_t o[2];
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-                o[k] = pack2_e4m3(v[h][4 * k] * r, v[h][4 * k + 1] * r) |
-                       (pack2_e4m3(v[h][4 * k + 2] * r, v[h][4 * k + 3] * r) << 16);
-            *reinterpret_cast<uint2 *>(dst + 256 * h + 8 * lane) = make_uint2(o[0], o[1]);
+    float cos_t, sin_t, cos_n = 0.f, sin_n = 0.f;
+    angle(pos, cos_t, sin_t);
+    for (; t < p.num_tokens; t += warps) {
+        const int tn = t + warps;
+        if (tn < p.num_tokens) {  // the next row's loads, and the position after it
+            slot_next = __ldg(p.slots + tn);
+            raw_next.load(base + tn * p.stride, lane, ia, ib);
+            angle(pos_next, cos_n, sin_n);
         }
-        const uint32_t ab = pack2_e4m3(a * r, b * r);
-        if (p.interleaved) {
-            *reinterpret_cast<unsigned short *>(dst + kLat + ia) = (unsigned short)ab;
-        } else {
-            dst[kLat + ia] = (uint8_t)ab;
-            dst[kLat + ib] = (uint8_t)(ab >> 8);
-        }
-        if (lane == 0) p.kv_scales[slot] = scale;
-    } else {
-        OutT *dst = static_cast<OutT *>(p.cache) + slot * kDK;
+        const int pos_after = position(tn + warps);
+        // a token without a page, or a position without an angle: nothing is written
+        if (slot >= 0 && slot < p.cache_rows && (!rope || (pos >= 0 && pos < p.max_pos))) {
+            float v[2][8];
+            raw.values(v);
+            float a = (float)raw.a, b = (float)raw.b;
+            if (rope) {
+                const float ra = a * cos_t - b * sin_t, rb = a * sin_t + b * cos_t;
+                a = ra;
+                b = rb;
+            }
+            if (norm) {
+                float sq = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-            *reinterpret_cast<uint4 *>(dst + 256 * h + 8 * lane) =
-                make_uint4(pack2_to(v[h][0], v[h][1], OutT()), pack2_to(v[h][2], v[h][3], OutT()),
-                           pack2_to(v[h][4], v[h][5], OutT()), pack2_to(v[h][6], v[h][7], OutT()));
-        const uint32_t ab = pack2_to(a, b, OutT());
-        if (p.interleaved) {
-            *reinterpret_cast<uint32_t *>(dst + kLat + ia) = ab;
-        } else {
-            reinterpret_cast<unsigned short *>(dst)[kLat + ia] = (unsigned short)ab;
-            reinterpret_cast<unsigned short *>(dst)[kLat + ib] = (unsigned short)(ab >> 16);
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sq = fmaf(v[h][k], v[h][k], sq);
+                sq = warp_sum(sq);
+                const float inv = rsqrtf(sq * (1.f / kLat) + p.eps);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[h][k] = v[h][k] * inv * g[h][k];
+            }
+            if constexpr (kFp8) {
+                float mx = fmaxf(fabsf(a), fabsf(b));
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(v[h][k]));
+                // (the largest of non-negative floats: their bits order like whole numbers)
+                mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                // a positive normal scale, as the decode asks for, also for rows of zeros or
+                // of the smallest numbers
+                const float scale = mx > 0.f ? fmaxf(mx / 448.f, 1.17549435e-38f) : 1.f;
+                const float r = 1.f / scale;
+                uint8_t *dst = static_cast<uint8_t *>(p.cache) + slot * kDK;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t o[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+                        o[k] = pack2_e4m3(v[h][4 * k] * r, v[h][4 * k + 1] * r) |
+                               (pack2_e4m3(v[h][4 * k + 2] * r, v[h][4 * k + 3] * r) << 16);
+                    *reinterpret_cast<uint2 *>(dst + 256 * h + 8 * lane) = make_uint2(o[0], o[1]);
+                }
+                const uint32_t ab = pack2_e4m3(a * r, b * r);
+                if (p.interleaved) {
+                    *reinterpret_cast<unsigned short *>(dst + kLat + ia) = (unsigned short)ab;
+                } else {
+                    dst[kLat + ia] = (uint8_t)ab;
+                    dst[kLat + ib] = (uint8_t)(ab >> 8);
+                }
+                if (lane == 0) p.kv_scales[slot] = scale;
+            } else {
+                OutT *dst = static_cast<OutT *>(p.cache) + slot * kDK;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<uint4 *>(dst + 256 * h + 8 * lane) =
+                        make_uint4(pack2_to(v[h][0], v[h][1], OutT()), pack2_to(v[h][2], v[h][3], OutT()),
+                                   pack2_to(v[h][4], v[h][5], OutT()), pack2_to(v[h][6], v[h][7], OutT()));
+                const uint32_t ab = pack2_to(a, b, OutT());
+                if (p.interleaved) {
+                    *reinterpret_cast<uint32_t *>(dst + kLat + ia) = ab;
+                } else {
+                    reinterpret_cast<unsigned short *>(dst)[kLat + ia] = (unsigned short)ab;
+                    reinterpret_cast<unsigned short *>(dst)[kLat + ib] = (unsigned short)(ab >> 16);
+                }
+            }
         }
+        raw = raw_next;
+        slot = slot_next;
+        pos = pos_next;
+        pos_next = pos_after;
+        cos_t = cos_n;
+        sin_t = sin_n;
     }
 }
 
