@@ -74,6 +74,7 @@ constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kPlanBuckets = 1024;
+constexpr uint64_t kAbortWaitNs = 10000000ull;  // after an error: for copies in flight
 constexpr uint32_t kMaxIdle = 100000000;  // tries of 200 ns and more: 20 s and more
 
 struct PrefillParams {
@@ -303,150 +304,172 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp == 0) {
             // ------------------------------------------------------ TMA producer
-            if (lane == 0) {
-                uint32_t at = 0;           // slots filled so far
-                uint32_t qn[2] = {0, 0};   // Q tiles loaded so far
-                uint32_t tails = 0;        // V tiles handed to the V tail warp so far
-                bool ok = true;
-                auto acquire = [&](uint32_t &full, bool tail = false) -> uint32_t {  // next slot's address, its full barrier
-                    const uint32_t s = at % kSlots;
-                    if (!ok || *abort_flag || !ptx::mbar_wait_now(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty)) {
-                        ok = false;
-                        return 0;
-                    }
-                    ++at;
-                    full = bar(tail ? kBarTail + (tails & 1) : kBarFull + s);
-                    if (!tail) ptx::mbar_arrive_expect_tx(full, kBox);
-                    return sbase + kOffRing + s * kBox;
-                };
-                auto load_q = [&](int t) {
-                    if (!ok || *abort_flag || !ptx::mbar_wait_now(bar(kBarQEmpty + t), (qn[t] & 1) ^ 1, kErrWaitEmpty)) {
-                        ok = false;
-                        return;
-                    }
-                    ++qn[t];
-                    ptx::mbar_arrive_expect_tx(bar(kBarQFull + t), kQBytes);
-                    const int row = it.s.q0 + it.row + t * kTileQ;
-                    for (int c = 0; c < kKBlk; ++c)
-                        ptx::tma_load_3d(sbase + t * kQBytes + c * kBox, &qmap, c * 64, it.h, row, bar(kBarQFull + t));
-                };
-                auto load_k = [&](int j) {
-                    const int row = it.s.k0 + j * kTileK;
-                    uint32_t full = 0;
-                    for (int c = 0; c < kKBlk; ++c) {
-                        const uint32_t dst = acquire(full);
-                        if (!ok) return;
-                        if (c < 2) ptx::tma_load_3d(dst, &kmap, c * 64, it.h, row, full);
-                        else ptx::tma_load_2d(dst, &rmap, 0, row, full);
-                    }
-                };
-                auto load_v = [&](int j) {
-                    const int row = it.s.k0 + j * kTileK;
-                    const bool tail = (j + 1) * kTileK > it.s.lk;
-                    uint32_t full = 0;
-                    for (int c = 0; c < 2; ++c) {
-                        const uint32_t dst = acquire(full, tail);
-                        if (!ok) return;
-                        if (tail && c == 0) ptx::mbar_arrive_expect_tx(full, 2 * kBox);
-                        ptx::tma_load_3d(dst, &vmap, 0, it.h, row + c * kVHalf, full);
-                        ptx::tma_load_3d(dst + kVBox, &vmap, 64, it.h, row + c * kVHalf, full);
-                    }
-                    if (tail) ++tails;
-                };
-                while (ok && cur.next(p, it)) {
-                    if (it.nmax <= 0) continue;
-                    if (it.n[0] > 0) load_q(0);
-                    load_k(0);
-                    if (it.n[1] > 0) load_q(1);
-                    for (int j = 0; ok && j < it.nmax; ++j) {
-                        load_v(j);
-                        if (j + 1 < it.nmax) load_k(j + 1);
-                    }
-                }
-                if (!ok) *abort_flag = 1;
-                // every load has landed before this CTA's shared memory goes
-                for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
-                    ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
-                for (uint32_t k = tails > 2 ? tails - 2 : 0; k < tails; ++k)
-                    ptx::mbar_wait(bar(kBarTail + (k & 1)), (k >> 1) & 1, kErrWaitFull);
-                for (int t = 0; t < 2; ++t)
-                    if (qn[t] > 0) ptx::mbar_wait(bar(kBarQFull + t), (qn[t] - 1) & 1, kErrWaitFull);
-            }
-        } else if (warp == 1) {
-            // ------------------------------------------------------ MMA issuer
-            if (lane == 0) {
-                const uint32_t idesc_qk = ptx::idesc_f16_f32(kTileQ, kTileK, 0, 0, kBf16);
-                const uint32_t idesc_pv = ptx::idesc_f16_f32(kTileQ, kV, 0, 1, kBf16);
-                uint32_t at = 0;  // ring slots of the items before this one
-                uint32_t qn[2] = {0, 0}, pn[2] = {0, 0};
-                bool ok = true;
-                auto full = [&](uint32_t k) {
-                    if (ok && !ptx::mbar_spin(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull)) ok = false;
-                };
-                // S_t = Q_t . K(j)^T; the last reader frees the slots
-                auto qk = [&](int t, int j, bool free_slots, bool last) {
-                    const uint32_t k0 = at + j * kSlotsPerTile;
-                    for (int c = 0; c < kKBlk; ++c) {
-                        full(k0 + c);
-                        if (!ok) return;
-                        const uint32_t slot = (k0 + c) % kSlots;
-                        const uint64_t a = ptx::sdesc_sw128(sbase + t * kQBytes + c * kBox, 16, 1024);
-                        const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, 16, 1024);
+            // (This role and the next run as whole warps with uniform control flow and one
+            // elected lane behind each instruction, so that descriptors and coordinates
+            // stay in uniform registers.)
+            const uint32_t e = ptx::elect_one();
+            uint32_t at = 0;           // slots filled so far
+            uint32_t qn[2] = {0, 0};   // Q tiles loaded so far
+            uint32_t tails = 0;        // V tiles handed to the V tail warp so far
+            bool ok = true;
+            auto acquire = [&]() -> uint32_t {  // the next slot, once it is free
+                const uint32_t s = at % kSlots;
+                ok = ok && !*abort_flag && ptx::mbar_wait_now(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty);
+                ok = __all_sync(0xffffffffu, ok);
+                ++at;
+                return s;
+            };
+            while (ok && cur.next(p, it)) {
+                if (it.nmax <= 0) continue;
+                const int nmax = __shfl_sync(0xffffffffu, it.nmax, 0), h = __shfl_sync(0xffffffffu, it.h, 0);
+                const int k0 = __shfl_sync(0xffffffffu, it.s.k0, 0), q0 = __shfl_sync(0xffffffffu, it.s.q0 + it.row, 0);
+                const int lk = __shfl_sync(0xffffffffu, it.s.lk, 0);
+                const bool has[2] = {it.n[0] > 0, it.n[1] > 0};
+                // Q0 K(0) Q1 | V(0) K(1) | V(1) K(2) | ..
+#pragma unroll 1
+                for (int j = -1; ok && j < nmax; ++j) {
+                    if (j >= 0) {
+                        const int row = k0 + j * kTileK;
+                        const bool tail = (j + 1) * kTileK > lk;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            ptx::mma_ss(tmem + t * kTileK, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
-                                        (c > 0 || k > 0) ? 1u : 0u);
-                        if (free_slots) ptx::mma_commit(bar(kBarEmpty + slot));
-                    }
-                    ptx::mma_commit(bar(kBarS + t));
-                    if (last) ptx::mma_commit(bar(kBarQEmpty + t));
-                };
-                // O_t += P_t . V(j)
-                auto pv = [&](int t, int j, bool free_slots) {
-                    if (!ptx::mbar_spin(bar(kBarP + t), pn[t] & 1, kErrWaitMma)) { ok = false; return; }
-                    ++pn[t];
-                    const uint32_t k0 = at + j * kSlotsPerTile + kKBlk;
-                    ptx::tc_fence_after();  // P (and a corrected O) were stored by other threads
-                    for (int c = 0; c < 2; ++c) {
-                        full(k0 + c);
-                        if (!ok) return;
-                        const uint32_t slot = (k0 + c) % kSlots;
-                        const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, kVBox, 1024);
-#pragma unroll
-                        for (int k = 0; k < kVHalf / 16; ++k)
-                            ptx::mma_ts(tmem + kTmemO + t * kV, tmem + t * kTileK + (c * 4 + k) * 8,
-                                        b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || c > 0 || k > 0) ? 1u : 0u);
-                        if (free_slots) ptx::mma_commit(bar(kBarEmpty + slot));
-                    }
-                    ptx::mma_commit(bar(kBarO + t));
-                };
-                while (ok && cur.next(p, it)) {
-                    if (it.nmax <= 0) continue;
-                    for (int t = 0; t < 2; ++t) {
-                        if (it.n[t] <= 0) continue;
-                        if (*abort_flag || !ptx::mbar_spin(bar(kBarQFull + t), qn[t] & 1, kErrWaitFull)) { ok = false; break; }
-                        ++qn[t];
-                        qk(t, 0, t == 1 || it.n[1] <= 0, it.n[t] == 1);
+                        for (int c = 0; c < 2; ++c) {
+                            const uint32_t s = acquire();
+                            if (!ok) break;
+                            const uint32_t full = bar(tail ? kBarTail + (tails & 1) : kBarFull + s);
+                            const uint32_t dst = sbase + kOffRing + s * kBox;
+                            if (!tail || c == 0) ptx::mbar_arrive_expect_tx_if(e, full, tail ? 2 * kBox : kBox);
+                            ptx::tma_load_3d_if(e, dst, &vmap, 0, h, row + c * kVHalf, full);
+                            ptx::tma_load_3d_if(e, dst + kVBox, &vmap, 64, h, row + c * kVHalf, full);
+                        }
+                        if (tail) ++tails;
                         if (!ok) break;
                     }
-                    for (int j = 0; ok && j < it.nmax; ++j) {
-                        if (*abort_flag) { ok = false; break; }
 #pragma unroll
-                        for (int t = 0; t < 2; ++t) {
-                            if (j < it.n[t]) {
-                                // tile 1 reads last, where it reads at all
-                                pv(t, j, t == 1 || j >= it.n[1]);
-                                if (ok && j + 1 < it.n[t]) qk(t, j + 1, t == 1 || j + 1 >= it.n[1], j + 2 == it.n[t]);
+                    for (int t = 0; t < 2; ++t) {
+                        if (j < 0 && has[t]) {
+                            ok = ok && !*abort_flag && ptx::mbar_wait_now(bar(kBarQEmpty + t), (qn[t] & 1) ^ 1, kErrWaitEmpty);
+                            ok = __all_sync(0xffffffffu, ok);
+                            if (!ok) break;
+                            ++qn[t];
+                            ptx::mbar_arrive_expect_tx_if(e, bar(kBarQFull + t), kQBytes);
+#pragma unroll
+                            for (int c = 0; c < kKBlk; ++c)
+                                ptx::tma_load_3d_if(e, sbase + t * kQBytes + c * kBox, &qmap, c * 64, h, q0 + t * kTileQ,
+                                                    bar(kBarQFull + t));
+                        }
+                        if (t == 0 && j + 1 < nmax) {
+                            const int row = k0 + (j + 1) * kTileK;
+#pragma unroll
+                            for (int c = 0; c < kKBlk; ++c) {
+                                const uint32_t s = acquire();
+                                if (!ok) break;
+                                const uint32_t full = bar(kBarFull + s), dst = sbase + kOffRing + s * kBox;
+                                ptx::mbar_arrive_expect_tx_if(e, full, kBox);
+                                if (c < 2) ptx::tma_load_3d_if(e, dst, &kmap, c * 64, h, row, full);
+                                else ptx::tma_load_2d_if(e, dst, &rmap, 0, row, full);
                             }
+                            if (!ok) break;
                         }
                     }
-                    at += it.nmax * kSlotsPerTile;
                 }
-                if (!ok) *abort_flag = 1;
-                // every MMA has retired before TMEM and shared memory go
-                ptx::mma_commit(bar(kBarDrain));
-                ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
             }
+            if (!ok) *abort_flag = 1;
+            // every load has landed before this CTA's shared memory goes (the slots' own
+            // barriers, and those of tails not yet zeroed)
+            if (ok) {
+                for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
+                    ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
+            } else {
+                --at;  // (acquired in vain)
+                for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
+                    ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull, kAbortWaitNs);
+            }
+            for (uint32_t k = tails > 2 ? tails - 2 : 0; k < tails; ++k)
+                ptx::mbar_wait(bar(kBarTail + (k & 1)), (k >> 1) & 1, kErrWaitFull, ok ? kWaitLimitNs : kAbortWaitNs);
+            for (int t = 0; t < 2; ++t)
+                if (qn[t] > 0) ptx::mbar_wait(bar(kBarQFull + t), (qn[t] - 1) & 1, kErrWaitFull);
+        } else if (warp == 1) {
+            // ------------------------------------------------------ MMA issuer
+            // (A wait that runs out does not branch off: the tile is finished on whatever
+            // the buffers hold and then given up.)
+            const uint32_t e = ptx::elect_one();
+            constexpr uint32_t idesc_qk = ptx::idesc_f16_f32(kTileQ, kTileK, 0, 0, kBf16);
+            constexpr uint32_t idesc_pv = ptx::idesc_f16_f32(kTileQ, kV, 0, 1, kBf16);
+            uint32_t at = 0;  // ring slots of the items before this one
+            uint32_t qn[2] = {0, 0}, pn[2] = {0, 0};
+            bool ok = true;
+            auto full = [&](uint32_t k) {
+                ok &= ptx::mbar_spin(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
+            };
+            // S_t = Q_t . K(j)^T; the last reader frees the slots
+            auto qk = [&](int t, int j, bool free_slots, bool last) {
+                const uint32_t k0 = at + j * kSlotsPerTile;
+#pragma unroll
+                for (int c = 0; c < kKBlk; ++c) {
+                    full(k0 + c);
+                    const uint32_t slot = (k0 + c) % kSlots;
+                    const uint64_t a = ptx::sdesc_sw128(sbase + t * kQBytes + c * kBox, 16, 1024);
+                    const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, 16, 1024);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        ptx::mma_ss_if(e, tmem + t * kTileK, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
+                                       (c > 0 || k > 0) ? 1u : 0u);
+                    if (free_slots) ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                }
+                ptx::mma_commit_if(e, bar(kBarS + t));
+                if (last) ptx::mma_commit_if(e, bar(kBarQEmpty + t));
+            };
+            // O_t += P_t . V(j)
+            auto pv = [&](int t, int j, bool free_slots) {
+                ok &= ptx::mbar_spin(bar(kBarP + t), pn[t] & 1, kErrWaitMma);
+                ++pn[t];
+                const uint32_t k0 = at + j * kSlotsPerTile + kKBlk;
+                ptx::tc_fence_after();  // P (and a corrected O) were stored by other threads
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    full(k0 + c);
+                    const uint32_t slot = (k0 + c) % kSlots;
+                    const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, kVBox, 1024);
+#pragma unroll
+                    for (int k = 0; k < kVHalf / 16; ++k)
+                        ptx::mma_ts_if(e, tmem + kTmemO + t * kV, tmem + t * kTileK + (c * 4 + k) * 8,
+                                       b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || c > 0 || k > 0) ? 1u : 0u);
+                    if (free_slots) ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                }
+                ptx::mma_commit_if(e, bar(kBarO + t));
+            };
+            while (ok && cur.next(p, it)) {
+                if (it.nmax <= 0) continue;
+                const int n0 = __shfl_sync(0xffffffffu, it.n[0], 0), n1 = __shfl_sync(0xffffffffu, it.n[1], 0);
+                const int nmax = max(n0, n1);
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int n = t == 0 ? n0 : n1;
+                    if (n <= 0) continue;
+                    ok &= ptx::mbar_spin(bar(kBarQFull + t), qn[t] & 1, kErrWaitFull);
+                    ++qn[t];
+                    qk(t, 0, t == 1 || n1 <= 0, n == 1);
+                }
+#pragma unroll 1
+                for (int j = 0; j < nmax; ++j) {
+                    ok = ok && !*abort_flag;
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int n = t == 0 ? n0 : n1;
+                        if (j < n) {
+                            // tile 1 reads last, where it reads at all
+                            pv(t, j, t == 1 || j >= n1);
+                            if (j + 1 < n) qk(t, j + 1, t == 1 || j + 1 >= n1, j + 2 == n);
+                        }
+                    }
+                }
+                at += nmax * kSlotsPerTile;
+            }
+            if (!__all_sync(0xffffffffu, ok)) *abort_flag = 1;
+            // every MMA has retired before TMEM and shared memory go
+            ptx::mma_commit_if(e, bar(kBarDrain));
+            ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
         } else if (warp == 2) {
             // ------------------------------------------------------ V tail
             // The rows of a sequence's last V tile past its end hold the next
