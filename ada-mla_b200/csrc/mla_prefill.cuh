@@ -11,9 +11,9 @@
 // persistent CTA per SM.  Both tiles read each key / value tile of 128 tokens once.
 // While the tensor core works on one tile, the other tile's softmax runs:
 //
-//   MMA thread:  PV0(j)  QK0(j+1)  PV1(j)  QK1(j+1)  PV0(j+1) ...
-//   softmax 0:           [ tile 0, j+1 ......... ]
-//   softmax 1:                              [ tile 1, j+1 ......... ]
+//   tensor core:  PV0(j)  QK0(j+1)  PV1(j)  QK1(j+1)  PV0(j+1) ...
+//   softmax 0:            [ tile 0, j+1 ......... ]
+//   softmax 1:                               [ tile 1, j+1 ......... ]
 //
 // TMEM (512 columns): S0 S1 [128 x 128] fp32, O0 O1 [128 x 128] fp32; P (16-bit)
 // overwrites the first half of its S and is PV's A operand.  A tile of the pair costs
@@ -24,8 +24,8 @@
 // 64-column block of 128 keys or 64 tokens of V: K(0) V(0) K(1) V(1) .. in 3 + 2
 // slots each.  Slots of one size let the two kinds share 128 KB (1.6 tiles).
 //
-// Roles (384 threads): warp 0 TMA producer, warp 1 MMA issuer, warp 2 TMEM owner and
-// V tail, warps 4-7 softmax of tile 0, warps 8-11 of tile 1 (a thread per row: no
+// Roles (384 threads): warp 0 TMA producer, warps 1 and 3 MMA issuers (one per query
+// tile), warp 2 TMEM owner and V tail, warps 4-7 softmax of tile 0, warps 8-11 of tile 1 (a thread per row: no
 // shuffles).  The softmax warps rescale O themselves, rarely: the running maximum is
 // only raised when it grew by more than 2^8.  Every wait is bounded.
 #pragma once
@@ -58,19 +58,19 @@ enum : int {
     kBarQFull = 2 * kSlots,      // [2] Q tile landed
     kBarQEmpty = kBarQFull + 2,  // [2] last QK of the item done
     kBarS = kBarQEmpty + 2,      // [2] S tile complete
-    kBarP = kBarS + 2,           // [2] P tile written, O corrected (128 threads)
-    kBarO = kBarP + 2,           // [2] PV done
+    kBarP = kBarS + 2,           // [2][2] half a P tile written, O corrected (128 threads)
+    kBarO = kBarP + 4,           // [2] PV done
     kBarTail = kBarO + 2,        // [2] a sequence's last V tile landed, rows past its end not yet zeroed
-    kBarDrain = kBarTail + 2,
-    kNumBars = kBarDrain + 1
+    kBarDrain = kBarTail + 2,    // [2]
+    kNumBars = kBarDrain + 2
 };
 constexpr int kOffSlot = kOffBar + kNumBars * 8;
 constexpr int kOffAbort = kOffSlot + 4;
 constexpr int kSmemBytes = kOffAbort + 4 + 1024;  // + 1024 alignment slack
 static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
-// 384 threads x 168 registers at launch = 64512; the softmax warpgroups take 200
-// each and the first one keeps 104: 2 x 128 x 200 + 128 x 104 = 64512.
-constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
+// 384 threads x 168 registers at launch = 64512; the softmax warpgroups take 208
+// each and the first one keeps 88: 2 x 128 x 208 + 128 x 88 = 64512.
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 208, kRegsOther = 88;
 static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "register split");
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kPlanBuckets = 1024;
@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
-        for (int i = 0; i < kNumBars; ++i) ptx::mbar_init(bar(i), i == kBarP || i == kBarP + 1 ? 128 : 1);
+        for (int i = 0; i < kNumBars; ++i)  // (a ring slot is free when both MMA issuers are done with it)
+            ptx::mbar_init(bar(i), i >= kBarP && i < kBarP + 4 ? 128 : i >= kBarEmpty && i < kBarEmpty + kSlots ? 2 : 1);
         *abort_flag = 0;
         ptx::fence_mbarrier_init_cluster();
     }
@@ -388,88 +389,91 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ptx::mbar_wait(bar(kBarTail + (k & 1)), (k >> 1) & 1, kErrWaitFull, ok ? kWaitLimitNs : kAbortWaitNs);
             for (int t = 0; t < 2; ++t)
                 if (qn[t] > 0) ptx::mbar_wait(bar(kBarQFull + t), (qn[t] - 1) & 1, kErrWaitFull);
-        } else if (warp == 1) {
-            // ------------------------------------------------------ MMA issuer
+        } else if (warp == 1 || warp == 3) {
+            // ------------------------------------------------------ MMA issuers
+            // Warp 1 issues for query tile 0, warp 3 for tile 1: one thread's waits, fences
+            // and issue slots took 2250 cycles a tile, the products themselves need 1280.
             // (A wait that runs out does not branch off: the tile is finished on whatever
             // the buffers hold and then given up.)
+            const int t = warp == 1 ? 0 : 1;
             const uint32_t e = ptx::elect_one();
             constexpr uint32_t idesc_qk = ptx::idesc_f16_f32(kTileQ, kTileK, 0, 0, kBf16);
             constexpr uint32_t idesc_pv = ptx::idesc_f16_f32(kTileQ, kV, 0, 1, kBf16);
+            const uint32_t s_col = tmem + t * kTileK, o_col = tmem + kTmemO + t * kV;
             uint32_t at = 0;  // ring slots of the items before this one
-            uint32_t qn[2] = {0, 0}, pn[2] = {0, 0};
+            uint32_t qn = 0, pn = 0;
             bool ok = true;
             auto full = [&](uint32_t k) {
                 ok &= ptx::mbar_spin(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
             };
-            // S_t = Q_t . K(j)^T; the last reader frees the slots
-            auto qk = [&](int t, int j, bool free_slots, bool last) {
+            // S = Q . K(j)^T (the slots have landed)
+            auto qk = [&](int j, bool last) {
                 const uint32_t k0 = at + j * kSlotsPerTile;
 #pragma unroll
                 for (int c = 0; c < kKBlk; ++c) {
-                    full(k0 + c);
                     const uint32_t slot = (k0 + c) % kSlots;
                     const uint64_t a = ptx::sdesc_sw128(sbase + t * kQBytes + c * kBox, 16, 1024);
                     const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, 16, 1024);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        ptx::mma_ss_if(e, tmem + t * kTileK, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
+                        ptx::mma_ss_if(e, s_col, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
                                        (c > 0 || k > 0) ? 1u : 0u);
-                    if (free_slots) ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                    ptx::mma_commit_if(e, bar(kBarEmpty + slot));
                 }
                 ptx::mma_commit_if(e, bar(kBarS + t));
                 if (last) ptx::mma_commit_if(e, bar(kBarQEmpty + t));
             };
-            // O_t += P_t . V(j)
-            auto pv = [&](int t, int j, bool free_slots) {
-                ok &= ptx::mbar_spin(bar(kBarP + t), pn[t] & 1, kErrWaitMma);
-                ++pn[t];
-                const uint32_t k0 = at + j * kSlotsPerTile + kKBlk;
+            // half c of O += P . V(j)
+            auto pv = [&](int j, int c) {
+                const uint32_t slot = (at + j * kSlotsPerTile + kKBlk + c) % kSlots;
+                ok &= ptx::mbar_spin(bar(kBarP + 2 * t + c), pn & 1, kErrWaitMma);
                 ptx::tc_fence_after();  // P (and a corrected O) were stored by other threads
+                const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, kVBox, 1024);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int k = 0; k < kVHalf / 16; ++k)
+                    ptx::mma_ts_if(e, o_col, s_col + (c * 4 + k) * 8, b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv,
+                                   (j > 0 || c > 0 || k > 0) ? 1u : 0u);
+                ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+            };
+            // the slots of a key tile that this query tile does not see
+            auto skip = [&](uint32_t k0, int n) {
+                for (int c = 0; c < n; ++c) {
                     full(k0 + c);
-                    const uint32_t slot = (k0 + c) % kSlots;
-                    const uint64_t b = ptx::sdesc_sw128(sbase + kOffRing + slot * kBox, kVBox, 1024);
-#pragma unroll
-                    for (int k = 0; k < kVHalf / 16; ++k)
-                        ptx::mma_ts_if(e, tmem + kTmemO + t * kV, tmem + t * kTileK + (c * 4 + k) * 8,
-                                       b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || c > 0 || k > 0) ? 1u : 0u);
-                    if (free_slots) ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                    if (e) ptx::mbar_arrive(bar(kBarEmpty + (k0 + c) % kSlots));
                 }
-                ptx::mma_commit_if(e, bar(kBarO + t));
             };
             while (ok && cur.next(p, it)) {
                 if (it.nmax <= 0) continue;
-                const int n0 = __shfl_sync(0xffffffffu, it.n[0], 0), n1 = __shfl_sync(0xffffffffu, it.n[1], 0);
-                const int nmax = max(n0, n1);
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int n = t == 0 ? n0 : n1;
-                    if (n <= 0) continue;
-                    ok &= ptx::mbar_spin(bar(kBarQFull + t), qn[t] & 1, kErrWaitFull);
-                    ++qn[t];
-                    qk(t, 0, t == 1 || n1 <= 0, n == 1);
+                const int n = __shfl_sync(0xffffffffu, it.n[t], 0), nmax = __shfl_sync(0xffffffffu, it.nmax, 0);
+                if (n > 0) {
+                    ok &= ptx::mbar_spin(bar(kBarQFull + t), qn & 1, kErrWaitFull);
+                    ++qn;
+                    for (int c = 0; c < kKBlk; ++c) full(at + c);
+                    qk(0, n == 1);
                 }
 #pragma unroll 1
-                for (int j = 0; j < nmax; ++j) {
+                for (int j = 0; j < n; ++j) {
                     ok = ok && !*abort_flag;
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int n = t == 0 ? n0 : n1;
-                        if (j < n) {
-                            // tile 1 reads last, where it reads at all
-                            pv(t, j, t == 1 || j >= n1);
-                            if (j + 1 < n) qk(t, j + 1, t == 1 || j + 1 >= n1, j + 2 == n);
-                        }
-                    }
+                    // (the waits for what the ring brings go before those for P)
+                    const uint32_t k0 = at + j * kSlotsPerTile;
+                    full(k0 + kKBlk);
+                    full(k0 + kKBlk + 1);
+                    pv(j, 0);
+                    if (j + 1 < n)
+                        for (int c = 0; c < kKBlk; ++c) full(k0 + kSlotsPerTile + c);
+                    pv(j, 1);
+                    ++pn;
+                    ptx::mma_commit_if(e, bar(kBarO + t));
+                    if (j + 1 < n) qk(j + 1, j + 2 == n);
                 }
+                if (ok && n < nmax) skip(at + n * kSlotsPerTile, (nmax - n) * kSlotsPerTile);
                 at += nmax * kSlotsPerTile;
             }
             if (!__all_sync(0xffffffffu, ok)) *abort_flag = 1;
             // every MMA has retired before TMEM and shared memory go
-            ptx::mma_commit_if(e, bar(kBarDrain));
-            ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
+            ptx::mma_commit_if(e, bar(kBarDrain + t));
+            ptx::mbar_wait(bar(kBarDrain + t), 0, kErrWaitMma);
         } else if (warp == 2) {
             // ------------------------------------------------------ V tail
             // The rows of a sequence's last V tile past its end hold the next
@@ -582,10 +586,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         pk[k] = tc::pack2<kBf16>(x.x, x.y);
                     }
                     ptx::tmem_st_x32(s_addr + hf * 32, pk);
+                    // (the first half's product runs under the second half's exponentials)
+                    ptx::tmem_wait_st();
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(bar(kBarP + 2 * t + hf));
                 }
-                ptx::tmem_wait_st();
-                ptx::tc_fence_before();
-                ptx::mbar_arrive(bar(kBarP + t));
                 const float2 a = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
                 l_run = l_run * alpha + (a.x + a.y);
             }
