@@ -242,6 +242,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return d;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float m;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
 // The V tail warp may have nothing to do for the whole of a long item: its limit
 // starts anew while the other roles are at work, and an abort ends it.
 __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile int *abort_flag) {
@@ -545,11 +551,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 float m8[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) m8[k] = tc::f32_of(s[k]);
+                for (int k = 0; k < 8; ++k) m8[k] = fmaxf(tc::f32_of(s[k]), tc::f32_of(s[8 + k]));
 #pragma unroll
-                for (int k = 8; k < kTileK; ++k) m8[k & 7] = fmaxf(m8[k & 7], tc::f32_of(s[k]));
-                const float mx = fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                                       fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7]))) * p.scale_log2;
+                for (int k = 16; k < kTileK; k += 16)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) m8[i] = max3(m8[i], tc::f32_of(s[k + i]), tc::f32_of(s[k + 8 + i]));
+                const float mx = max3(max3(m8[0], m8[1], m8[2]), max3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * p.scale_log2;
                 float alpha = 1.f;
                 if (mx > m_used + kRescaleLog2) {
                     alpha = m_used == -INFINITY ? 0.f : ptx::ex2(m_used - mx);
