@@ -457,19 +457,15 @@ std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k
     shape.pop_back();
     if (!return_lse) shape[0] = 0;
     at::Tensor lse = fresh(shape, at::kFloat, query);
-    at::Tensor w;
-    size_t ws = 0;
-    if (packed && b > 1) {
-        ws = mla_b200_workspace_size_prefill((int)b, tq);
-        w = fresh({(int64_t)ws}, at::kByte, query);
-    }
+    const size_t ws = mla_b200_workspace_size_prefill((int)b, tq);
+    at::Tensor w = fresh({(int64_t)ws}, at::kByte, query);
     auto *fn = bf16 ? mla_b200_prefill_bf16 : mla_b200_prefill_f16;
     const int64_t d = lead - 1;
     check_status(fn(query.data_ptr(), query.stride(d), query.stride(d + 1), k_nope.data_ptr(), k_nope.stride(d),
                     k_nope.stride(d + 1), k_rope.data_ptr(), k_rope.stride(d), v.data_ptr(), v.stride(d),
                     v.stride(d + 1), cu_q, cu_k, (int)b, (int)nh, tq, tk, (int)max_seq_len_q, (int)max_seq_len_k,
                     causal ? 1 : 0, (float)softmax_scale, out.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
-                    ws > 0 ? w.data_ptr() : nullptr, ws, stream_ptr()),
+                    w.data_ptr(), ws, stream_ptr()),
                  "mla_prefill");
     return {out, lse};
 }

@@ -1066,7 +1066,7 @@ int make_tmap_operand(CUtensorMap *map, const Operand &o, int box_rows, bool bf1
 
 struct PrefillWs {
     int2 *pairs;
-    int *num_pairs;
+    int *num_pairs, *next_item;
     long long cap;
     size_t bytes;
 };
@@ -1075,6 +1075,7 @@ PrefillWs prefill_ws(void *base, int batch, long long total_q) {
     PrefillWs w;
     w.cap = total_q / prefill::kItemQ + batch;
     w.num_pairs = static_cast<int *>(base);
+    w.next_item = w.num_pairs + 1;
     w.pairs = reinterpret_cast<int2 *>(static_cast<char *>(base) + 256);
     w.bytes = 256 + (size_t)w.cap * sizeof(int2);
     return w;
@@ -1102,14 +1103,15 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
     if (q.rows >= (1LL << 31) || kn.rows >= (1LL << 31)) return MLA_B200_ERR_UNSUPPORTED;
     const PrefillWs ws = prefill_ws(workspace, batch, q.rows);
     const int blocks = (int)cdiv(max_q, prefill::kItemQ);
-    const bool planned = cu_q != nullptr && batch > 1;
-    const long long pairs = planned ? ws.cap : (long long)batch * blocks;
+    const long long pairs = std::min(ws.cap, (long long)batch * blocks);  // (a bound: lengths are on the device)
     if (pairs * heads >= (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
     int dev;
     DevInfo info;
     int st = current_device(&dev, &info);
     if (st != MLA_B200_OK) return st;
     if (batch == 0 || q.rows == 0 || max_q == 0) return MLA_B200_OK;
+    // up to one item for each SM: no list of them is needed, and nothing to deal out
+    const bool planned = (long long)batch * blocks * heads > info.sms;
     if (planned && (workspace == nullptr || workspace_bytes < ws.bytes)) return MLA_B200_ERR_WORKSPACE;
     if (planned && !aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
     CUtensorMap qm, km, rm, vm;
@@ -1134,17 +1136,18 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
     p.total_k = (int)kn.rows;
     p.causal = causal;
     p.scale_log2 = scale * kLog2e;
-    p.dense_blocks = blocks;
+    p.blocks = blocks;
     const long long head_bytes = std::max(1LL, kn.rows * (MLA_B200_HEAD_DIM + prefill::kV) * 2);
     p.head_group = (int)std::max(1LL, std::min((long long)heads, kPrefillL2 / head_bytes));
     p.out = out;
     p.out_lse = out_lse;
     if (planned) {
-        prefill::plan_kernel<<<1, 1024, 0, stream>>>(p, (int)ws.cap, ws.pairs, ws.num_pairs);
+        prefill::plan_kernel<<<1, 1024, 0, stream>>>(p, (int)ws.cap, ws.pairs, ws.num_pairs, ws.next_item);
         p.pairs = ws.pairs;
         p.num_pairs = ws.num_pairs;
+        p.next_item = ws.next_item;
     }
-    const int grid = (int)std::min<long long>(pairs * heads, info.sms);
+    const int grid = (int)std::min<long long>(planned ? pairs * heads : (long long)batch * blocks * heads, info.sms);
     timing_mark(t_ev_start, stream);
     launch_dependent(prefill::prefill_kernel<kBf16>, dim3(grid), dim3(prefill::kThreads), prefill::kSmemBytes, stream,
                      planned, qm, km, rm, vm, p);

@@ -62,11 +62,17 @@ enum : int {
     kBarO = kBarP + 4,           // [2] PV done
     kBarTail = kBarO + 2,        // [2] a sequence's last V tile landed, rows past its end not yet zeroed
     kBarDrain = kBarTail + 2,    // [2]
-    kNumBars = kBarDrain + 2
+    kBarItem = kBarDrain + 2,    // [4] an item is in the queue
+    kBarItemFree = kBarItem + 4, // [4] every role has read it (11 warps)
+    kNumBars = kBarItemFree + 4
 };
 constexpr int kOffSlot = kOffBar + kNumBars * 8;
 constexpr int kOffAbort = kOffSlot + 4;
-constexpr int kSmemBytes = kOffAbort + 4 + 1024;  // + 1024 alignment slack
+constexpr int kQueue = 4;                        // items
+constexpr int kQueueReaders = 11;                // producer, two MMA issuers, eight softmax warps
+constexpr int kOffItems = (kOffAbort + 4 + 15) / 16 * 16;
+constexpr int kItemBytes = 48;
+constexpr int kSmemBytes = kOffItems + kQueue * kItemBytes + 1024;  // + 1024 alignment slack
 static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
 // 384 threads x 168 registers at launch = 64512; the softmax warpgroups take 208
 // each and the first one keeps 88: 2 x 128 x 208 + 128 x 88 = 64512.
@@ -75,7 +81,7 @@ static_assert(2 * 128 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunc
 constexpr float kRescaleLog2 = 8.f;
 constexpr int kPlanBuckets = 1024;
 constexpr uint64_t kAbortWaitNs = 10000000ull;  // after an error: for copies in flight
-constexpr uint32_t kMaxIdle = 100000000;  // tries of 200 ns and more: 20 s and more
+constexpr uint32_t kMaxIdle = 200000000;  // tries of 40 ns and more: 8 s and more
 
 struct PrefillParams {
     const int32_t *cu_q, *cu_k;  // null: dense
@@ -83,9 +89,10 @@ struct PrefillParams {
     int total_q, total_k;
     int causal;
     float scale_log2;
-    const int2 *pairs;      // {sequence, first query row}, longest first; null: one sequence or a dense batch
+    const int2 *pairs;      // {sequence, first query row}, longest first; null: at most an item for each CTA
     const int *num_pairs;
-    int dense_blocks;       // without pairs: 256-row blocks per sequence
+    int *next_item;         // with pairs: items given out
+    int blocks;             // without pairs: 256-row blocks per sequence
     int head_group;         // heads walked together
     void *out;              // [total_q, heads, 128]
     float *out_lse;         // [total_q, heads] or null
@@ -127,53 +134,47 @@ struct Item {
     int nmax;
 };
 
-// Walks this CTA's items.  Items are laid out by head group (so that the keys and
-// values of the heads in flight stay in L2), within a group by pair (longest first),
-// and dealt to the CTAs back and forth (a CTA that got a long item in one round
-// gets a short one in the next).
-struct Cursor {
-    int round = 0;
-    int pairs, total;
-    __device__ __forceinline__ void init(const PrefillParams &p) {
-        pairs = p.pairs != nullptr ? *p.num_pairs : p.batch * p.dense_blocks;
-        total = pairs * p.heads;
-    }
-    __device__ __forceinline__ bool next(const PrefillParams &p, Item &it) {
-        const int g = gridDim.x, c = blockIdx.x;
-        const int u = round * g + ((round & 1) ? g - 1 - c : c);
-        if (round * g >= total) return false;
-        ++round;
-        it.nmax = -1;  // no item in this round
-        if (u >= total) return true;
+// Item u of the launch, if it has rows.  Items are laid out by head group (so that the
+// keys and values of the heads in flight stay in L2), within a group by pair, longest
+// first.
+__device__ __forceinline__ bool item_at(const PrefillParams &p, int pairs, int u, Item &it) {
+    int b;
+    if (p.pairs != nullptr) {
         const int per = pairs * p.head_group;
         const int grp = u / per, r = u - grp * per;
         const int heads = min(p.head_group, p.heads - grp * p.head_group);
         const int pair = r / heads;
         it.h = grp * p.head_group + (r - pair * heads);
-        int b;
-        if (p.pairs != nullptr) {
-            const int2 pr = p.pairs[pair];
-            b = pr.x;
-            it.row = pr.y;
-        } else {  // last blocks first
-            const int lvl = pair / p.batch;
-            b = pair - lvl * p.batch;
-            it.row = (p.dense_blocks - 1 - lvl) * kItemQ;
-        }
-        it.s = seq_of(p, b);
-        if (it.row >= it.s.lq) return true;
-        it.n[0] = tiles_of(p, it.s, it.row);
-        it.n[1] = tiles_of(p, it.s, it.row + kTileQ);
-        it.nmax = max(it.n[0], it.n[1]);
-        return true;
+        const int2 pr = p.pairs[pair];
+        b = pr.x;
+        it.row = pr.y;
+    } else {
+        const int pair = u / p.heads;
+        it.h = u - pair * p.heads;
+        b = pair / p.blocks;
+        it.row = (pair - b * p.blocks) * kItemQ;
     }
+    it.s = seq_of(p, b);
+    if (it.row >= it.s.lq) return false;
+    it.n[0] = tiles_of(p, it.s, it.row);
+    it.n[1] = tiles_of(p, it.s, it.row + kTileQ);
+    it.nmax = max(it.n[0], it.n[1]);
+    return true;
+}
+static_assert(sizeof(Item) <= kItemBytes, "item queue");
+constexpr int kNoMore = -1;  // nmax of the queue's last entry
+
+// A role's place in the CTA's item queue (whole warps).
+struct Cursor {
+    uint32_t n = 0;
+    __device__ __forceinline__ bool next(uint8_t *smem, uint32_t bar0, volatile int *abort_flag, Item &it);
 };
 
 // {sequence, first row} of every 256-row block, most key tiles first (a counting
 // sort; blocks of one bucket come in any order, which no result depends on).  One
 // block, a warp per sequence.
 __global__ void __launch_bounds__(1024) plan_kernel(const PrefillParams p, int cap, int2 *__restrict__ pairs,
-                                                    int *__restrict__ num_pairs) {
+                                                    int *__restrict__ num_pairs, int *__restrict__ next_item) {
     __shared__ int count[kPlanBuckets];
     __shared__ int warp_tot[32];
     griddep_launch();
@@ -215,7 +216,10 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PrefillParams p, int c
             }
             __syncthreads();
             count[tid] = (warp > 0 ? warp_tot[warp - 1] : 0) + v - own;
-            if (tid == 1023) *num_pairs = min(warp_tot[31], cap);
+            if (tid == 1023) {
+                *num_pairs = min(warp_tot[31], cap);
+                *next_item = 0;
+            }
             __syncthreads();
         }
     }
@@ -254,7 +258,7 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
     for (uint32_t n = 0; n < kMaxIdle; ++n) {
         if (*abort_flag) return false;
         if (ptx::mbar_try_wait(bar, parity)) return true;
-        __nanosleep(200);
+        __nanosleep(40);
     }
     set_device_error(kErrWaitFull);
     return false;
@@ -264,6 +268,17 @@ __device__ __forceinline__ void store32(void *dst, const uint32_t (&v)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
                  : "memory");
+}
+
+__device__ __forceinline__ bool Cursor::next(uint8_t *smem, uint32_t bar0, volatile int *abort_flag, Item &it) {
+    const uint32_t e = n % kQueue;
+    bool ok = wait_or_abort(bar0 + 8 * (kBarItem + e), (n / kQueue) & 1, abort_flag);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    it = *reinterpret_cast<const Item *>(smem + kOffItems + e * kItemBytes);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(bar0 + 8 * (kBarItemFree + e));
+    ++n;
+    return it.nmax != kNoMore;
 }
 
 // qmap: q as (192, heads, rows), box (64, 1, 128); kmap: k_nope as (128, heads,
@@ -283,7 +298,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < kNumBars; ++i)  // (a ring slot is free when both MMA issuers are done with it)
-            ptx::mbar_init(bar(i), i >= kBarP && i < kBarP + 4 ? 128 : i >= kBarEmpty && i < kBarEmpty + kSlots ? 2 : 1);
+            ptx::mbar_init(bar(i), i >= kBarP && i < kBarP + 4 ? 128 : i >= kBarEmpty && i < kBarEmpty + kSlots ? 2 : i >= kBarItemFree && i < kBarItemFree + kQueue ? kQueueReaders : 1);
         *abort_flag = 0;
         ptx::fence_mbarrier_init_cluster();
     }
@@ -305,8 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     griddep_wait();
 
     Cursor cur;
-    cur.init(p);
     Item it{};
+    auto next_item = [&]() -> bool { return cur.next(smem, sbase + kOffBar, abort_flag, it); };
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp == 0) {
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ++at;
                 return s;
             };
-            while (ok && cur.next(p, it)) {
+            while (ok && next_item()) {
                 if (it.nmax <= 0) continue;
                 const int nmax = __shfl_sync(0xffffffffu, it.nmax, 0), h = __shfl_sync(0xffffffffu, it.h, 0);
                 const int k0 = __shfl_sync(0xffffffffu, it.s.k0, 0), q0 = __shfl_sync(0xffffffffu, it.s.q0 + it.row, 0);
@@ -448,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (e) ptx::mbar_arrive(bar(kBarEmpty + (k0 + c) % kSlots));
                 }
             };
-            while (ok && cur.next(p, it)) {
+            while (ok && next_item()) {
                 if (it.nmax <= 0) continue;
                 const int n = __shfl_sync(0xffffffffu, it.n[t], 0), nmax = __shfl_sync(0xffffffffu, it.nmax, 0);
                 if (n > 0) {
@@ -488,9 +503,49 @@ __global__ void __launch_bounds__(kThreads, 1)
             // completes the slots' own barriers.  Two barriers in turn: the producer
             // may be one item ahead, but not two, as the ring does not hold the
             // second's values before the first's are used.
-            uint32_t at = 0, tails = 0;
-            bool ok = true;
-            while (ok && cur.next(p, it)) {
+            //
+            // It also keeps the item queue filled, two ahead of the item it is at: each CTA
+            // takes the next item that nobody has (dealt out in advance, the CTAs ended up to
+            // 30 % apart).
+            uint32_t at = 0, tails = 0, put = 0;
+            bool ok = true, more = true;
+            const int pairs = p.pairs != nullptr ? *p.num_pairs : p.batch * p.blocks, total = pairs * p.heads;
+            auto publish = [&]() {
+                if (!more || !ok) return;
+                const uint32_t q = put % kQueue;
+                ok = __all_sync(0xffffffffu, wait_or_abort(bar(kBarItemFree + q), ((put / kQueue) & 1) ^ 1, abort_flag));
+                if (!ok) return;
+                Item next{};
+                for (;;) {  // (items without rows are left out)
+                    int u = p.pairs != nullptr ? 0 : put == 0 && more ? (int)blockIdx.x : total;
+                    if (p.pairs != nullptr && lane == 0) u = atomicAdd(p.next_item, 1);
+                    u = __shfl_sync(0xffffffffu, u, 0);
+                    if (u >= total) {
+                        more = false;
+                        next.nmax = kNoMore;
+                        break;
+                    }
+                    if (item_at(p, pairs, u, next)) break;
+                    if (p.pairs == nullptr) {  // (its only item)
+                        more = false;
+                        next.nmax = kNoMore;
+                        break;
+                    }
+                }
+                if (lane == 0) {
+                    *reinterpret_cast<Item *>(smem + kOffItems + q * kItemBytes) = next;
+                    ptx::mbar_arrive(bar(kBarItem + q));
+                }
+                __syncwarp();
+                ++put;
+            };
+            publish();
+            publish();
+            for (uint32_t n = 0; ok; ++n) {
+                publish();
+                if (!ok) break;
+                it = *reinterpret_cast<const Item *>(smem + kOffItems + (n % kQueue) * kItemBytes);
+                if (it.nmax == kNoMore) break;
                 if (it.nmax <= 0) continue;
                 const int left = it.s.lk - (it.nmax - 1) * kTileK;  // tokens in the last tile
                 if (left < kTileK) {
@@ -525,8 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t sn = 0;  // S tiles so far (PV tile k completes phase k of kBarO)
         bool ok = true;
         const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-        while (ok && cur.next(p, it)) {
-            if (it.nmax < 0) continue;
+        while (ok && next_item()) {
             const int row = it.row + t * kTileQ + r;
             if (it.row + t * kTileQ >= it.s.lq) continue;
             const int n = it.n[t];
