@@ -65,7 +65,7 @@ SIGNATURES = {
                                                                      _c_size, _vp]),
     "mla_b200_decode_tree_bf16": (_c_int, [_vp] * 5 + [_c_int] * 8 + [_c_float, _c_int, _vp, _c_int, _vp, _vp,
                                                                       _c_size, _vp]),
-    "mla_b200_workspace_size_prefill": (_c_size, [_c_int, _c_ll]),
+    "mla_b200_workspace_size_prefill": (_c_size, [_c_int, _c_int, _c_ll, _c_int, _c_int]),
     **{f"mla_b200_prefill_{t}": (_c_int, [_vp, _c_ll, _c_ll, _vp, _c_ll, _c_ll, _vp, _c_ll, _vp, _c_ll, _c_ll, _vp, _vp,
                                           _c_int, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_float, _vp, _vp,
                                           _vp, _c_size, _vp]) for t in ("f16", "bf16")},

@@ -457,8 +457,8 @@ std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k
     shape.pop_back();
     if (!return_lse) shape[0] = 0;
     at::Tensor lse = fresh(shape, at::kFloat, query);
-    const size_t ws = mla_b200_workspace_size_prefill((int)b, tq);
-    at::Tensor w = fresh({(int64_t)ws}, at::kByte, query);
+    const size_t ws = mla_b200_workspace_size_prefill((int)b, (int)nh, tq, (int)max_seq_len_q, (int)max_seq_len_k);
+    at::Tensor w = fresh({(int64_t)std::max<size_t>(ws, 256)}, at::kByte, query);
     auto *fn = bf16 ? mla_b200_prefill_bf16 : mla_b200_prefill_f16;
     const int64_t d = lead - 1;
     check_status(fn(query.data_ptr(), query.stride(d), query.stride(d + 1), k_nope.data_ptr(), k_nope.stride(d),

@@ -1064,20 +1064,37 @@ int make_tmap_operand(CUtensorMap *map, const Operand &o, int box_rows, bool bf1
     return encode_tmap(map, o.rows > 0 ? o.base : some, 3, dims, strides, box, bf16);
 }
 
+// Shares of the keys for a call with `items` items at most (256 queries of one head):
+// as many as fill the SMs, of four key tiles at least, so that a share's loop is longer
+// than what its start and the join cost (100 queries over 3000 keys, 2 heads: 24.3 us in
+// one share).  1: no split.
+int prefill_splits(long long items, int max_k, int sms) {
+    if (items <= 0 || 2 * items > sms) return 1;
+    const long long tiles = cdiv(max_k, prefill::kTileK);
+    return (int)std::max(1LL, std::min({(long long)sms / items, tiles / 4, (long long)prefill::kMaxSplits}));
+}
+
 struct PrefillWs {
     int2 *pairs;
+    float *part_o, *part_lse;
     int *num_pairs, *next_item;
     long long cap;
     size_t bytes;
 };
 
-PrefillWs prefill_ws(void *base, int batch, long long total_q) {
+PrefillWs prefill_ws(void *base, int batch, long long total_q, int heads = 0, int splits = 1) {
     PrefillWs w;
     w.cap = total_q / prefill::kItemQ + batch;
     w.num_pairs = static_cast<int *>(base);
     w.next_item = w.num_pairs + 1;
     w.pairs = reinterpret_cast<int2 *>(static_cast<char *>(base) + 256);
-    w.bytes = 256 + (size_t)w.cap * sizeof(int2);
+    w.bytes = align_up(256 + (size_t)w.cap * sizeof(int2), 256);
+    if (splits > 1) {
+        const size_t rows = (size_t)splits * total_q * heads;
+        w.part_o = reinterpret_cast<float *>(static_cast<char *>(base) + w.bytes);
+        w.part_lse = w.part_o + rows * prefill::kV;
+        w.bytes += rows * (prefill::kV + 1) * sizeof(float);
+    }
     return w;
 }
 
@@ -1101,9 +1118,9 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
         !aligned(out_lse, 4) || !aligned(cu_q, 4) || !aligned(cu_k, 4))
         return MLA_B200_ERR_INVALID_ARG;
     if (q.rows >= (1LL << 31) || kn.rows >= (1LL << 31)) return MLA_B200_ERR_UNSUPPORTED;
-    const PrefillWs ws = prefill_ws(workspace, batch, q.rows);
     const int blocks = (int)cdiv(max_q, prefill::kItemQ);
-    const long long pairs = std::min(ws.cap, (long long)batch * blocks);  // (a bound: lengths are on the device)
+    const long long most = (long long)batch * blocks;
+    const long long pairs = std::min(q.rows / prefill::kItemQ + batch, most);  // (a bound: lengths are on the device)
     if (pairs * heads >= (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
     int dev;
     DevInfo info;
@@ -1111,9 +1128,11 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
     if (st != MLA_B200_OK) return st;
     if (batch == 0 || q.rows == 0 || max_q == 0) return MLA_B200_OK;
     // up to one item for each SM: no list of them is needed, and nothing to deal out
-    const bool planned = (long long)batch * blocks * heads > info.sms;
-    if (planned && (workspace == nullptr || workspace_bytes < ws.bytes)) return MLA_B200_ERR_WORKSPACE;
-    if (planned && !aligned(workspace, 16)) return MLA_B200_ERR_INVALID_ARG;
+    const bool planned = most * heads > info.sms;
+    const int splits = prefill_splits(most * heads, max_k, info.sms);
+    const PrefillWs ws = prefill_ws(workspace, batch, q.rows, heads, splits);
+    if ((planned || splits > 1) && (workspace == nullptr || workspace_bytes < ws.bytes)) return MLA_B200_ERR_WORKSPACE;
+    if ((planned || splits > 1) && !aligned(workspace, 32)) return MLA_B200_ERR_INVALID_ARG;
     CUtensorMap qm, km, rm, vm;
     st = make_tmap_operand(&qm, q, prefill::kTileQ, kBf16, q.base);
     if (st == MLA_B200_OK) st = make_tmap_operand(&km, kn, prefill::kTileK, kBf16, q.base);
@@ -1141,17 +1160,24 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
     p.head_group = (int)std::max(1LL, std::min((long long)heads, kPrefillL2 / head_bytes));
     p.out = out;
     p.out_lse = out_lse;
+    p.splits = splits;
+    p.part_o = ws.part_o;
+    p.part_lse = ws.part_lse;
     if (planned) {
         prefill::plan_kernel<<<1, 1024, 0, stream>>>(p, (int)ws.cap, ws.pairs, ws.num_pairs, ws.next_item);
         p.pairs = ws.pairs;
         p.num_pairs = ws.num_pairs;
         p.next_item = ws.next_item;
     }
-    const int grid = (int)std::min<long long>(planned ? pairs * heads : (long long)batch * blocks * heads, info.sms);
+    const int grid = (int)std::min<long long>(planned ? pairs * heads : most * heads * splits, info.sms);
     timing_mark(t_ev_start, stream);
     launch_dependent(prefill::prefill_kernel<kBf16>, dim3(grid), dim3(prefill::kThreads), prefill::kSmemBytes, stream,
                      planned, qm, km, rm, vm, p);
     timing_mark(t_ev_stop, stream);
+    if (splits > 1) {
+        using OutT = std::conditional_t<kBf16, __nv_bfloat16, __half>;
+        launch_dependent(prefill::merge_kernel<OutT>, dim3((unsigned)cdiv(q.rows * heads, 8)), dim3(256), 0, stream, true, p);
+    }
     return launch_status();
 }
 }  // namespace
@@ -1270,8 +1296,17 @@ int mla_b200_plan(int batch, int num_heads, long long total_tokens, int max_seq_
     return MLA_B200_OK;
 }
 
-size_t mla_b200_workspace_size_prefill(int batch, long long total_q) {
-    return batch < 0 || total_q < 0 ? 0 : prefill_ws(nullptr, batch, total_q).bytes;
+size_t mla_b200_workspace_size_prefill(int batch, int num_heads, long long total_q, int max_seq_len_q,
+                                       int max_seq_len_k) {
+    if (batch < 0 || num_heads <= 0 || total_q < 0 || max_seq_len_q < 0 || max_seq_len_k < 0) return 0;
+    int num_sms = 0, dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        cudaGetLastError();
+        num_sms = 148;
+    }
+    const long long items = (long long)batch * cdiv(max_seq_len_q, prefill::kItemQ) * num_heads;
+    return prefill_ws(nullptr, batch, total_q, num_heads, prefill_splits(items, max_seq_len_k, num_sms)).bytes;
 }
 
 int mla_b200_prefill_f16(const void *query, long long query_stride, long long query_head_stride, const void *k_nope,

@@ -30,6 +30,7 @@
 // only raised when it grew by more than 2^8.  Every wait is bounded.
 #pragma once
 
+#include "mla_combine.cuh"
 #include "mla_tc.cuh"
 
 namespace mla {
@@ -94,6 +95,9 @@ struct PrefillParams {
     int *next_item;         // with pairs: items given out
     int blocks;             // without pairs: 256-row blocks per sequence
     int head_group;         // heads walked together
+    int splits;             // without pairs: shares of the keys, an item each, joined by merge_kernel
+    float *part_o;          // [splits, total_q, heads, 128], normalized
+    float *part_lse;        // [splits, total_q, heads]
     void *out;              // [total_q, heads, 128]
     float *out_lse;         // [total_q, heads] or null
 };
@@ -128,10 +132,12 @@ __device__ __forceinline__ int tiles_of(const PrefillParams &p, const Seq &s, in
 }
 
 struct Item {
-    Seq s;
+    Seq s;        // (a split's keys start at its own share's first)
     int h, row;   // head, first query row of the item in its sequence
     int n[2];     // key tiles of its two query tiles (n[0] <= n[1] unless tile 1 has no rows)
     int nmax;
+    int ahead;    // keys of the share before and at query row 0 of the sequence, less one (causal)
+    int split;
 };
 
 // Item u of the launch, if it has rows.  Items are laid out by head group (so that the
@@ -139,6 +145,7 @@ struct Item {
 // first.
 __device__ __forceinline__ bool item_at(const PrefillParams &p, int pairs, int u, Item &it) {
     int b;
+    it.split = 0;
     if (p.pairs != nullptr) {
         const int per = pairs * p.head_group;
         const int grp = u / per, r = u - grp * per;
@@ -149,6 +156,8 @@ __device__ __forceinline__ bool item_at(const PrefillParams &p, int pairs, int u
         b = pr.x;
         it.row = pr.y;
     } else {
+        it.split = u % p.splits;
+        u /= p.splits;
         const int pair = u / p.heads;
         it.h = u - pair * p.heads;
         b = pair / p.blocks;
@@ -159,6 +168,16 @@ __device__ __forceinline__ bool item_at(const PrefillParams &p, int pairs, int u
     it.n[0] = tiles_of(p, it.s, it.row);
     it.n[1] = tiles_of(p, it.s, it.row + kTileQ);
     it.nmax = max(it.n[0], it.n[1]);
+    it.ahead = it.s.lk - it.s.lq;
+    if (p.splits > 1) {
+        const int share = (it.nmax + p.splits - 1) / p.splits, j0 = it.split * share;
+        it.n[0] = min(max(it.n[0] - j0, 0), share);
+        it.n[1] = min(max(it.n[1] - j0, 0), share);
+        it.nmax = max(it.n[0], it.n[1]);
+        it.s.k0 += j0 * kTileK;
+        it.s.lk -= j0 * kTileK;
+        it.ahead -= j0 * kTileK;
+    }
     return true;
 }
 static_assert(sizeof(Item) <= kItemBytes, "item queue");
@@ -509,7 +528,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 30 % apart).
             uint32_t at = 0, tails = 0, put = 0;
             bool ok = true, more = true;
-            const int pairs = p.pairs != nullptr ? *p.num_pairs : p.batch * p.blocks, total = pairs * p.heads;
+            const int pairs = p.pairs != nullptr ? *p.num_pairs : p.batch * p.blocks, total = pairs * p.heads * p.splits;
             auto publish = [&]() {
                 if (!more || !ok) return;
                 const uint32_t q = put % kQueue;
@@ -586,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = it.n[t];
             // keys this row sees (rows past the sequence's end: like its last row)
             int sees = it.s.lk;
-            if (p.causal) sees = min(sees, min(row, it.s.lq - 1) + 1 + it.s.lk - it.s.lq);
+            if (p.causal) sees = min(sees, min(row, it.s.lq - 1) + 1 + it.ahead);
             float m_used = -INFINITY, l_run = 0.f;
             for (int j = 0; j < n; ++j, ++sn) {
                 ok = !*abort_flag && ptx::mbar_wait_now(bar(kBarS + t), sn & 1, kErrWaitMma);
@@ -658,8 +677,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             // ------------------------------------------------------ epilogue
             const bool real = row < it.s.lq;
-            const long long orow = (long long)(it.s.q0 + row) * p.heads + it.h;
-            uint8_t *dst = static_cast<uint8_t *>(p.out) + orow * (kV * 2);
+            const bool part = p.splits > 1;
+            const long long orow = ((long long)it.split * p.total_q + it.s.q0 + row) * p.heads + it.h;
+            uint8_t *dst = part ? reinterpret_cast<uint8_t *>(p.part_o + orow * kV)
+                                : static_cast<uint8_t *>(p.out) + orow * (kV * 2);
             const float inv = l_run != 0.f ? 1.f / l_run : 0.f;  // (NaN stays NaN)
             if (n > 0) {
                 ok = __all_sync(0xffffffffu, ptx::mbar_wait_now(bar(kBarO + t), (sn - 1) & 1, kErrWaitMma));
@@ -676,18 +697,29 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = 0u;
                 }
-                uint32_t w[2][8];
+                if (part) {
+                    uint32_t w[4][8];
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    w[k >> 3][k & 7] = tc::pack2<kBf16>(tc::f32_of(o[2 * k]) * inv, tc::f32_of(o[2 * k + 1]) * inv);
-                if (real) {
-                    store32(dst + c * 64, w[0]);
-                    store32(dst + c * 64 + 32, w[1]);
+                    for (int k = 0; k < 32; ++k) w[k >> 3][k & 7] = tc::u32_of(tc::f32_of(o[k]) * inv);
+                    if (real) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) store32(dst + c * 128 + k * 32, w[k]);
+                    }
+                } else {
+                    uint32_t w[2][8];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        w[k >> 3][k & 7] = tc::pack2<kBf16>(tc::f32_of(o[2 * k]) * inv, tc::f32_of(o[2 * k + 1]) * inv);
+                    if (real) {
+                        store32(dst + c * 64, w[0]);
+                        store32(dst + c * 64 + 32, w[1]);
+                    }
                 }
             }
             ptx::tc_fence_before();  // O is read before this thread's next P arrival lets a PV overwrite it
-            if (real && p.out_lse != nullptr)
-                p.out_lse[orow] = l_run != 0.f ? (m_used + __log2f(l_run)) * kLn2 : -INFINITY;
+            float *lse = part ? p.part_lse : p.out_lse;
+            if (real && lse != nullptr)
+                lse[orow] = l_run != 0.f ? (m_used + __log2f(l_run)) * kLn2 : -INFINITY;
         }
         if (!ok) *abort_flag = 1;
     }
@@ -700,6 +732,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tmem_dealloc(tmem, kTmemCols);
     }
 }
+
+// Joins the shares of the keys: out = sum_s e^(lse_s - M) o_s / sum_s e^(lse_s - M).  A
+// warp per (query, head), 4 columns a lane; the shares are few and small (they are made
+// only where there are fewer items than SMs).
+template <typename OutT>
+__global__ void __launch_bounds__(256) merge_kernel(const PrefillParams p) {
+    griddep_wait();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)p.total_q * p.heads, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row >= rows) return;
+    // (a row outside every sequence has no shares)
+    if (p.cu_q != nullptr) {
+        const int i = (int)(row / p.heads);
+        bool in = false;
+        for (int b = lane; b < p.batch; b += 32) {
+            const Seq s = seq_of(p, b);
+            in |= i >= s.q0 && i < s.q0 + s.lq;
+        }
+        if (!__any_sync(0xffffffffu, in)) return;
+    }
+    const float mine = lane < p.splits ? p.part_lse[lane * rows + row] : -INFINITY;
+    const float mx = __any_sync(0xffffffffu, mine != mine) ? NAN : warp_max(mine);
+    const float w = mx == -INFINITY ? 0.f : __expf(mine - mx);  // exp(-inf) = 0
+    const float total = warp_sum(w);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+        const float ws = __shfl_sync(0xffffffffu, w, s);
+        const float4 o = __ldg(reinterpret_cast<const float4 *>(p.part_o + (s * rows + row) * kV) + lane);
+        if (ws != 0.f) {
+            acc.x = fmaf(ws, o.x, acc.x);
+            acc.y = fmaf(ws, o.y, acc.y);
+            acc.z = fmaf(ws, o.z, acc.z);
+            acc.w = fmaf(ws, o.w, acc.w);
+        }
+    }
+    const float inv = total != 0.f ? 1.f / total : 0.f;
+    *reinterpret_cast<uint2 *>(static_cast<OutT *>(p.out) + row * kV + 4 * lane) =
+        make_uint2(pack_out2<OutT>(acc.x * inv, acc.y * inv), pack_out2<OutT>(acc.z * inv, acc.w * inv));
+    if (lane == 0 && p.out_lse != nullptr) p.out_lse[row] = total != 0.f ? mx + __logf(total) : -INFINITY;
+}
+constexpr int kMaxSplits = 32;  // a lane each
 
 }  // namespace prefill
 }  // namespace mla

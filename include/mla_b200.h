@@ -376,10 +376,10 @@ MLA_B200_API int mla_b200_decode_split_f16_noalloc(const void *query, const void
  * last Lq tokens: a chunk of a prompt sees what came before it).  Rows that see no
  * key: out 0 and LSE -inf.  out [total_q, num_heads, 128] in the inputs' type, 32-byte
  * aligned; out_lse [total_q, num_heads] fp32 natural log, or NULL.  Rows of query
- * outside every sequence are not written.  Workspace (with more blocks of 256 queries
- * and heads than the device has SMs; NULL otherwise): mla_b200_workspace_size_prefill,
- * which serves any call of these sizes. */
-MLA_B200_API size_t mla_b200_workspace_size_prefill(int batch, long long total_q);
+ * outside every sequence are not written.  Few queries over many keys are split over
+ * the keys and joined.  Workspace, 32-byte aligned: mla_b200_workspace_size_prefill. */
+MLA_B200_API size_t mla_b200_workspace_size_prefill(int batch, int num_heads, long long total_q,
+                                                    int max_seq_len_q, int max_seq_len_k);
 MLA_B200_API int mla_b200_prefill_f16(const void *query, long long query_stride, long long query_head_stride,
                                       const void *k_nope, long long k_stride, long long k_head_stride,
                                       const void *k_rope, long long rope_stride, const void *v,

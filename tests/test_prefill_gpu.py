@@ -94,6 +94,15 @@ def test_packed_batches_over_longer_keys(lens_q, lens_k, heads, dtype):
     check(lens_q, lens_k, heads, dtype, causal=False, seed=sum(lens_q))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens_q,lens_k,heads", [
+    ([1], [9000], 1), ([300], [5000], 3), ([256, 17, 130], [4096, 2000, 513], 4), ([40, 300], [0, 6000], 2), ([700, 1], [800, 8191], 1)])
+def test_few_queries_over_many_keys(lens_q, lens_k, heads, dtype):
+    """Fewer items than SMs: the keys are split and the shares joined."""
+    check(lens_q, lens_k, heads, dtype, seed=sum(lens_k))
+    check(lens_q, lens_k, heads, dtype, causal=False, seed=sum(lens_k))
+
+
 def test_rows_without_keys():
     got, lse = check([300, 5], [100, 0], 3, torch.float16)   # the first 200 queries come before every key
     assert bool((got[:200] == 0).all()) and bool((got[300:] == 0).all())

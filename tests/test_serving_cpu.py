@@ -87,4 +87,5 @@ def test_prefill_arguments():
     if not torch.cuda.is_available():
         assert call() == capi.ERR_NO_DEVICE
     size = capi.lib().mla_b200_workspace_size_prefill
-    assert size(3, 1000) >= 8 * (1000 // 256 + 3) and size(-1, 5) == 0
+    assert size(3, 128, 1000, 500, 500) >= 8 * (1000 // 256 + 3) and size(-1, 8, 5, 5, 5) == 0
+    assert size(1, 2, 100, 100, 8192) >= 16 * 100 * 2 * 129 * 4  # 2 items: the keys are split
