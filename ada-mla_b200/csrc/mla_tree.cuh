@@ -182,15 +182,19 @@ __device__ void plan_here(const TreeParams &p, int ntiles, int item_cost, int *c
         lens[k] = v < ntiles ? p.seq_lens[v / p.tiles] : 0;
     }
     // the drafts seen, a thread per (tile, draft): one round of loads, beside the lengths'
+    auto draft_mask = [&](int i) -> unsigned long long {
+        const int v = i / p.tile_drafts, b = v / p.tiles;
+        const int d = (v - b * p.tiles) * p.tile_drafts + (i - v * p.tile_drafts);
+        if (i >= ntiles * p.tile_drafts || d >= p.drafts) return 0;
+        const unsigned long long m = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
+        return p.drafts < 64 ? m & ((1ull << p.drafts) - 1) : m;
+    };
+    unsigned long long mine = draft_mask(tid);
     for (int v = tid; v < ntiles; v += kThreads) seen[v] = 0;
     __syncthreads();
     for (int i = tid; i < ntiles * p.tile_drafts; i += kThreads) {
-        const int v = i / p.tile_drafts, b = v / p.tiles;
-        const int d = (v - b * p.tiles) * p.tile_drafts + (i - v * p.tile_drafts);
-        if (d < p.drafts) {
-            const unsigned long long m = p.mask != nullptr ? p.mask[(long long)b * p.mask_stride + d] : (2ull << d) - 1;
-            atomicOr(seen + v, p.drafts < 64 ? m & ((1ull << p.drafts) - 1) : m);
-        }
+        if (i != tid) mine = draft_mask(i);
+        if (mine != 0) atomicOr(seen + i / p.tile_drafts, mine);
     }
 #pragma unroll
     for (int k = 0; k < kPer; ++k) {
@@ -304,6 +308,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         ptx::tmem_alloc(sbase + kOffSlot, kTmemCols);
         ptx::tmem_relinquish();
     }
+    // The cluster barrier is .aligned: a warp that came to it in parts (lanes 1-31 of warp 0
+    // while lane 0 still initialises barriers) would be counted too early, and the partner
+    // could then use barriers that are not there yet.
+    __syncwarp();
     ptx::tc_fence_before();
     ptx::cluster_sync();
     ptx::tc_fence_after();
@@ -819,8 +827,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     // ---------------------------------------------------------------- teardown
     ptx::tc_fence_before();
-    __syncwarp();
     __syncthreads();
+    __syncwarp();
     ptx::cluster_sync();  // neither CTA leaves while its partner may still target it
     if (warp == 2) {
         ptx::tc_fence_after();

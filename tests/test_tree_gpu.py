@@ -173,6 +173,28 @@ def test_large_logits_and_equal_logits():
     assert float((lse.cpu().double() - w[1]).abs().max()) <= 8 * LSE_TOL
 
 
+@pytest.mark.parametrize("batch,k,heads,lens", [(2, 5, 128, [700, 333]), (1, 12, 128, [2000]), (3, 40, 128, [97, 1300, 5]), (1, 64, 3, [900]), (2, 64, 16, [0, 800])])
+def test_bound_far_above_the_lengths(batch, k, heads, lens):
+    """max_seq_len is a bound: the schedule goes by the lengths."""
+    import ada_mla
+
+    lens = [n if n == 0 else max(n, k) for n in lens]
+    q, pool, table, n = problem(batch, k, heads, lens, 32, torch.float16, seed=batch + k)
+    mask = random_tree(batch, k, seed=k)
+    want = expect(q, pool, table, n, mask, torch.float16)
+    wide = torch.full((batch, 2200), -1, dtype=torch.int32)
+    wide[:, :table.shape[1]] = table
+    dev = [t.cuda() for t in (q, pool, wide, n, mask)]
+    for bound in (int(n.max()), 70000):
+        got, lse = ada_mla.mla_decode_tree(*dev, max_seq_len=bound, softmax_scale=SCALE, return_lse=True)
+        assert ada_mla.mla_get_device_error() == 0
+        diff = (got.double().cpu() - want[0]).abs()
+        assert bool((diff <= want[2]).all()), float((diff / want[2].clamp(min=1e-30)).max())
+        none = torch.isinf(want[1])
+        assert bool((torch.isneginf(lse.cpu()) == none).all())
+        assert bool(((lse.cpu().double() - want[1])[~none].abs() <= LSE_TOL).all())
+
+
 def test_max_seq_len_read_from_device_and_other_stream():
     import ada_mla
 
