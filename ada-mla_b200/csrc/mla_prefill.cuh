@@ -434,7 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             // Warp 1 issues for query tile 0, warp 3 for tile 1: one thread's waits, fences
             // and issue slots took 2250 cycles a tile, the products themselves need 1280.
             // (A wait that runs out does not branch off: the tile is finished on whatever
-            // the buffers hold and then given up.)
+            // the buffers hold and then given up, its slots not freed: a load may still be
+            // on its way to one.)
             const int t = warp == 1 ? 0 : 1;
             const uint32_t e = ptx::elect_one();
             constexpr uint32_t idesc_qk = ptx::idesc_f16_f32(kTileQ, kTileK, 0, 0, kBf16);
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int k = 0; k < 4; ++k)
                         ptx::mma_ss_if(e, s_col, a + (uint64_t)(k * 2), b + (uint64_t)(k * 2), idesc_qk,
                                        (c > 0 || k > 0) ? 1u : 0u);
-                    ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                    ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + slot));
                 }
                 ptx::mma_commit_if(e, bar(kBarS + t));
                 if (last) ptx::mma_commit_if(e, bar(kBarQEmpty + t));
@@ -473,13 +474,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < kVHalf / 16; ++k)
                     ptx::mma_ts_if(e, o_col, s_col + (c * 4 + k) * 8, b + (uint64_t)((k * 16 * 128) >> 4), idesc_pv,
                                    (j > 0 || c > 0 || k > 0) ? 1u : 0u);
-                ptx::mma_commit_if(e, bar(kBarEmpty + slot));
+                ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + slot));
             };
             // the slots of a key tile that this query tile does not see
             auto skip = [&](uint32_t k0, int n) {
                 for (int c = 0; c < n; ++c) {
                     full(k0 + c);
-                    if (e) ptx::mbar_arrive(bar(kBarEmpty + (k0 + c) % kSlots));
+                    if (ok && e) ptx::mbar_arrive(bar(kBarEmpty + (k0 + c) % kSlots));
                 }
             };
             while (ok && next_item()) {

@@ -85,7 +85,7 @@ constexpr int kMsgBytes = kMsgP + 2048;        // 26624
 constexpr int kMsgSlots = 3;
 
 enum BarId {
-    kBarFull = 0,                       // ring slot landed (and its hidden rows zeroed)
+    kBarFull = 0,                       // ring slot landed (and its hidden rows zeroed); S-CTA: one of issuer 0's
     kBarEmpty = kSlotsS,                // ring slot consumed
     kBarSFull = 2 * kSlotsS,            // [2] S-CTA: S tile in TMEM
     kBarSEmpty = kBarSFull + 2,         // [2] S-CTA: S tile read (256)
@@ -99,7 +99,8 @@ enum BarId {
     kBarDrain = kBarTail + kSlotsO,     // [2] an issuer's operations retired
     kBarStaged = kBarDrain + 2,         //     S-CTA: a message is in the staging buffer (256)
     kBarStgFree = kBarStaged + 1,       //     S-CTA: it has left it
-    kNumBars = kBarStgFree + 1
+    kBarFull1 = kBarStgFree + 1,        //     S-CTA: ring slot of issuer 1's landed
+    kNumBars = kBarFull1 + kSlotsS
 };
 static_assert(kSlotsS >= kSlotsO, "ring barriers");
 
@@ -346,6 +347,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int nslots = role == 0 ? kSlotsS : kSlotsO;
         tc::Ring rg;
         int prev_b = -1;
+        uint32_t jt = 0;
         bool ok = true;
         auto acquire = [&]() {
             ok = ok && !*abort_flag && ptx::mbar_wait_now(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
@@ -370,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 int n;
                 tree_rows(p, v, q_row, n);
             }
-            for (int t0 = 0; ok && t0 < len; t0 += kTS) {
+            for (int t0 = 0; ok && t0 < len; t0 += kTS, ++jt) {
                 const int piece = t0 / kTO, at = piece % (kRowTiles * kOPerS);
                 if (at == 0) {
                     row = row_next;
@@ -380,6 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int c = 0; c < kOPerS; ++c) pr[c] = __shfl_sync(0xffffffffu, row, at + c);
                 if (role == 0) {
+                    const int full = (jt & 1) ? kBarFull1 : kBarFull;  // the tile's issuer's
 #pragma unroll 1
                     for (int sl = 0; sl < kSlotsPerTile; ++sl) {
                         if (new_q && t0 == 0) {
@@ -390,21 +393,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 if (!ok) break;
                                 const int nb = min(2, kKBlocks - kb);
                                 const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                                ptx::mbar_arrive_expect_tx_if(e, bar(kBarFull + rg.slot), nb * kQBoxBytes);
+                                ptx::mbar_arrive_expect_tx_if(e, bar(full + rg.slot), nb * kQBoxBytes);
                                 for (int j = 0; j < nb; ++j)
                                     ptx::tma_load_2d_if(e, dst + j * kQBoxBytes, &qmap, (kb + j) * 64, (int)q_row,
-                                                        bar(kBarFull + rg.slot));
+                                                        bar(full + rg.slot));
                                 rg.next(nslots);
                             }
                         }
                         acquire();
                         if (!ok) break;
                         const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                        ptx::mbar_arrive_expect_tx_if(e, bar(kBarFull + rg.slot), kSlotS);
+                        ptx::mbar_arrive_expect_tx_if(e, bar(full + rg.slot), kSlotS);
 #pragma unroll
                         for (int c = 0; c < kOPerS; ++c)
                             ptx::tma_load_4d_if(e, dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3,
-                                                bar(kBarFull + rg.slot));
+                                                bar(full + rg.slot));
                         rg.next(nslots);
                     }
                 } else {
@@ -434,7 +437,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // lane behind each instruction, so that descriptors stay in uniform registers: 48
         // cycles an MMA of N = 96 against 53 from a branch of lane 0, and ~100 there when
         // math warps share the scheduler.  So a wait that runs out does not branch off
-        // either: the tile is finished on whatever the buffers hold and then given up.)
+        // either: the tile is finished on whatever the buffers hold and then given up, its
+        // slots not freed: a load may still be on its way to one.)
         const uint32_t e = ptx::elect_one();
         tc::Ring rg;
         uint32_t jt = 0;
@@ -461,11 +465,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             ptx::mma_ss_if(e, tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
                                            c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), tc::idesc_o<kBf16>(),
                                            kk > 0 ? 1u : acc0);
-                    ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                    ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
                     rg.next(kSlotsO);
                 }
-                ptx::mma_commit_mc_if(e, bar(kBarPFree + ms), 0x3);
+                // (in this order: once a message has come through a freed slot, the slot's
+                // last kBarMmaDone phase is known to be complete)
                 ptx::mma_commit_if(e, bar(kBarMmaDone + ms));
+                ptx::mma_commit_mc_if(e, bar(kBarPFree + ms), 0x3);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             }
         }
@@ -477,18 +483,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // Two warps take alternate S tiles (and S buffers).  At the first S tile of a
         // row tile its issuer copies Q into TMEM once every GEMM1 of the previous one
         // is done; the other waits for the copy before its next S tile.
+        //
+        // A wait by parity is exact only while the phase before the awaited one is known
+        // to be complete, and an issuer does not wait for the other's slots: a load that
+        // comes in late would let it take the slot's next use for landed.  So each has
+        // its own set of barriers for the slots, and waits on the barriers they share
+        // (kBarSFull, kBarQReady) only after kBarSEmpty: then the softmax has read tile
+        // jt - 2, so every GEMM1 and copy of Q up to that tile is complete.
         const uint32_t e = ptx::elect_one();
         const uint32_t me = warp == 1 ? 0u : 1u;
         tc::Ring rg;
         uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
+        uint32_t phases = 0;  // per slot: parity of this issuer's next use
         int prev_b = -1;
         bool ok = true;
+        auto full = [&]() {
+            ok &= ptx::mbar_spin(bar((me == 0 ? kBarFull : kBarFull1) + rg.slot), (phases >> rg.slot) & 1, kErrWaitFull);
+            phases ^= 1u << rg.slot;
+        };
         while (ok && items_next<kSched>(wl, cur, it, id)) {
             const int len = __shfl_sync(0xffffffffu, it.len, 0), v = __shfl_sync(0xffffffffu, it.b, 0);
             const bool new_seq = v != prev_b;
             prev_b = v;
             for (int t0 = 0; t0 < len; t0 += kTS, ++jt) {
                 const bool mine = (jt & 1u) == me;
+                const uint32_t sb = jt & 1, use = jt >> 1;
+                if (mine) {
+                    ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                }
                 if (new_seq && t0 == 0) {
                     ++nseq;
                     if (mine) {
@@ -517,8 +540,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     ok &= ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma);
                     qready_seq = nseq;
                 }
-                const uint32_t sb = jt & 1, use = jt >> 1;
-                ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
                 const uint32_t d = tmem + kTmemS + sb * kTS;
@@ -526,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     if (copy_q) {  // K-blocks 0-3, 4-5, 6-8 of Q (see the producer)
                         const int kb0 = sl == 0 ? 0 : sl == 1 ? 4 : 6, kb1 = sl == 0 ? 4 : sl == 1 ? 6 : kKBlocks;
                         for (int kb = kb0; kb < kb1; kb += 2) {
-                            ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                            full();
                             const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
                             const int nb = min(2, kKBlocks - kb);
                             for (int j = 0; j < nb; ++j) {
@@ -535,12 +556,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                     ptx::tmem_cp_128x256b_if(e, tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
                                                              ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
                             }
-                            ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                            ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
                             rg.next(kSlotsS);
                         }
                         if (sl == kSlotsPerTile - 1) ptx::mma_commit_if(e, bar(kBarQReady));
                     }
-                    ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                    full();
                     const uint32_t acc0 = sl > 0 ? 1u : 0u;
                     // the slot's K-blocks interleave per 8-row group: groups 3 KB apart
                     const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kKbPerSlot * 1024);
@@ -549,7 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int k = 0; k < kKbPerSlot * 4; ++k)
                         ptx::mma_ts_if(e, d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * 1024 + (k & 3) * 32) >> 4),
                                        tc::idesc_s<kBf16>(), k > 0 ? 1u : acc0);
-                    ptx::mma_commit_if(e, bar(kBarEmpty + rg.slot));
+                    ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
                     rg.next(kSlotsS);
                 }
                 ptx::mma_commit_if(e, bar(kBarSFull + sb));

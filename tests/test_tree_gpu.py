@@ -226,3 +226,28 @@ def test_refusals():
     with pytest.raises(ValueError):
         ada_mla.mla_decode_tree(**ok, out_dtype=torch.bfloat16)
     assert ada_mla.mla_decode_tree(q[:0], pool, table[:0], n[:0]).shape == (0, 3, 16, 512)
+
+
+def test_calls_back_to_back():
+    """Streams longer than the L2, 112 rows a tile, call after call: loads come in late and
+    out of order, and every call gives the first one's bits."""
+    import ada_mla
+
+    g = torch.Generator().manual_seed(5)
+    lens = [1000 + 97 * i for i in range(48)]
+    sets = []
+    for s in range(2):
+        need = [-(-n // 64) for n in lens]
+        perm = torch.randperm(sum(need), generator=g).to(torch.int32)
+        table = torch.full((48, max(need)), -1, dtype=torch.int32)
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = perm[at:at + n]
+            at += n
+        sets.append((torch.randn(48, 7, 16, 576, generator=g).half().cuda(), torch.randn(sum(need), 64, 576, device="cuda").half(),
+                     table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()))
+    first = [ada_mla.mla_decode_tree(*s, max_seq_len=max(lens), softmax_scale=SCALE) for s in sets]
+    for _ in range(20):
+        outs = [ada_mla.mla_decode_tree(*sets[i % 2], max_seq_len=max(lens), softmax_scale=SCALE) for i in range(40)]
+        assert all(torch.equal(o, first[i % 2]) for i, o in enumerate(outs))
+    assert ada_mla.mla_get_device_error() == 0
