@@ -15,7 +15,10 @@ module (csrc/mla_api.cpp:115-120):
 plus ``mla_decode_batched`` (batch / varlen), ``mla_decode_paged`` (a paged
 latent cache through a block table), ``mla_combine`` (the LSE merge the
 multi-GPU layer uses), ``mla_get_device_error`` and the model constants the
-reference left as a TODO in mla.py:29-34.
+reference left as a TODO in mla.py:29-34; and, for a serving step around the
+decode, ``mla_build_slots`` (pages and slots of new tokens), ``mla_cache_write``
+(latent rows into the cache), ``mla_decode_tree`` (drafts in a tree over the
+pages; ``tree_mask``) and ``mla_prefill`` (prompts in expanded form).
 
 Importing never compiles: the native libraries are built in-tree by
 ``ada_mla._build.build()`` (or the repository's ``__graft_entry__.build()``).

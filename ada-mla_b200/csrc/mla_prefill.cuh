@@ -28,6 +28,11 @@
 // tile), warp 2 TMEM owner and V tail, warps 4-7 softmax of tile 0, warps 8-11 of tile 1 (a thread per row: no
 // shuffles).  The softmax warps rescale O themselves, rarely: the running maximum is
 // only raised when it grew by more than 2^8.  Every wait is bounded.
+//
+// 2048 queries over 8192 keys, 128 heads: 1155-1200 us, 1.00-1.04 PFLOP/s (the GPU's power
+// cap holds the clock near 1.5 GHz); six prompts of 262-1884 tokens, 128 heads: 570-590 us,
+// 0.62 PFLOP/s, where an item's start and end (11 key tiles long on average) cost a quarter;
+// 77 queries, 128 heads: 10.3 us.
 #pragma once
 
 #include "mla_combine.cuh"
