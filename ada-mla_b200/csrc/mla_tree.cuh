@@ -45,9 +45,10 @@
 //
 // A call, with its merge: 64 sequences of 1024-8192 tokens x 112 rows (356 MB of rows)
 // 104 us, 3.4 TB/s and 0.69 PFLOP/s at once; 8 x 1536 rows 148 us, 0.93 PFLOP/s; 512 rows
-// over 131072 tokens 165 us, 0.89 PFLOP/s; 128 rows over 4104 tokens 26 us.  Each S tile
-// takes the pair 2600 cycles where GEMM1 alone needs 1728; the merge and the last items'
-// epilogues are 15 to 20 us of a call.
+// over 131072 tokens 165 us, 0.89 PFLOP/s; 128 rows over 4104 tokens 26 us.  Bound by
+// shared memory: an S tile's rows are written and read once on either SM (220 KB) and its
+// weights as well (50 KB), 2110 cycles at 128 bytes a cycle; 2550 are measured, GEMM1 alone
+// needs 1728.  The merge and the last items' epilogues are 15 to 20 us of a call.
 #pragma once
 
 #include "mla_combine.cuh"
