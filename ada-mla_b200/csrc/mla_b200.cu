@@ -822,12 +822,12 @@ void launch_tree_merge(const tree::TreeParams &p, cudaStream_t stream, bool chai
     // splits: the call takes 26.3 us, 45.6 with a warp per row); many tiles have one or two:
     // a warp per row (64 tiles of 112 rows: 104 us, 122 with 8 warps)
     const dim3 block(32 * tree::kMergeWarps);
-    const unsigned rows = (unsigned)p.num_heads, tiles = (unsigned)p.wl.batch;
+    const unsigned groups = (unsigned)cdiv(p.num_heads, 32), tiles = (unsigned)p.wl.batch, pieces = kDV / 16;
     if (tiles < 8)
-        launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(rows, tiles), block, 0, stream, chain,
-                         p);
+        launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(groups * pieces, tiles), block, 0, stream,
+                         chain, p);
     else
-        launch_dependent(tree::merge_kernel<OutT, 1>, dim3((unsigned)cdiv(rows, tree::kMergeWarps), tiles), block, 0,
+        launch_dependent(tree::merge_kernel<OutT, 1>, dim3(groups * (pieces / tree::kMergeWarps), tiles), block, 0,
                          stream, chain, p);
 }
 

@@ -276,6 +276,12 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
 }
 
+__device__ __forceinline__ void load32(const void *src, uint32_t (&v)[8]) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "l"(src));
+}
+
 __device__ __forceinline__ void store32(void *dst, const uint32_t *v) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(v[0]), "r"(v[1]),
                  "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -865,23 +871,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 }
 
 // O = sum_i e^(lse_i - M) O_i / sum_i e^(lse_i - M), M = max_i lse_i, over the items i
-// of tile v that hold row r's partials.  kRowWarps warps share a row (each every
-// kRowWarps-th split, joined in shared memory in a fixed order): 8 where a few tiles
-// have many splits, else 1.  Lane l owns columns 16 l .. 16 l + 15 (a piece).  Rows of
-// tiles that were one item are complete already.  Bound by the partials' bytes, 1 KB a
-// row and split, and by the latency of three dependent loads; the first splits' partials
-// are asked for before their weights are known.
+// of tile v that hold row r's partials.  A lane per row and a warp per piece of 16
+// columns, as the partials lie: every load is a kilobyte (weights and scales 128 bytes)
+// in a row.  (With a warp per row, its 32 pieces 4 KB apart, the loads took 5 of this
+// kernel's 8 us.)  kRowWarps warps share a piece's splits, each every kRowWarps-th with its
+// own maximum, joined in shared memory in a fixed order: 8 where a few tiles have many
+// splits, else 1.  Rows of tiles that were one item are complete already.  Bound by the
+// latency of two dependent loads, then by the partials' bytes, 1 KB a row and split.
 template <typename OutT, int kRowWarps>
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParams p) {
-    constexpr int kRows = kMergeWarps / kRowWarps;  // rows per block
-    __shared__ float acc_s[kRowWarps > 1 ? kRowWarps - 1 : 1][16][33];
-    __shared__ float sum_s[kMergeWarps];
+    constexpr int kPieces = kMergeWarps / kRowWarps;  // of a block
+    constexpr int kBlocks = kDV / 16 / kPieces;       // that share 32 rows
+    __shared__ float acc_s[kRowWarps > 1 ? kRowWarps - 1 : 1][16][32];
+    __shared__ float max_s[kMergeWarps][32], sum_s[kMergeWarps][32];
     griddep_launch();
     griddep_wait();
     const WorkList &wl = p.wl;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int v = blockIdx.y;
-    const int r = blockIdx.x * kRows + warp / kRowWarps, g = warp % kRowWarps;
+    const int v = blockIdx.y, group = blockIdx.x / kBlocks, g = warp % kRowWarps;
+    const int piece = (blockIdx.x - group * kBlocks) * kPieces + warp / kRowWarps;
     long long row0;
     int rows;
     tree_rows(p, v, row0, rows);
@@ -893,79 +901,76 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
     } else {
         item_range(wl, v, i0, i1);
     }
-    if (i1 - i0 == 1) return;               // the same for the whole block
-    if (r >= rows) return;                  // (with kRowWarps > 1 a block has one row)
-    const int n = i1 - i0;
-    const float *lse0 = p.part_lse + (size_t)i0 * p.num_heads + r;
-    const float *scale0 = p.part_scale + ((size_t)i0 * (kDV / 32) + lane / 2) * p.num_heads + r;
-    const uint8_t *src = p.part_o + part_piece(p, i0, lane, r);
+    // (both the same for the whole block)
+    if (i1 - i0 == 1) return;
+    if (group * 32 >= rows) return;
+    const int n = i1 - i0, r = group * 32 + lane, rr = min(r, rows - 1);
+    const float *lse0 = p.part_lse + (size_t)i0 * p.num_heads + rr;
+    const float *scale0 = p.part_scale + ((size_t)i0 * (kDV / 32) + piece / 2) * p.num_heads + rr;
+    const uint8_t *src = p.part_o + part_piece(p, i0, piece, rr);
     const size_t step = (size_t)p.num_heads * kDV * 2;
     constexpr int kAhead = 4;
-    uint4 u[kAhead][2];
+    uint32_t u[kAhead][8];
     float sc[kAhead];
     auto fetch = [&](int s) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int sj = s + j * kRowWarps;
             if (sj < n) {
-                const uint4 *at = reinterpret_cast<const uint4 *>(src + (size_t)sj * step);
-                u[j][0] = __ldg(at);
-                u[j][1] = __ldg(at + 1);
+                load32(src + (size_t)sj * step, u[j]);
                 sc[j] = __ldg(scale0 + (size_t)sj * (kDV / 32) * p.num_heads);
             }
         }
     };
     fetch(g);
-    float mx = -INFINITY;
-    bool nan = false;
-    for (int s = lane; s < n; s += 32) {
-        const float l = lse0[(size_t)s * p.num_heads];
-        mx = fmaxf(mx, l);
-        nan |= l != l;
-    }
-    mx = __any_sync(0xffffffffu, nan) ? NAN : warp_max(mx);
+    float mx = -INFINITY;  // NaN if any weight is
+#pragma unroll 4
+    for (int s = g; s < n; s += kRowWarps) mx = max_nan(mx, lse0[(size_t)s * p.num_heads]);
     float acc[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
     float wsum = 0.f;
-    if (mx != -INFINITY) {
-        for (int s = g; s < n; s += kRowWarps * kAhead) {
-            if (s != g) fetch(s);
+    for (int s = g; s < n; s += kRowWarps * kAhead) {
+        if (s != g) fetch(s);
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const int sj = s + j * kRowWarps;
-                const float w = sj < n ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;  // exp(-inf) = 0
-                if (w != 0.f) {  // (a split that saw nothing holds zeros)
-                    wsum += w;
-                    const float ws = w * sc[j];
-                    const uint32_t x[8] = {u[j][0].x, u[j][0].y, u[j][0].z, u[j][0].w,
-                                           u[j][1].x, u[j][1].y, u[j][1].z, u[j][1].w};
+        for (int j = 0; j < kAhead; ++j) {
+            const int sj = s + j * kRowWarps;
+            // (exp(-inf) = 0; nothing is added where no split has seen anything)
+            const float w = sj < n && mx != -INFINITY ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;
+            if (w != 0.f) {  // (a split that saw nothing holds zeros)
+                wsum += w;
+                const float ws = w * sc[j];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        acc[2 * k] = fmaf(ws, f32_of_i16(x[k]), acc[2 * k]);
-                        acc[2 * k + 1] = fmaf(ws, f32_of_i16(x[k] >> 16), acc[2 * k + 1]);
-                    }
+                for (int k = 0; k < 8; ++k) {
+                    acc[2 * k] = fmaf(ws, f32_of_i16(u[j][k]), acc[2 * k]);
+                    acc[2 * k + 1] = fmaf(ws, f32_of_i16(u[j][k] >> 16), acc[2 * k + 1]);
                 }
             }
         }
     }
     if constexpr (kRowWarps > 1) {
+        max_s[g][lane] = mx;
+        sum_s[g][lane] = wsum;
         if (g > 0) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc_s[g - 1][e][lane] = acc[e];
-            if (lane == 0) sum_s[g] = wsum;
         }
         __syncthreads();
         if (g > 0) return;
 #pragma unroll
-        for (int k = 1; k < kRowWarps; ++k) {
-            wsum += sum_s[k];
+        for (int k = 1; k < kRowWarps; ++k) mx = max_nan(mx, max_s[k][lane]);
+        wsum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] += acc_s[k - 1][e][lane];
+        for (int k = 0; k < kRowWarps; ++k) {
+            const float f = mx == -INFINITY ? 0.f : __expf(max_s[k][lane] - mx);
+            wsum = fmaf(f, sum_s[k][lane], wsum);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = k == 0 ? acc[e] * f : fmaf(f, acc_s[k > 0 ? k - 1 : 0][e][lane], acc[e]);
         }
     }
+    if (r >= rows) return;
     const float inv = wsum != 0.f ? 1.f / wsum : 0.f;
-    OutT *dst = static_cast<OutT *>(p.out) + (row0 + r) * kDV + lane * 16;
+    OutT *dst = static_cast<OutT *>(p.out) + (row0 + r) * kDV + piece * 16;
     uint32_t o[16];
     if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
@@ -977,7 +982,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
         for (int e = 0; e < 8; ++e) o[e] = pack_out2<OutT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
         store32(dst, o);
     }
-    if (p.out_lse != nullptr && lane == 0) p.out_lse[row0 + r] = wsum != 0.f ? mx + __logf(wsum) : -INFINITY;
+    if (p.out_lse != nullptr && piece == 0) p.out_lse[row0 + r] = wsum != 0.f ? mx + __logf(wsum) : -INFINITY;
 }
 
 }  // namespace tree
