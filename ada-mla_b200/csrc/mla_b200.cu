@@ -818,12 +818,12 @@ TreeTiles tree_tiles(int drafts, int heads) {
 
 template <typename OutT>
 void launch_tree_merge(const tree::TreeParams &p, cudaStream_t stream, bool chain) {
-    // a few tiles have many splits each: a block of 8 warps per row (1 tile of 128 rows, 43
-    // splits: the call takes 26.3 us, 45.6 with a warp per row); many tiles have one or two:
-    // a warp per row (64 tiles of 112 rows: 104 us, 122 with 8 warps)
+    // Few rows have many splits each: 8 warps per 32 rows and piece (1 tile of 128 rows: the
+    // call takes 21.7 us, 33.4 with one warp).  From 512 warps on, one is enough (4 tiles of
+    // 128 rows: 152 us, 156 with 8; 64 tiles of 112 rows: 99 us, 124 with 8).
     const dim3 block(32 * tree::kMergeWarps);
     const unsigned groups = (unsigned)cdiv(p.num_heads, 32), tiles = (unsigned)p.wl.batch, pieces = kDV / 16;
-    if (tiles < 8)
+    if (tiles * groups * pieces < 512)
         launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(groups * pieces, tiles), block, 0, stream,
                          chain, p);
     else
