@@ -44,11 +44,12 @@
 // is bounded.
 //
 // A call, with its merge: 64 sequences of 1024-8192 tokens x 112 rows (356 MB of rows)
-// 104 us, 3.4 TB/s and 0.69 PFLOP/s at once; 8 x 1536 rows 148 us, 0.93 PFLOP/s; 512 rows
-// over 131072 tokens 165 us, 0.89 PFLOP/s; 128 rows over 4104 tokens 26 us.  Bound by
+// 99-104 us, 3.5 TB/s and 0.7 PFLOP/s at once; 8 x 1536 rows 143-150 us, 0.95 PFLOP/s; 512
+// rows over 131072 tokens 152-156 us, 0.95 PFLOP/s; 128 rows over 4104 tokens 21.7 us, one
+// tile through the pair after the other.  Bound by
 // shared memory: an S tile's rows are written and read once on either SM (220 KB) and its
 // weights as well (50 KB), 2110 cycles at 128 bytes a cycle; 2550 are measured, GEMM1 alone
-// needs 1728.  The merge and the last items' epilogues are 15 to 20 us of a call.
+// needs 1728.  An item's epilogue takes 3 us: 128 KB of partials leave one SM.
 #pragma once
 
 #include "mla_combine.cuh"
