@@ -912,7 +912,8 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     p.tiles = tt.tiles;
     p.tile_drafts = tt.tile_drafts;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // a few tiles chain decode -> merge -> next decode (see run_split_decode)
+    // a few tiles chain decode -> merge -> next decode (see run_split_decode; all chained:
+    // 64 tiles 104 -> 102.5 us, 96 tiles 148 -> 155)
     const bool chain = tiles < 8;
     p.chain = chain ? 1 : 0;
     if (empty) {
