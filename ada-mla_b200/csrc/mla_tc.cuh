@@ -102,10 +102,11 @@ constexpr int kMsgSlots = 3;                     // O-CTA receive ring
 
 constexpr int kRingSlots = kSlotsS8;             // the deepest ring (fp8 S-CTA)
 static_assert(kRingSlots >= kSlotsS && kRingSlots >= kSlotsO, "ring barriers");
+constexpr int kFullSets = 2;                     // sets of slot barriers: one for each GEMM1 issuer
 enum BarId {
-    kBarFull = 0,                      // [4] ring slot landed            (count 1 + tx)
-    kBarEmpty = kRingSlots,            // [4] ring slot consumed          (count 1, commit)
-    kBarSFull = 2 * kRingSlots,        // [2] S-CTA: S tile in TMEM        (count 1, commit)
+    kBarFull = 0,                             // [2][slots] ring slot landed (count 1 + tx); O-CTA: set 0
+    kBarEmpty = kFullSets * kRingSlots,       // [slots] ring slot consumed  (count 1, commit)
+    kBarSFull = kBarEmpty + kRingSlots,       // [2] S-CTA: S tile in TMEM   (count 1, commit)
     kBarSEmpty = kBarSFull + 2,        // [2] S-CTA: S tile read           (count 128)
     kBarQFree = kBarSEmpty + 2,        // [2] S-CTA: an issuer's GEMM1s reading Q done (count 1, commit)
     kBarQReady = kBarQFree + 2,        //     S-CTA: a sequence's Q copied into TMEM (count 1, commit)
@@ -375,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
     if (tid == 0) {
         for (int i = 0; i < kRingSlots; ++i) {
-            ptx::mbar_init(bar(kBarFull + i), 1);
+            for (int k = 0; k < kFullSets; ++k) ptx::mbar_init(bar(kBarFull + k * kRingSlots + i), 1);
             ptx::mbar_init(bar(kBarEmpty + i), 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -426,6 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             Ring rg;
             int prev_b = -1;
             bool ok = true;
+            int full = kBarFull;  // S-CTA: the set of the issuer that takes the next S tile
             auto acquire = [&]() -> bool {
                 return !*abort_flag && ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
             };
@@ -449,9 +451,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     for (int kb = 0; kb < kKBlocks; ++kb) {
                         if (!acquire()) { ok = false; break; }
                         const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS8;
-                        ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), 2 * kQBox8);
-                        ptx::tma_load_2d(dst, &qmap, kb * 64, qrow, bar(kBarFull + rg.slot));
-                        ptx::tma_load_2d(dst + kQBox8, &qmap, kb * 64, lo_row, bar(kBarFull + rg.slot));
+                        ptx::mbar_arrive_expect_tx(bar(full + rg.slot), 2 * kQBox8);
+                        ptx::tma_load_2d(dst, &qmap, kb * 64, qrow, bar(full + rg.slot));
+                        ptx::tma_load_2d(dst + kQBox8, &qmap, kb * 64, lo_row, bar(full + rg.slot));
                         rg.next(nslots);
                     }
                     prev_b = it.b;
@@ -462,9 +464,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         if (!acquire()) { ok = false; break; }
                         const int nb = min(2, kKBlocks - kb);
                         const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                        ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), nb * kQBoxBytes);
+                        ptx::mbar_arrive_expect_tx(bar(full + rg.slot), nb * kQBoxBytes);
                         for (int j = 0; j < nb; ++j)
-                            ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, qrow, bar(kBarFull + rg.slot));
+                            ptx::tma_load_2d(dst + j * kQBoxBytes, &qmap, (kb + j) * 64, qrow, bar(full + rg.slot));
                         rg.next(nslots);
                     }
                     prev_b = it.b;
@@ -480,10 +482,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             for (int sl = 0; sl < kSlotsPerTile; ++sl) {
                                 if (!acquire()) { ok = false; break; }
                                 const uint32_t dst = sbase + kOffRing + rg.slot * kSlotS;
-                                ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kSlotS);
+                                ptx::mbar_arrive_expect_tx(bar(full + rg.slot), kSlotS);
 #pragma unroll
                                 for (int c = 0; c < kOPerS; ++c)
-                                    ptx::tma_load_4d(dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3, bar(kBarFull + rg.slot));
+                                    ptx::tma_load_4d(dst + c * kPieceS, &cmap_s, 0, 0, sl * kKbPerSlot, pr[c] >> 3, bar(full + rg.slot));
                                 rg.next(nslots);
                             }
                         } else {
@@ -491,8 +493,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             for (int sl = 0; sl < kSlotsPerTile; ++sl) {
                                 if (!acquire()) { ok = false; break; }
                                 const uint32_t dst = sbase + kOffRing + rg.slot * kSlotBytes;
-                                ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kSlotBytes);
-                                ptx::tma_load_3d(dst, &cmap_s, 0, row, sl * kKbPerSlot, bar(kBarFull + rg.slot));
+                                ptx::mbar_arrive_expect_tx(bar(full + rg.slot), kSlotBytes);
+                                ptx::tma_load_3d(dst, &cmap_s, 0, row, sl * kKbPerSlot, bar(full + rg.slot));
                                 rg.next(nslots);
                             }
                         }
@@ -503,8 +505,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             if constexpr (kPaged) r = ct == 0 ? pr[0] : (ct == 1 ? pr[1] : pr[2]);
                             if (!acquire()) { ok = false; break; }
                             const uint32_t dst = sbase + kOffRing + rg.slot * (kFp8 ? kSlotO8 : kSlotO);
-                            ptx::mbar_arrive_expect_tx(bar(kBarFull + rg.slot), kFp8 ? kSlotO8 : kSlotO);
-                            ptx::tma_load_3d(dst, &cmap_o, 0, r, 0, bar(kBarFull + rg.slot));
+                            ptx::mbar_arrive_expect_tx(bar(full + rg.slot), kFp8 ? kSlotO8 : kSlotO);
+                            ptx::tma_load_3d(dst, &cmap_o, 0, r, 0, bar(full + rg.slot));
                             rg.next(nslots);
                         }
                     }
@@ -512,6 +514,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int c = 0; c < kOPerS; ++c) pr[c] = pn[c];
                     }
+                    if (role == 0) full = kBarFull + kRingSlots - full;
                 }
             }
             if (!ok) *abort_flag = 1;
@@ -529,14 +532,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // sequence (its own and the other issuer's last tile) is done, and the
         // other issuer waits for the copy before its next tile.  Both walk the
         // same items and ring positions, skipping the other's slots.
+        // A wait by parity is exact only while the phase before the awaited one is
+        // known to be complete, and an issuer does not wait for the other's slots: a
+        // load that comes in late would let it take a slot's next use for landed.  So
+        // each has its own set of barriers for the slots, and waits on the barriers
+        // they share (kBarSFull, kBarQReady) only after kBarSEmpty: then the softmax
+        // has read tile jt - 2, so every GEMM1 and copy of Q up to it is complete.
         // O-CTA: lane 0 of warp 1 issues GEMM2.
         if (lane == 0) {
             const int nslots = role == 0 ? (kFp8 ? kSlotsS8 : kSlotsS) : (kFp8 ? kSlotsO8 : kSlotsO);
             const uint32_t me = warp == 1 ? 0u : 1u;
             Ring rg;
             uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
+            uint32_t phases = 0;  // per slot: parity of this issuer's next use
             int prev_b = -1;
             bool ok = true;
+            auto landed = [&]() -> bool {  // (once per use: the next call is for the slot's next use)
+                const uint32_t parity = (phases >> rg.slot) & 1;
+                phases ^= 1u << rg.slot;
+                return ptx::mbar_spin(bar(kBarFull + me * kRingSlots + rg.slot), parity, kErrWaitFull);
+            };
             ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
             Item it;
             int i;
@@ -546,6 +561,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
                     if (role == 0) {
                         const bool mine = (jt & 1u) == me;
+                        const uint32_t sb = jt & 1, use = jt >> 1;
+                        if (mine && (*abort_flag || !ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma))) { ok = false; break; }
                         if (new_seq && t0 == 0) {
                             ++nseq;
                             if (mine) {
@@ -564,7 +581,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                 // copy / MMA reads them.  (A fence stalls this thread until
                                 // the tensor pipe drains, ~230 cycles.)
                                 for (int kb = 0; ok && kb < kKBlocks; kb += kFp8 ? 1 : 2) {
-                                    if (*abort_flag || !ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                                    if (*abort_flag || !landed()) { ok = false; break; }
                                     if constexpr (kFp8) {
                                         // K-block kb of the hi and lo planes: 64 B per row, 16 columns each
                                         const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS8;
@@ -603,12 +620,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             if (!ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma)) { ok = false; break; }
                             qready_seq = nseq;
                         }
-                        const uint32_t sb = jt & 1, use = jt >> 1;
-                        if (*abort_flag || !ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma)) { ok = false; break; }
                         ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
                         const uint32_t d = tmem + kTmemS + sb * kTS;
                         for (int sl = 0; sl < kSlotsPerTile; ++sl) {
-                            if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                            if (!landed()) { ok = false; break; }
                             // descriptor of the slot, plus compile-time offsets per K-step: a
                             // short issue sequence between MMAs
                             const uint32_t acc0 = sl > 0 ? 1u : 0u;
@@ -648,7 +663,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         ptx::tc_fence_after();
                         const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsgO + ms * kMsgStride, 16, 512);
                         for (int ct = 0; ct < nct; ++ct) {
-                            if (!ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull)) { ok = false; break; }
+                            if (!landed()) { ok = false; break; }
                             if constexpr (kPaged) {
                                 // an item's last tile ending inside a 32-row piece: the rows past
                                 // its end are zeroed by the whole warp (the other lanes wait at
