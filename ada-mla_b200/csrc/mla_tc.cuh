@@ -711,8 +711,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             rg.next(nslots);
                         }
                         if (!ok) break;
-                        ptx::mma_commit_mc(bar(kBarPFree + ms), 0x3);
+                        // (in this order: once a message has come through a freed slot, the
+                        // slot's last kBarMmaDone phase is known to be complete)
                         ptx::mma_commit(bar(kBarMmaDone + ms));
+                        ptx::mma_commit_mc(bar(kBarPFree + ms), 0x3);
                     }
                 }
             }

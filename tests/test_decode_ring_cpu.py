@@ -193,3 +193,11 @@ def test_the_model_tells(slots, q_slots, sets, s_empty_first):
         except AssertionError:
             bad += 1
     assert bad > 0
+
+
+def test_gemm2_done_before_its_slot_is_free():
+    """Once a message has come through a freed slot, the slot's last kBarMmaDone phase is
+    known to be complete only if its commit came before the one that freed the slot."""
+    for name in ("mla_tc.cuh", "mla_tree.cuh"):
+        text = source(name)
+        assert text.index("bar(kBarMmaDone + ms)") < text.index("bar(kBarPFree + ms), 0x3")
