@@ -515,8 +515,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 if (ok && n < nmax) skip(at + n * kSlotsPerTile, (nmax - n) * kSlotsPerTile);
                 at += nmax * kSlotsPerTile;
+                // (a wait runs out by each lane's own clock: the lanes go on to the next
+                // item's vote, or to the end, together)
+                ok = __all_sync(0xffffffffu, ok);
             }
-            if (!__all_sync(0xffffffffu, ok)) *abort_flag = 1;
+            if (!ok) *abort_flag = 1;
             // every MMA has retired before TMEM and shared memory go
             ptx::mma_commit_if(e, bar(kBarDrain + t));
             ptx::mbar_wait(bar(kBarDrain + t), 0, kErrWaitMma);
