@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t s = at % kSlots;
                 ok = ok && !*abort_flag && ptx::mbar_wait_now(bar(kBarEmpty + s), ((at / kSlots) & 1) ^ 1, kErrWaitEmpty);
                 ok = __all_sync(0xffffffffu, ok);
-                ++at;
+                if (ok) ++at;
                 return s;
             };
             while (ok && next_item()) {
@@ -426,7 +426,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
                     ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull);
             } else {
-                --at;  // (acquired in vain)
                 for (uint32_t k = at > kSlots ? at - kSlots : 0; k < at; ++k)
                     ptx::mbar_wait(bar(kBarFull + k % kSlots), (k / kSlots) & 1, kErrWaitFull, kAbortWaitNs);
             }

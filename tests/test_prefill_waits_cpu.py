@@ -61,3 +61,23 @@ def test_issuer_lanes_stay_together(seed):
             wait()
         if after:
             ok = [all(ok)] * 32
+
+
+def counts_on_success():
+    """Whether the producer counts a slot only once it has it, and takes none back."""
+    text = role("-- TMA producer", "-- MMA issuers")
+    return "if(ok)++at;" in text and "--at" not in text
+
+
+@pytest.mark.parametrize("fails", ["slot", "q"])
+@pytest.mark.parametrize("before", [0, 1, 7, 8, 9, 20])
+def test_producer_drains_every_load(fails, before):
+    """After a wait that ran out, for a slot or for Q's buffer, the producer waits for the
+    loads it has issued: the last eight slots' may be on their way."""
+    slots, success = 8, counts_on_success()
+    at = before
+    if not success:
+        at += 1 if fails == "slot" else 0  # counted before the wait ran out
+        at -= 1
+    drained = set(range(max(at - slots, 0), at))
+    assert set(range(max(before - slots, 0), before)) <= drained
