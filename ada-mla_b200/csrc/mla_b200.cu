@@ -1123,6 +1123,9 @@ int run_prefill(const Operand &q, const Operand &kn, const Operand &kr, const Op
         !aligned(out_lse, 4) || !aligned(cu_q, 4) || !aligned(cu_k, 4))
         return MLA_B200_ERR_INVALID_ARG;
     if (q.rows >= (1LL << 31) || kn.rows >= (1LL << 31)) return MLA_B200_ERR_UNSUPPORTED;
+    // bounds on the lengths may lie far above them: no sequence is longer than all rows
+    max_q = (int)std::min<long long>(max_q, q.rows);
+    max_k = (int)std::min<long long>(max_k, kn.rows);
     const int blocks = (int)cdiv(max_q, prefill::kItemQ);
     const long long most = (long long)batch * blocks;
     const long long pairs = std::min(q.rows / prefill::kItemQ + batch, most);  // (a bound: lengths are on the device)
@@ -1311,7 +1314,8 @@ size_t mla_b200_workspace_size_prefill(int batch, int num_heads, long long total
         cudaGetLastError();
         num_sms = 148;
     }
-    const long long items = (long long)batch * cdiv(max_seq_len_q, prefill::kItemQ) * num_heads;
+    // (as the call does; its bound on the keys is at most this one, so are its splits)
+    const long long items = (long long)batch * cdiv(std::min<long long>(max_seq_len_q, total_q), prefill::kItemQ) * num_heads;
     return prefill_ws(nullptr, batch, total_q, num_heads, prefill_splits(items, max_seq_len_k, num_sms)).bytes;
 }
 

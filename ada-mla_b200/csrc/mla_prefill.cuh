@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PrefillParams p, int c
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     count[tid] = 0;
     __syncthreads();
-    const int most = (p.max_k + kTileK - 1) / kTileK + 1;
+    const long long most = ((long long)p.max_k + kTileK - 1) / kTileK + 1;  // (above every n: no bucket below 0)
     auto bucket = [&](const Seq &s, int row) {
         const int n = max(tiles_of(p, s, row), tiles_of(p, s, row + kTileQ));
         return kPlanBuckets - 1 - (int)((long long)n * kPlanBuckets / (most + 1));

@@ -221,3 +221,23 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             ada_mla.mla_prefill(**{**ok, **bad})
     assert ada_mla.mla_prefill(q[:0], kv[:0, :, :128], rope[:0], kv[:0, :, 128:], c[:1], c[:1]).shape == (0, 4, 128)
+
+
+@pytest.mark.parametrize("lens_q,lens_k,heads", [([300, 20, 513], [300, 700, 600], 64), ([100], [3000], 2), ([0, 0], [40, 7], 3)])
+def test_bounds_far_above_the_lengths(lens_q, lens_k, heads):
+    """max_seq_len_q / _k are bounds: any that lies above the lengths gives the same bits."""
+    import ada_mla
+
+    q, kv, rope = (t.cuda() for t in problem(lens_q, lens_k, heads, torch.float16, 21))
+
+    def call(bq, bk):
+        return ada_mla.mla_prefill(q, kv[..., :128], rope, kv[..., 128:], cu(lens_q).cuda(), cu(lens_k).cuda(), max_seq_len_q=bq, max_seq_len_k=bk,
+                                   softmax_scale=SCALE, return_lse=True)
+
+    # (bounds at or above all rows are one and the same, so the keys are split alike)
+    want, lse = call(sum(lens_q), sum(lens_k))
+    compare(want, lse, expect(q, kv, rope, lens_q, lens_k, True))
+    for bound in (1 << 20, 2 ** 31 - 128, 2 ** 31 - 127, 2 ** 31 - 1):
+        got, l2 = call(bound, bound)
+        assert torch.equal(got, want) and torch.equal(l2, lse), bound
+    assert ada_mla.mla_get_device_error() == 0
