@@ -80,9 +80,11 @@ __device__ __forceinline__ void unpack_part(const uint4 u, float (&v)[N]) {
 // part_stride: elements from one partial's [num_heads, 512] block to the next
 // (num_heads * 512 in the workspace; larger in a packed exchange buffer, where
 // each part's LSE follows its O), lse_stride likewise for part_lse.
+// (The partials are read with plain loads: this kernel may be resident while the decode
+// still writes them, and the read-only path is for data that nobody writes meanwhile.)
 template <typename OutT, typename PartT>
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(
-    const PartT *__restrict__ part_o, const float *__restrict__ part_lse, WorkList wl,
+    const PartT *part_o, const float *part_lse, WorkList wl,
     int num_heads, long long rows, OutT *__restrict__ out, float *__restrict__ out_lse,
     int skip_single, size_t part_stride, size_t lse_stride) {
     constexpr int kVec = 16 / (int)sizeof(PartT);       // partial elements per thread
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(
                 uint4 u[kInflight];
 #pragma unroll
                 for (int j = 0; j < kInflight; ++j)
-                    if (k + j * kGroups < n) u[j] = __ldg(src + (size_t)(k + j * kGroups) * step);
+                    if (k + j * kGroups < n) u[j] = src[(size_t)(k + j * kGroups) * step];
 #pragma unroll
                 for (int j = 0; j < kInflight; ++j) {
                     if (k + j * kGroups < n) {
@@ -192,12 +194,12 @@ template <typename PartT>
 __device__ __forceinline__ void load16(const PartT *row, int lane, uint4 (&u)[16 / (16 / (int)sizeof(PartT))]) {
     const uint4 *src = reinterpret_cast<const uint4 *>(row) + lane * (16 * (int)sizeof(PartT) / 16);
 #pragma unroll
-    for (int j = 0; j < 16 * (int)sizeof(PartT) / 16; ++j) u[j] = __ldg(src + j);
+    for (int j = 0; j < 16 * (int)sizeof(PartT) / 16; ++j) u[j] = src[j];
 }
 
 template <typename OutT, typename PartT>
 __global__ void __launch_bounds__(32 * kRowsPerCombineBlock) combine_rows_kernel(
-    const PartT *__restrict__ part_o, const float *__restrict__ part_lse, WorkList wl, int num_heads,
+    const PartT *part_o, const float *part_lse, WorkList wl, int num_heads,
     OutT *__restrict__ out, float *__restrict__ out_lse, int skip_single) {
     constexpr int kU = 16 * (int)sizeof(PartT) / 16;  // 16-byte vectors per lane per split
     griddep_launch();

@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const PrefillParams p) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s = 0; s < p.splits; ++s) {
         const float ws = __shfl_sync(0xffffffffu, w, s);
-        const float4 o = __ldg(reinterpret_cast<const float4 *>(p.part_o + (s * rows + row) * kV) + lane);
+        const float4 o = reinterpret_cast<const float4 *>(p.part_o + (s * rows + row) * kV)[lane];
         if (ws != 0.f) {
             acc.x = fmaf(ws, o.x, acc.x);
             acc.y = fmaf(ws, o.y, acc.y);

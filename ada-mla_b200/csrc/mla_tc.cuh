@@ -818,7 +818,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
                                 for (int k = 0; k < kTS; ++k) {
                                     if (k < nv) {
-                                        const float sc = __ldg(kvs + k);
+                                        const float sc = kvs[k];
                                         r[k] = u32_of(fmaf(f32_of(r[k]) * sc, sl2, (float)scale_exp(sc)));
                                     }
                                 }
@@ -858,8 +858,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                     const float p0 = ptx::ex2(f32_of(r[k]) + nmk);
                                     const float p1 = ptx::ex2(f32_of(r[k + 1]) + nmk);
                                     // row sum of w * 2^-e; GEMM2 weight w * mantissa
-                                    const float sc0 = k < valid ? __ldg(kvs + k) : 1.f;
-                                    const float sc1 = k + 1 < valid ? __ldg(kvs + k + 1) : 1.f;
+                                    const float sc0 = k < valid ? kvs[k] : 1.f;
+                                    const float sc1 = k + 1 < valid ? kvs[k + 1] : 1.f;
                                     s4[(k >> 1) & 3] += p0 * scale_pow2_inv(sc0) + p1 * scale_pow2_inv(sc1);
                                     pk[k >> 1] = pack2<false>(p0 * scale_mant(sc0), p1 * scale_mant(sc1));
                                 }

@@ -334,7 +334,7 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 __device__ __forceinline__ void load32(const void *src, uint32_t (&v)[8]) {
-    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "l"(src));
 }
@@ -942,6 +942,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // own maximum, joined in shared memory in a fixed order: 8 where a few tiles have many
 // splits, else 1.  Rows of tiles that were one item are complete already.  Bound by the
 // latency of two dependent loads, then by the partials' bytes, 1 KB a row and split.
+// (Plain loads, not the read-only path: it may be resident while the decode writes.)
 template <typename OutT, int kRowWarps>
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParams p) {
     constexpr int kPieces = kMergeWarps / kRowWarps;  // of a block
@@ -982,7 +983,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
             const int sj = s + j * kRowWarps;
             if (sj < n) {
                 load32(src + (size_t)sj * step, u[j]);
-                sc[j] = __ldg(scale0 + (size_t)sj * (kDV / 32) * p.num_heads);
+                sc[j] = scale0[(size_t)sj * (kDV / 32) * p.num_heads];
             }
         }
     };

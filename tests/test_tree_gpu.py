@@ -251,3 +251,21 @@ def test_calls_back_to_back():
         outs = [ada_mla.mla_decode_tree(*sets[i % 2], max_seq_len=max(lens), softmax_scale=SCALE) for i in range(40)]
         assert all(torch.equal(o, first[i % 2]) for i, o in enumerate(outs))
     assert ada_mla.mla_get_device_error() == 0
+
+
+@pytest.mark.parametrize("batch,k,heads,n", [(1, 8, 16, 1500), (2, 7, 16, 700), (1, 12, 128, 900), (7, 3, 16, 400)])
+def test_chained_calls_back_to_back(batch, k, heads, n):
+    """Up to 7 row tiles decode, merge and next decode are chained: a merge is resident while
+    its decode writes.  Calls on inputs in turn give each input's own bits."""
+    import ada_mla
+
+    lens = [n - 40 * b for b in range(batch)]
+    sets = [[t.cuda() for t in problem(batch, k, heads, lens, 64, torch.float16, seed=30 + s)] for s in range(3)]
+    first = []
+    for s in sets:
+        first.append(ada_mla.mla_decode_tree(*s, max_seq_len=n, softmax_scale=SCALE, return_lse=True))
+        torch.cuda.synchronize()
+    for _ in range(20):
+        outs = [ada_mla.mla_decode_tree(*sets[i % 3], max_seq_len=n, softmax_scale=SCALE, return_lse=True) for i in range(60)]
+        assert all(torch.equal(o, first[i % 3][0]) and torch.equal(l, first[i % 3][1]) for i, (o, l) in enumerate(outs))
+    assert ada_mla.mla_get_device_error() == 0
