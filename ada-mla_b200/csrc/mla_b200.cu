@@ -893,9 +893,8 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     tree::TreeParams p{};
     p.num_heads = rows;
     p.scale_log2 = softmax_scale * kLog2e;
-    // (the workspace has room for fp32 partials: the 16-bit ones, then their scales)
-    p.part_o = reinterpret_cast<uint8_t *>(L.part_o);
-    p.part_scale = reinterpret_cast<float *>(p.part_o + align_up((size_t)max_items * rows * kDV * 2, 256));
+    p.part_hi = reinterpret_cast<uint8_t *>(L.part_o);  // (32-bit partials in two planes)
+    p.part_lo = p.part_hi + (size_t)max_items * rows * kDV * 2;
     p.part_lse = L.part_lse;
     p.out = out;
     p.out_kind = out_dtype == MLA_B200_OUT_F16 ? tc::kOutF16 : out_dtype == MLA_B200_OUT_BF16 ? tc::kOutBF16 : tc::kOutF32;

@@ -28,13 +28,12 @@
 //     padded drafts that may never have been written) are zeroed by a warp of their own
 //     before GEMM2 (0 x NaN is not 0): such tiles land on that warp's barrier, which
 //     then completes the slot's.  No other tile pays for it;
-//   * partials are 16-bit whole numbers with an fp32 scale for every 32 columns of a row
-//     (its largest value / 32767): half the bytes of fp32, whose 256 KB an item took one SM
-//     8 us to store, and an error of 2^-16 of the largest of 32 neighbours (about 2e-5 of
-//     a typical value), where a 16-bit float's 2^-12 would add a third rounding of the
-//     size of the output's own.  They lie 32 bytes (16 columns) of all rows together, so a
-//     warp's store is one kilobyte in a row.  (A partial that is not finite makes its 32
-//     columns NaN.)
+//   * partials are fp32, in two planes: the upper 16 bits of each value and what is kept of
+//     the lower ones, all 16 for fp32 output, 8 for 16-bit output.  24 bits keep every value
+//     to 2^-15 of itself (1/16 of fp16's rounding, whatever its neighbours hold) at three
+//     quarters of the bytes (128 rows over 4104 tokens 23.3 us a call, 24.8 with 32 bits; 64
+//     sequences x 112 rows 121.6, 124).  Each plane lies 16 columns (32 or 16 bytes) of all
+//     rows together, so a warp's stores are whole kilobytes in a row;
 //
 //   * the schedule is made inside the kernel (plan_here).
 //
@@ -139,8 +138,8 @@ struct TreeParams {
     WorkList wl;
     int num_heads;     // rows of a full tile = rows between partials: tile_drafts * heads
     float scale_log2;  // softmax scale * log2(e)
-    uint8_t *part_o;   // [items, 32 pieces, num_heads, 16] int16: see part_piece
-    float *part_scale; // [items, 16 chunks, num_heads]
+    uint8_t *part_hi;  // [items, 32 pieces, num_heads, 16] upper 16 bits: see part_piece
+    uint8_t *part_lo;  // the same of the lower 16 bits (fp32 output), or the upper 8 of them
     float *part_lse;   // [items, num_heads]
     void *out;         // [batch, drafts, heads, 512]: written directly for tiles of one item
     int out_kind;      // tc::OutKind
@@ -308,21 +307,15 @@ __device__ __forceinline__ int pool_row(const TreeParams &p, int b, int t, int l
     return pg * p.page_size + (tc - blk * p.page_size);
 }
 
-// Byte offset of 16 columns (16 piece ..) of row r of an item's partial.
+// Place of 16 columns (16 piece ..) of row r of an item's partial, in units of 16 columns.
 __device__ __forceinline__ size_t part_piece(const TreeParams &p, int item, int piece, int r) {
-    return (((size_t)item * (kDV / 16) + piece) * p.num_heads + r) * 32;
+    return ((size_t)item * (kDV / 16) + piece) * p.num_heads + r;
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float m;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
     return m;
-}
-
-// A 16-bit whole number as fp32, without the conversion instruction: its bits with the
-// sign flipped are the last of 2^23 + 2^15 + x.
-__device__ __forceinline__ float f32_of_i16(uint32_t x) {
-    return tc::f32_of((x & 0xffffu) ^ 0x4b008000u) - 8421376.f;
 }
 
 __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -337,6 +330,17 @@ __device__ __forceinline__ void load32(const void *src, uint32_t (&v)[8]) {
     asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
                  : "l"(src));
+}
+
+__device__ __forceinline__ void load16(const void *src, uint32_t (&v)[4]) {
+    asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "l"(src));
+}
+
+__device__ __forceinline__ void store16(void *dst, const uint32_t *v) {
+    asm volatile("st.global.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                 : "memory");
 }
 
 __device__ __forceinline__ void store32(void *dst, const uint32_t *v) {
@@ -872,25 +876,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             ptx::tmem_ld_x32(o_addr + c * 32, r);
                             ptx::tmem_wait_ld();
                             if (!single) {
-                                float top[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) top[k & 3] = max_nan(top[k & 3], fabsf(tc::f32_of(r[k])));
-                                const float most = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
-                                const float up = most > 0.f ? 32767.f / most : 0.f;
-                                // round(x * up) by the addition of 1.5 * 2^23, whose low bits then
-                                // are the whole number (a conversion instruction has a quarter of
-                                // an addition's rate: 4096 cycles an item)
+                                const int piece = half * (kDV / 32) + 2 * c;
+                                const size_t at = part_piece(p, id, piece, h), next = part_piece(p, id, piece + 1, h);
                                 uint32_t o[16];
 #pragma unroll
-                                for (int k = 0; k < 16; ++k)
-                                    o[k] = __byte_perm(tc::u32_of(fmaf(tc::f32_of(r[2 * k]), up, 12582912.f)),
-                                                       tc::u32_of(fmaf(tc::f32_of(r[2 * k + 1]), up, 12582912.f)), 0x5410);
+                                for (int k = 0; k < 32; ++k) r[k] = tc::u32_of(tc::f32_of(r[k]) * inv_l);
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __byte_perm(r[2 * k], r[2 * k + 1], 0x7632);
                                 if (h < nrows) {
-                                    const int piece = half * (kDV / 32) + 2 * c;
-                                    store32(p.part_o + part_piece(p, id, piece, h), o);
-                                    store32(p.part_o + part_piece(p, id, piece + 1, h), o + 8);
-                                    p.part_scale[((size_t)id * (kDV / 32) + piece / 2) * p.num_heads + h] =
-                                        most * (1.f / 32767.f) * inv_l + most * 0.f;  // (infinite: NaN)
+                                    store32(p.part_hi + at * 32, o);
+                                    store32(p.part_hi + next * 32, o + 8);
+                                }
+                                if (f32) {
+#pragma unroll
+                                    for (int k = 0; k < 16; ++k) o[k] = __byte_perm(r[2 * k], r[2 * k + 1], 0x5410);
+                                    if (h < nrows) {
+                                        store32(p.part_lo + at * 32, o);
+                                        store32(p.part_lo + next * 32, o + 8);
+                                    }
+                                } else {  // cut, not rounded: a carry could turn a NaN into a number
+#pragma unroll
+                                    for (int k = 0; k < 8; ++k)
+                                        o[k] = __byte_perm(__byte_perm(r[4 * k], r[4 * k + 1], 0x0051),
+                                                           __byte_perm(r[4 * k + 2], r[4 * k + 3], 0x0051), 0x5410);
+                                    if (h < nrows) {
+                                        store16(p.part_lo + at * 16, o);
+                                        store16(p.part_lo + next * 16, o + 4);
+                                    }
                                 }
                             } else if (f32) {
 #pragma unroll
@@ -936,12 +948,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // O = sum_i e^(lse_i - M) O_i / sum_i e^(lse_i - M), M = max_i lse_i, over the items i
 // of tile v that hold row r's partials.  A lane per row and a warp per piece of 16
-// columns, as the partials lie: every load is a kilobyte (weights and scales 128 bytes)
+// columns, as the partials lie: every load is whole kilobytes (the weights' 128 bytes)
 // in a row.  (With a warp per row, its 32 pieces 4 KB apart, the loads took 5 of this
 // kernel's 8 us.)  kRowWarps warps share a piece's splits, each every kRowWarps-th with its
 // own maximum, joined in shared memory in a fixed order: 8 where a few tiles have many
 // splits, else 1.  Rows of tiles that were one item are complete already.  Bound by the
-// latency of two dependent loads, then by the partials' bytes, 1 KB a row and split.
+// latency of two dependent loads, then by the partials' bytes, 1.5 KB a row and split (2
+// for fp32 output).
 // (Plain loads, not the read-only path: it may be resident while the decode writes.)
 template <typename OutT, int kRowWarps>
 __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParams p) {
@@ -971,19 +984,21 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
     if (group * 32 >= rows) return;
     const int n = i1 - i0, r = group * 32 + lane, rr = min(r, rows - 1);
     const float *lse0 = p.part_lse + (size_t)i0 * p.num_heads + rr;
-    const float *scale0 = p.part_scale + ((size_t)i0 * (kDV / 32) + piece / 2) * p.num_heads + rr;
-    const uint8_t *src = p.part_o + part_piece(p, i0, piece, rr);
-    const size_t step = (size_t)p.num_heads * kDV * 2;
+    constexpr bool kWhole = sizeof(OutT) == 4;  // 32 bits of a partial, else 24
+    constexpr int kLo = kWhole ? 32 : 16;        // bytes of 16 columns' lower plane
+    const uint8_t *hi0 = p.part_hi + part_piece(p, i0, piece, rr) * 32;
+    const uint8_t *lo0 = p.part_lo + part_piece(p, i0, piece, rr) * kLo;
+    const size_t step = (size_t)p.num_heads * (kDV / 16);
     constexpr int kAhead = 4;
-    uint32_t u[kAhead][8];
-    float sc[kAhead];
+    uint32_t hi[kAhead][8], lo[kAhead][kLo / 4];
     auto fetch = [&](int s) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int sj = s + j * kRowWarps;
             if (sj < n) {
-                load32(src + (size_t)sj * step, u[j]);
-                sc[j] = scale0[(size_t)sj * (kDV / 32) * p.num_heads];
+                load32(hi0 + (size_t)sj * step * 32, hi[j]);
+                if constexpr (kWhole) load32(lo0 + (size_t)sj * step * kLo, lo[j]);
+                else load16(lo0 + (size_t)sj * step * kLo, lo[j]);
             }
         }
     };
@@ -1004,11 +1019,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
             const float w = sj < n && mx != -INFINITY ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;
             if (w != 0.f) {  // (a split that saw nothing holds zeros)
                 wsum += w;
-                const float ws = w * sc[j];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    acc[2 * k] = fmaf(ws, f32_of_i16(u[j][k]), acc[2 * k]);
-                    acc[2 * k + 1] = fmaf(ws, f32_of_i16(u[j][k] >> 16), acc[2 * k + 1]);
+                for (int e = 0; e < 16; ++e) {
+                    const uint32_t up = hi[j][e / 2];
+                    uint32_t x;
+                    if constexpr (kWhole) x = __byte_perm(lo[j][e / 2], up, e & 1 ? 0x7632 : 0x5410);
+                    else x = __byte_perm(lo[j][e / 4], up, (e & 1 ? 0x7600 : 0x5400) + (e & 3) * 16) & 0xffffff00u;
+                    acc[e] = fmaf(w, tc::f32_of(x), acc[e]);
                 }
             }
         }

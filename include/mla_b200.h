@@ -260,8 +260,10 @@ MLA_B200_API int mla_b200_decode_mtp_bf16(const void *query, const void *cache,
  * Sequences shorter than num_drafts have only their last drafts' rows.
  * num_drafts <= 64, num_heads <= 128.  The drafts fill tiles of 128 / num_heads
  * whole drafts, and each tile is one pass over the cache.  out [batch, num_drafts,
- * num_heads, 512] and the workspace are 32-byte aligned; out_lse [batch, num_drafts, num_heads] or NULL; otherwise the
- * contract of mla_b200_decode_paged_f16 / _bf16.  Workspace:
+ * num_heads, 512] and the workspace are 32-byte aligned; out_lse [batch, num_drafts,
+ * num_heads] or NULL; otherwise the contract of mla_b200_decode_paged_f16 / _bf16.  Where
+ * a sequence is split, its partial outputs keep 24 bits of each fp32 value (all 32 for fp32
+ * output).  Workspace:
  * mla_b200_workspace_size_tree (0 for sizes that the decode refuses). */
 MLA_B200_API size_t mla_b200_workspace_size_tree(int batch, int num_drafts, int num_heads,
                                                  int max_seq_len, int num_splits);

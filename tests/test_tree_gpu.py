@@ -269,3 +269,60 @@ def test_chained_calls_back_to_back(batch, k, heads, n):
         outs = [ada_mla.mla_decode_tree(*sets[i % 3], max_seq_len=n, softmax_scale=SCALE, return_lse=True) for i in range(60)]
         assert all(torch.equal(o, first[i % 3][0]) and torch.equal(l, first[i % 3][1]) for i, (o, l) in enumerate(outs))
     assert ada_mla.mla_get_device_error() == 0
+
+
+def uneven(batch, k, heads, lens, dtype, seed, span):
+    """Latent columns of sizes 1 to 2^span within any 32 neighbours, all of one sign, so that
+    no column's output averages out; the queries take the sizes out of the logits again."""
+    q, pool, table, n = problem(batch, k, heads, lens, 64, dtype, seed)
+    size = 2.0 ** (torch.arange(512) * 7 % (span + 1))
+    pool[..., :512] = (pool[..., :512].float().abs() * size).to(dtype)
+    q[..., :512] = (q[..., :512].float() / size).to(dtype)
+    return q, pool, table, n
+
+
+@pytest.mark.parametrize("out_dtype", [None, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("span", [6, 10])
+@pytest.mark.parametrize("k,heads,lens", [(8, 16, [1900]), (7, 16, [1100, 300, 2000]), (12, 128, [800])])
+def test_columns_of_different_sizes(k, heads, lens, span, dtype, out_dtype):
+    """A column's error goes by that column's values, whatever its neighbours hold and
+    whether the sequence is split or not.  For 16-bit output the split partials are fp32 cut
+    to 24 bits, below 2^-15 of each value: 2^-15 A on top of the bound above."""
+    import ada_mla
+
+    q, pool, table, n = uneven(len(lens), k, heads, lens, dtype, 40 + k, span)
+    mask = random_tree(len(lens), k, seed=k)
+    w, wl, tol = expect(q, pool, table, n, mask, dtype, out_dtype)
+    if out_dtype is None:
+        tol = tol + 2.0 ** -15 * w  # (all values are positive: A is the output itself)
+    for splits in (-1, 1, 3):
+        got, _ = check(q, pool, table, n, mask, num_splits=splits, out_dtype=out_dtype, want=(w, wl, tol))
+    assert ada_mla.mla_get_device_error() == 0
+
+
+@pytest.mark.parametrize("num_splits", [-1, 1, 4])
+def test_an_infinite_value_stays_in_its_column(num_splits):
+    """A cached row with an infinite value whose logit is -inf: 0 x inf in that column, and
+    nothing else changes."""
+    import ada_mla
+
+    q, pool, table, n = problem(1, 8, 16, [1500], 64, torch.float16, seed=50)
+    q[..., 100] = -1.0
+    at = int(table[0, 3]) * 64 + 5
+    flat = pool.view(-1, 576)
+    flat[at, 100] = float("inf")
+    rows = torch.arange(1500) != 3 * 64 + 5
+    c = rows_of(pool, table, 0, 1500)[rows].double()
+    dev = [t.cuda() for t in (q, pool, table, n)]
+    got, lse = ada_mla.mla_decode_tree(*dev, max_seq_len=1500, softmax_scale=SCALE, num_splits=num_splits, return_lse=True)
+    got = got.double().cpu()
+    assert bool(got[..., 100].isnan().all())
+    keep = torch.arange(512) != 100
+    for i in range(8):
+        see = c[:1499 - 7 + i]
+        p = torch.softmax(q[0, i].double() @ see.t() * SCALE, 1)
+        o, a = p @ see[:, :512], p @ see[:, :512].abs()
+        tol = (2.0 ** -11 + 2.0 ** -13) * a + 2.0 ** -25 * see[:, :512].abs().sum(0) + 2.0 ** -11 * o.abs() + 2.0 ** -24 + 2.0 ** -15 * a
+        assert bool(((got[0, i] - o).abs() <= tol)[:, keep].all())
+    assert ada_mla.mla_get_device_error() == 0
