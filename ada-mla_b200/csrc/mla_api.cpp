@@ -505,10 +505,17 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> mla_build
         head = free_head->data_ptr<int32_t>();
     }
     c10::cuda::CUDAGuard g(seq_lens.device());
-    Carve all(Carve::room(num_tokens, 8) + Carve::room(num_tokens, 4) + Carve::room(b + 1, 4) + Carve::room(b, 4) + 16,
-              seq_lens);
-    at::Tensor slots = all.take(num_tokens, at::kLong), positions = all.take(num_tokens, at::kInt);
-    at::Tensor cu_new = all.take(b + 1, at::kInt), lens = all.take(b, at::kInt), new_head = all.take(1, at::kInt);
+    // A caller keeps the lengths and the head from step to step.  In one allocation with the
+    // tokens' 12 bytes each they would keep those too, so that is for small steps alone (256
+    // tokens: 8.8 us a call, 9.5 with two allocations; 381 000 tokens: 10.2 either way).
+    const bool together = num_tokens <= 4096;
+    const int64_t token_bytes = Carve::room(num_tokens, 8) + Carve::room(num_tokens, 4);
+    const int64_t request_bytes = Carve::room(b + 1, 4) + Carve::room(b, 4) + 16;
+    Carve of_tokens(token_bytes + (together ? request_bytes : 0), seq_lens);
+    at::Tensor slots = of_tokens.take(num_tokens, at::kLong), positions = of_tokens.take(num_tokens, at::kInt);
+    Carve of_requests = together ? of_tokens : Carve(request_bytes, seq_lens);
+    at::Tensor cu_new = of_requests.take(b + 1, at::kInt), lens = of_requests.take(b, at::kInt);
+    at::Tensor new_head = of_requests.take(1, at::kInt);
     check_status(mla_b200_build_slots(seq_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
                                       block_table.data_ptr<int32_t>(),
                                       b > 1 ? block_table.stride(0) : block_table.size(1), (int)block_table.size(1),

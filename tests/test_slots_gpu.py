@@ -118,3 +118,18 @@ def test_other_stream():
         p = ada_mla.mla_build_slots(lens, torch.full_like(lens, 100), table, free, 64, 800)
     s.synchronize()
     assert p.cu_new.tolist() == list(range(0, 801, 100)) and int(p.free_head) == 8
+
+
+@pytest.mark.parametrize("tokens", [1, 256, 4096, 4097, 100000])
+def test_what_a_caller_keeps_is_small(tokens):
+    """The lengths and the head go on to the next step: what they keep alive does not grow
+    with the step's tokens."""
+    import ada_mla
+
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    table, free = torch.zeros(3, 2000, dtype=torch.int32, device="cuda"), torch.arange(2000, dtype=torch.int32, device="cuda")
+    p = ada_mla.mla_build_slots(lens, torch.tensor([tokens, 0, 0], dtype=torch.int32, device="cuda"), table, free, 64, tokens)
+    assert p.seq_lens.tolist() == [tokens, 0, 0] and int(p.free_head) == -(-tokens // 64)
+    assert p.slots[-1].item() == tokens - 1 and p.positions[-1].item() == tokens - 1
+    for kept in (p.seq_lens, p.free_head, p.cu_new):
+        assert kept.untyped_storage().nbytes() <= 12 * 4096 + 256
