@@ -287,7 +287,9 @@ def mla_prefill(query, k_nope, k_rope, v, cu_seqlens_q=None, cu_seqlens_k=None, 
     cu_seqlens_q, cu_seqlens_k
                  int32 [B + 1] on the device: sequence b's queries and keys.  Without
                  them the inputs are dense: [B, Lq, n_h, 192], [B, Lk, n_h, 128],
-                 [B, Lk, 64].  Pass the longest lengths to avoid device->host reads.
+                 [B, Lk, 64], sequences of more than one row following one another
+                 (stride(0) = L * stride(1); a slice like q[:, -1:] is taken as it is,
+                 q[:, -2:] needs a copy).  Pass the longest lengths to avoid device->host reads.
     causal       query i of a sequence sees keys 0 .. i + Lk - Lq: its queries are its
                  last Lq tokens, so a chunk of a prompt sees all that came before.
     Returns [.., n_h, 128] in the inputs' dtype and, with ``return_lse``, the

@@ -388,7 +388,8 @@ std::vector<at::Tensor> mla_decode_tree(const at::Tensor &query, const at::Tenso
 //   query [Tq, n_h, 192], k_nope and v [Tk, n_h, 128], k_rope [Tk, 64], fp16 or bf16
 //   alike, packed by int32 cu_seqlens_q / cu_seqlens_k [B + 1]; or, without them,
 //   [B, Lq, n_h, 192], [B, Lk, n_h, 128], [B, Lk, 64].  Any strides with a dense last
-//   dimension and 16-byte multiples.  max_seq_len_* < 0 reads them from the device.
+//   dimension and 16-byte multiples; dense sequences of more than one row follow one
+//   another.  max_seq_len_* < 0 reads them from the device.
 // Returns (out [.., n_h, 128], lse [.., n_h] fp32 or empty).
 std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k_nope, const at::Tensor &k_rope,
                                     const at::Tensor &v, const c10::optional<at::Tensor> &cu_seqlens_q,
@@ -400,17 +401,19 @@ std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k
     const int64_t lead = packed ? 1 : 2;
     const bool bf16 = query.scalar_type() == at::kBFloat16;
     TORCH_CHECK(query.scalar_type() == at::kHalf || bf16, "mla_prefill: float16 or bfloat16 inputs expected");
+    // elements from one row to the next (dense sequences of one row: from one to the next)
+    auto row_stride = [&](const at::Tensor &t) { return !packed && t.size(1) == 1 ? t.stride(0) : t.stride(lead - 1); };
     auto check = [&](const at::Tensor &t, const char *name, int64_t heads, int64_t width) {
         TORCH_CHECK(t.is_cuda() && t.device() == query.device(), name, " must be a CUDA tensor on the query's device");
         TORCH_CHECK(t.scalar_type() == query.scalar_type(), "mla_prefill: ", name, " must have the query's dtype");
         TORCH_CHECK(t.dim() == lead + (heads > 0 ? 2 : 1) && t.size(-1) == width && (heads <= 0 || t.size(-2) == heads),
                     "mla_prefill: ", name, " has the wrong shape");
         TORCH_CHECK(t.numel() == 0 || t.stride(-1) == 1, "mla_prefill: ", name, " must have a dense last dimension");
-        TORCH_CHECK(packed || t.size(0) <= 1 || t.size(1) == 0 || t.stride(0) == t.size(1) * t.stride(1),
+        TORCH_CHECK(packed || t.size(0) <= 1 || t.size(1) <= 1 || t.stride(0) == t.size(1) * t.stride(1),
                     "mla_prefill: ", name, "'s sequences must follow one another");
+        const int64_t rows = packed ? t.size(0) : t.size(0) * t.size(1);
         TORCH_CHECK(t.numel() == 0 || (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
-                                       (t.size(lead - 1) <= 1 || t.stride(lead - 1) % 8 == 0) &&
-                                       (heads <= 1 || t.stride(lead) % 8 == 0)),
+                                       (rows <= 1 || row_stride(t) % 8 == 0) && (heads <= 1 || t.stride(lead) % 8 == 0)),
                     "mla_prefill: ", name, " must start and step in multiples of 16 bytes");
     };
     TORCH_CHECK(query.is_cuda() && query.dim() == lead + 2 && query.size(-2) >= 1,
@@ -461,8 +464,8 @@ std::vector<at::Tensor> mla_prefill(const at::Tensor &query, const at::Tensor &k
     at::Tensor w = fresh({(int64_t)std::max<size_t>(ws, 256)}, at::kByte, query);
     auto *fn = bf16 ? mla_b200_prefill_bf16 : mla_b200_prefill_f16;
     const int64_t d = lead - 1;
-    check_status(fn(query.data_ptr(), query.stride(d), query.stride(d + 1), k_nope.data_ptr(), k_nope.stride(d),
-                    k_nope.stride(d + 1), k_rope.data_ptr(), k_rope.stride(d), v.data_ptr(), v.stride(d),
+    check_status(fn(query.data_ptr(), row_stride(query), query.stride(d + 1), k_nope.data_ptr(), row_stride(k_nope),
+                    k_nope.stride(d + 1), k_rope.data_ptr(), row_stride(k_rope), v.data_ptr(), row_stride(v),
                     v.stride(d + 1), cu_q, cu_k, (int)b, (int)nh, tq, tk, (int)max_seq_len_q, (int)max_seq_len_k,
                     causal ? 1 : 0, (float)softmax_scale, out.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
                     w.data_ptr(), ws, stream_ptr()),

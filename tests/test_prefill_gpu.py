@@ -241,3 +241,26 @@ def test_bounds_far_above_the_lengths(lens_q, lens_k, heads):
         got, l2 = call(bound, bound)
         assert torch.equal(got, want) and torch.equal(l2, lse), bound
     assert ada_mla.mla_get_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_dense_single_rows_of_longer_sequences(dtype):
+    """The last query of each dense sequence (q[:, -1:]), and single keys, are taken where
+    they lie; longer slices, whose sequences do not follow one another, are refused."""
+    import ada_mla
+
+    batch, n, heads = 5, 300, 6
+    q, kv, rope = problem([n] * batch, [n] * batch, heads, dtype, 17)
+    dev = [t.cuda() for t in (q, kv, rope)]
+    qd, kvd, rd = (t.view(batch, n, *t.shape[1:]) for t in dev)
+    got, lse = ada_mla.mla_prefill(qd[:, -1:], kvd[..., :128], rd, kvd[..., 128:], softmax_scale=SCALE, return_lse=True)
+    assert got.shape == (batch, 1, heads, 128) and lse.shape == (batch, 1, heads)
+    last = torch.arange(1, batch + 1) * n - 1
+    compare(got[:, 0], lse[:, 0], expect(q[last], kv, rope, [1] * batch, [n] * batch, True))
+    one, l1 = ada_mla.mla_prefill(qd[:, :1], kvd[:, 7:8, :, :128], rd[:, 7:8], kvd[:, 7:8, :, 128:], softmax_scale=SCALE, return_lse=True)
+    at = torch.arange(batch) * n
+    compare(one[:, 0], l1[:, 0], expect(q[at], kv[at + 7], rope[at + 7], [1] * batch, [1] * batch, True))
+    with pytest.raises(RuntimeError):
+        ada_mla.mla_prefill(qd[:, -2:], kvd[..., :128], rd, kvd[..., 128:])
+    with pytest.raises(RuntimeError):
+        ada_mla.mla_prefill(qd[:, -1:], kvd[:, 1:, :, :128], rd[:, 1:], kvd[:, 1:, :, 128:])
