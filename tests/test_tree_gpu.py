@@ -326,3 +326,25 @@ def test_an_infinite_value_stays_in_its_column(num_splits):
         tol = (2.0 ** -11 + 2.0 ** -13) * a + 2.0 ** -25 * see[:, :512].abs().sum(0) + 2.0 ** -11 * o.abs() + 2.0 ** -24 + 2.0 ** -15 * a
         assert bool(((got[0, i] - o).abs() <= tol)[:, keep].all())
     assert ada_mla.mla_get_device_error() == 0
+
+
+@pytest.mark.parametrize("batch,k,heads", [
+    (31, 4, 16), (32, 4, 16), (480, 2, 128), (961, 2, 16), (481, 2, 128), (1030, 3, 32), (35, 32, 128)])
+def test_many_row_tiles(batch, k, heads):
+    """31 / 32 and 960 / 961 row tiles are where the schedule is made in another way; above
+    1024 the plan kernel takes more than one round.  Lengths from zero on, a tree for each
+    sequence whose last draft is padding on a row of NaN."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, 130, (batch,), generator=g).tolist()
+    lens[0], lens[batch // 2], lens[-1] = 900, 0, 700
+    q, pool, table, n = problem(batch, k, heads, lens, 32, torch.float16, seed=60)
+    mask = random_tree(batch, k, seed=61)
+    mask[:, -1] = 0
+    want = expect(q, pool, table, n, mask, torch.float16)
+    flat = pool.view(-1, 576)
+    for b, m in enumerate(lens):
+        if m > 0:
+            flat[int(table[b, (m - 1) // 32]) * 32 + (m - 1) % 32] = float("nan")
+    a, la = check(q, pool, table, n, mask, want=want)
+    b, lb = check(q, pool, table, n, mask, want=want)
+    assert torch.equal(a, b) and torch.equal(la, lb)
