@@ -290,12 +290,15 @@ struct WsLayout {
     size_t bytes = 0;
 };
 
+// tree_slots: a draft tree's partial slots (0: every item has its own, and no tree).
 WsLayout ws_layout(void *base, long long max_items, int num_heads, int batch, bool fp8 = false,
-                   bool tree = false) {
+                   long long tree_slots = 0) {
     WsLayout L;
     size_t off = 0;
-    const size_t o_bytes = (size_t)max_items * num_heads * kDV * sizeof(float);
-    const size_t l_bytes = (size_t)max_items * num_heads * sizeof(float);
+    const bool tree = tree_slots > 0;
+    const long long slots = tree ? tree_slots : max_items;
+    const size_t o_bytes = (size_t)slots * num_heads * kDV * sizeof(float);
+    const size_t l_bytes = (size_t)slots * num_heads * sizeof(float);
     const size_t off_bytes = (size_t)(batch + 1) * sizeof(int);
     const size_t it_bytes = (size_t)max_items * sizeof(int4);
     char *p = static_cast<char *>(base);
@@ -816,6 +819,19 @@ TreeTiles tree_tiles(int drafts, int heads) {
     return {tiles, (int)cdiv(drafts, tiles)};
 }
 
+// Items of a call at most, partial slots, and rows of an item (0: the balanced schedule).
+struct TreeItems {
+    int chunk;
+    long long items, slots;
+};
+
+TreeItems tree_items(int tiles, int longest, int num_splits, int clusters) {
+    if (num_splits <= 0) return {0, (long long)tiles + clusters, 2LL * clusters};  // (part_slot)
+    const int chunk = (int)std::min<long long>(std::max(1LL, cdiv(cdiv(longest, num_splits), kTile)) * kTile, 1 << 30);
+    const long long items = max_items_for(tiles, (long long)tiles * longest, chunk);
+    return {chunk, items, items};
+}
+
 template <typename OutT>
 void launch_tree_merge(const tree::TreeParams &p, cudaStream_t stream, bool chain) {
     // Few rows have many splits each: 8 warps per 32 rows and piece (1 tile of 128 rows: the
@@ -870,10 +886,11 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     // 96 tokens 139 and 153); an explicit one: fixed chunks (whole S tiles), by a plan kernel.
     const bool balanced = num_splits <= 0;
     const bool planned_here = balanced && tiles <= tree::kPlanMax;
-    const int chunk = balanced ? 0 : (int)std::min<long long>(std::max(1LL, cdiv(cdiv(longest, num_splits), kTile)) * kTile, 1 << 30);
-    const long long max_items = balanced ? tiles + info.tc_clusters : max_items_for((int)tiles, tiles * longest, chunk);
+    const TreeItems ti = tree_items((int)tiles, longest, num_splits, info.tc_clusters);
+    const int chunk = ti.chunk;
+    const long long max_items = ti.items;
     if (max_items > (1LL << 30)) return MLA_B200_ERR_UNSUPPORTED;
-    const WsLayout L = ws_layout(workspace, max_items, rows, (int)tiles, false, true);
+    const WsLayout L = ws_layout(workspace, max_items, rows, (int)tiles, false, ti.slots);
     if (workspace == nullptr || workspace_bytes < L.bytes) return MLA_B200_ERR_WORKSPACE;
     if (!aligned(workspace, 32)) return MLA_B200_ERR_INVALID_ARG;
     const long long cost_most = tiles * (cdiv(longest, kTile) + item_cost_for(rows));
@@ -894,7 +911,7 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     p.num_heads = rows;
     p.scale_log2 = softmax_scale * kLog2e;
     p.part_hi = reinterpret_cast<uint8_t *>(L.part_o);  // (32-bit partials in two planes)
-    p.part_lo = p.part_hi + (size_t)max_items * rows * kDV * 2;
+    p.part_lo = p.part_hi + (size_t)ti.slots * rows * kDV * 2;
     p.part_lse = L.part_lse;
     p.out = out;
     p.out_kind = out_dtype == MLA_B200_OUT_F16 ? tc::kOutF16 : out_dtype == MLA_B200_OUT_BF16 ? tc::kOutBF16 : tc::kOutF32;
@@ -1347,21 +1364,27 @@ int mla_b200_prefill_bf16(const void *query, long long query_stride, long long q
 }
 
 namespace {
-size_t workspace_bytes_for(int batch, int num_heads, long long total_tokens, int max_seq_len,
-                           int num_splits, bool fp8, bool tree = false) {
-    if (batch < 0 || num_heads <= 0 || total_tokens < 0) return 0;
+// SMs of the current device, or B200's where there is none (sizes can be asked for anywhere).
+int sm_count() {
     int num_sms = 0, dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess ||
         cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
         cudaGetLastError();
         num_sms = 148;
     }
+    return num_sms;
+}
+
+size_t workspace_bytes_for(int batch, int num_heads, long long total_tokens, int max_seq_len,
+                           int num_splits, bool fp8) {
+    if (batch < 0 || num_heads <= 0 || total_tokens < 0) return 0;
+    const int num_sms = sm_count();
     if (max_seq_len <= 0 && batch > 0) max_seq_len = (int)cdiv(total_tokens, batch);
     const int chunk = chunk_for(batch, total_tokens, max_seq_len, num_splits, num_sms, num_heads);
     long long max_items = max_items_for(batch, total_tokens, chunk);
     // an automatic split may run the balanced schedule: batch + one item per cluster
     if (num_splits <= 0) max_items = std::max(max_items, (long long)batch + std::max(1, num_sms / 2));
-    return ws_layout(nullptr, max_items, num_heads, batch, fp8, tree).bytes;
+    return ws_layout(nullptr, max_items, num_heads, batch, fp8).bytes;
 }
 }  // namespace
 
@@ -1390,9 +1413,8 @@ size_t mla_b200_workspace_size_tree(int batch, int num_drafts, int num_heads, in
     const TreeTiles tt = tree_tiles(num_drafts, num_heads);
     const long long tiles = (long long)batch * tt.tiles;
     if (tiles > 65535) return 0;
-    // (paged items start on 96-token boundaries, so they are at least as long as planned here)
-    return workspace_bytes_for((int)tiles, tt.tile_drafts * num_heads, tiles * max_seq_len, max_seq_len, num_splits,
-                               false, true);
+    const TreeItems ti = tree_items((int)tiles, max_seq_len, num_splits, std::max(1, sm_count() / 2));
+    return ws_layout(nullptr, ti.items, tt.tile_drafts * num_heads, (int)tiles, false, ti.slots).bytes;
 }
 
 int mla_b200_decode_tree_f16(const void *query, const void *kv_pages, const int32_t *block_table,

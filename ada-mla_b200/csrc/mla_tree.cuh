@@ -138,9 +138,9 @@ struct TreeParams {
     WorkList wl;
     int num_heads;     // rows of a full tile = rows between partials: tile_drafts * heads
     float scale_log2;  // softmax scale * log2(e)
-    uint8_t *part_hi;  // [items, 32 pieces, num_heads, 16] upper 16 bits: see part_piece
+    uint8_t *part_hi;  // [slots, 32 pieces, num_heads, 16] upper 16 bits: see part_piece
     uint8_t *part_lo;  // the same of the lower 16 bits (fp32 output), or the upper 8 of them
-    float *part_lse;   // [items, num_heads]
+    float *part_lse;   // [slots, num_heads]
     void *out;         // [batch, drafts, heads, 512]: written directly for tiles of one item
     int out_kind;      // tc::OutKind
     float *out_lse;    // [batch, drafts, heads] or null
@@ -307,9 +307,17 @@ __device__ __forceinline__ int pool_row(const TreeParams &p, int b, int t, int l
     return pg * p.page_size + (tc - blk * p.page_size);
 }
 
-// Place of 16 columns (16 piece ..) of row r of an item's partial, in units of 16 columns.
-__device__ __forceinline__ size_t part_piece(const TreeParams &p, int item, int piece, int r) {
-    return ((size_t)item * (kDV / 16) + piece) * p.num_heads + r;
+// Partial slot of item `id`, the `s`-th of tile v.  The balanced schedule gives worker w
+// the items id = v + w (items_next): of a split tile's items the later ones are their
+// worker's first and the first one its worker's last, so two slots a worker hold all
+// partials, however many tiles there are.
+__device__ __forceinline__ size_t part_slot(const WorkList &wl, bool balanced, int v, int id, int s) {
+    return balanced ? id - v + (s == 0 ? wl.nworkers : 0) : id;
+}
+
+// Place of 16 columns (16 piece ..) of row r of a partial, in units of 16 columns.
+__device__ __forceinline__ size_t part_piece(const TreeParams &p, size_t slot, int piece, int r) {
+    return (slot * (kDV / 16) + piece) * p.num_heads + r;
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
@@ -868,7 +876,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         tree_rows(p, it.b, row0, nrows);
                         const float inv_l = l_fin != 0.f ? 1.f / l_fin : 0.f;  // (NaN stays NaN)
                         const bool f32 = p.out_kind == tc::kOutF32;
-                        const size_t row = single ? (size_t)row0 + h : (size_t)id * p.num_heads + h;
+                        const size_t slot = part_slot(wl, kSched == kSchedBalanced, it.b, id, id - i0);
+                        const size_t row = single ? (size_t)row0 + h : slot * p.num_heads + h;
                         uint8_t *dst = static_cast<uint8_t *>(p.out) + (row * kDV + half * (kDV / 2)) * (f32 ? 4 : 2);
 #pragma unroll 1
                         for (int c = 0; c < kDV / 64; ++c) {
@@ -877,7 +886,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                             ptx::tmem_wait_ld();
                             if (!single) {
                                 const int piece = half * (kDV / 32) + 2 * c;
-                                const size_t at = part_piece(p, id, piece, h), next = part_piece(p, id, piece + 1, h);
+                                const size_t at = part_piece(p, slot, piece, h), next = part_piece(p, slot, piece + 1, h);
                                 uint32_t o[16];
 #pragma unroll
                                 for (int k = 0; k < 32; ++k) r[k] = tc::u32_of(tc::f32_of(r[k]) * inv_l);
@@ -983,12 +992,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
     if (i1 - i0 == 1) return;
     if (group * 32 >= rows) return;
     const int n = i1 - i0, r = group * 32 + lane, rr = min(r, rows - 1);
-    const float *lse0 = p.part_lse + (size_t)i0 * p.num_heads + rr;
+    auto slot = [&](int s) { return part_slot(wl, wl.chunk == 0, v, i0 + s, s); };
+    auto lse = [&](int s) { return p.part_lse[slot(s) * p.num_heads + rr]; };
     constexpr bool kWhole = sizeof(OutT) == 4;  // 32 bits of a partial, else 24
     constexpr int kLo = kWhole ? 32 : 16;        // bytes of 16 columns' lower plane
-    const uint8_t *hi0 = p.part_hi + part_piece(p, i0, piece, rr) * 32;
-    const uint8_t *lo0 = p.part_lo + part_piece(p, i0, piece, rr) * kLo;
-    const size_t step = (size_t)p.num_heads * (kDV / 16);
     constexpr int kAhead = 4;
     uint32_t hi[kAhead][8], lo[kAhead][kLo / 4];
     auto fetch = [&](int s) {
@@ -996,16 +1003,17 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
         for (int j = 0; j < kAhead; ++j) {
             const int sj = s + j * kRowWarps;
             if (sj < n) {
-                load32(hi0 + (size_t)sj * step * 32, hi[j]);
-                if constexpr (kWhole) load32(lo0 + (size_t)sj * step * kLo, lo[j]);
-                else load16(lo0 + (size_t)sj * step * kLo, lo[j]);
+                const size_t at = part_piece(p, slot(sj), piece, rr);
+                load32(p.part_hi + at * 32, hi[j]);
+                if constexpr (kWhole) load32(p.part_lo + at * kLo, lo[j]);
+                else load16(p.part_lo + at * kLo, lo[j]);
             }
         }
     };
     fetch(g);
     float mx = -INFINITY;  // NaN if any weight is
 #pragma unroll 4
-    for (int s = g; s < n; s += kRowWarps) mx = max_nan(mx, lse0[(size_t)s * p.num_heads]);
+    for (int s = g; s < n; s += kRowWarps) mx = max_nan(mx, lse(s));
     float acc[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[e] = 0.f;
@@ -1016,7 +1024,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) merge_kernel(const TreeParam
         for (int j = 0; j < kAhead; ++j) {
             const int sj = s + j * kRowWarps;
             // (exp(-inf) = 0; nothing is added where no split has seen anything)
-            const float w = sj < n && mx != -INFINITY ? __expf(lse0[(size_t)sj * p.num_heads] - mx) : 0.f;
+            const float w = sj < n && mx != -INFINITY ? __expf(lse(sj) - mx) : 0.f;
             if (w != 0.f) {  // (a split that saw nothing holds zeros)
                 wsum += w;
 #pragma unroll

@@ -89,3 +89,41 @@ def test_prefill_arguments():
     size = capi.lib().mla_b200_workspace_size_prefill
     assert size(3, 128, 1000, 500, 500) >= 8 * (1000 // 256 + 3) and size(-1, 8, 5, 5, 5) == 0
     assert size(1, 2, 100, 100, 8192) >= 16 * 100 * 2 * 129 * 4  # 2 items: the keys are split
+
+
+def test_tree_workspace_does_not_grow_with_the_tiles():
+    """Two partial slots a cluster hold whatever the automatic schedule splits; only the
+    schedule's tables grow."""
+    size = capi.lib().mla_b200_workspace_size_tree
+    slots = 148 * 128 * (512 + 1) * 4  # 148 SMs, 128 rows
+    for batch, drafts in ((1, 4), (256, 8), (2000, 32), (65535, 1)):
+        tiles = batch * drafts  # 128 heads: a tile a draft
+        assert size(batch, drafts, 128, 32767, -1) <= slots + 64 * (tiles + 148) + 4096, (batch, drafts)
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_partial_slots_of_the_balanced_schedule(seed):
+    """The schedule's items, as its workers walk them: those of split tiles have slots of
+    their own below two a worker (part_slot in csrc/mla_tree.cuh)."""
+    import random
+
+    rng = random.Random(seed)
+    workers, cost = rng.choice((1, 2, 13, 74)), rng.randrange(1, 5)
+    tiles = [rng.choice((0, 1, 2, rng.randrange(0, 300))) for _ in range(rng.choice((1, 3, 31, 200, 1100)))]
+    base, total = [], 0
+    for n in tiles:
+        base.append(total + cost)
+        total += n + cost if n > 0 else 0
+    quota = max(1, -(-total // workers))
+    taken = set()
+    for v, n in enumerate(tiles):
+        if n == 0:
+            continue
+        first, last = base[v] // quota, (base[v] + n - 1) // quota
+        if first == last:
+            continue
+        for s, w in enumerate(range(first, last + 1)):
+            ident = v + w
+            slot = ident - v + (workers if s == 0 else 0)
+            assert 0 <= slot < 2 * workers and slot not in taken
+            taken.add(slot)
