@@ -36,8 +36,9 @@
 // tcgen05.cp before the GEMM1 MMAs that read it (the copy and the MMAs are
 // ordered in the tensor pipe), releasing the slot with a commit.
 //
-// Warp roles (256 threads): warp 0 TMA producer, warp 1 MMA issuer (one
-// thread), warp 2 TMEM allocator, warps 4-7 the math warpgroup (softmax in
+// Warp roles (256 threads): warp 0 TMA producer, warps 1 and 3 MMA issuers
+// (S-CTA: alternate S tiles; O-CTA: warp 1), each a whole warp with one elected
+// lane, warp 2 TMEM allocator, warps 4-7 the math warpgroup (softmax in
 // the S-CTA, correction + epilogue in the O-CTA); thread h of the warpgroup
 // owns TMEM lane h = head h.
 //
@@ -131,8 +132,7 @@ constexpr int kEndO = kOffMsgO + kMsgSlots * kMsgStride;         // 210944
 constexpr int kOffBar = kEndS > kEndO ? kEndS : kEndO;
 constexpr int kOffSlot = kOffBar + kNumBars * 8;
 constexpr int kOffAbort = kOffSlot + 4;
-constexpr int kOffZArg = kOffAbort + 4;                          // paged zero request: {tile, tail rows, stop}
-constexpr int kOffEpi = (kOffZArg + 12 + 1023) / 1024 * 1024;    // O-CTA epilogue staging
+constexpr int kOffEpi = (kOffAbort + 4 + 1023) / 1024 * 1024;    // O-CTA epilogue staging
 constexpr int kEpiWarpBytes = 32 * 128;                          // one warp's 32 rows x 128 bytes
 constexpr int kSmemBytes = kOffEpi + 4 * kEpiWarpBytes + 1024;   // + 1024 alignment slack
 static_assert(kSmemBytes <= 232448, "dynamic shared memory limit");
@@ -394,7 +394,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             ptx::mbar_init(bar(kBarDrain + i), 1);
         }
         ptx::mbar_init(bar(kBarQReady), 1);
-        if constexpr (kPaged) reinterpret_cast<volatile int *>(smem + kOffZArg)[2] = 0;
         *abort_flag = 0;
         ptx::fence_mbarrier_init_cluster();
     }
@@ -522,227 +521,227 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             for (int k = 0; k < nslots; ++k, rg.next(nslots))
                 ptx::mbar_wait(bar(kBarEmpty + rg.slot), rg.phase ^ 1, kErrWaitEmpty);
         }
-    } else if (warp == 1 || (warp == 3 && role == 0)) {
-        // ------------------------------------------------------------ MMA issuers
-        // S-CTA: GEMM1 is issued by two threads, lane 0 of warps 1 and 3, taking
-        // alternate S tiles (and so alternate S buffers).  One thread issues an
-        // N=96 MMA every ~90 cycles in this kernel, twice the MMA's tensor time;
-        // two issuers keep the tensor pipe busy.  At the first tile of a sequence
-        // the tile's issuer copies Q into TMEM once every GEMM1 of the previous
-        // sequence (its own and the other issuer's last tile) is done, and the
-        // other issuer waits for the copy before its next tile.  Both walk the
-        // same items and ring positions, skipping the other's slots.
+    } else if (role == 0 && (warp == 1 || warp == 3)) {
+        // ------------------------------------------------------------ S-CTA: GEMM1
+        // Two warps issue, taking alternate S tiles (and so alternate S buffers): one
+        // thread issued an N=96 MMA every ~90 cycles in this kernel, twice the MMA's
+        // tensor time; two keep the tensor pipe busy.  Each runs as a whole warp with
+        // uniform control flow and one elected lane behind each instruction, so that
+        // descriptors stay in uniform registers (128 sequences, 589 000 tokens in 64-row
+        // pages: 202 us a step, 258 from a branch of lane 0; 4096 tokens, contiguous: 17.3
+        // and 17.9).  A wait that runs out does not branch off: the tile is finished on
+        // whatever the buffers hold and then given up, its slots not freed (a load may
+        // still be on its way to one).
+        // At the first tile of a sequence the tile's issuer copies Q into TMEM once every
+        // GEMM1 of the previous sequence (its own and the other issuer's last tile) is
+        // done, and the other issuer waits for the copy before its next tile.  Both walk
+        // the same items and ring positions, skipping the other's slots.
         // A wait by parity is exact only while the phase before the awaited one is
         // known to be complete, and an issuer does not wait for the other's slots: a
         // load that comes in late would let it take a slot's next use for landed.  So
         // each has its own set of barriers for the slots, and waits on the barriers
         // they share (kBarSFull, kBarQReady) only after kBarSEmpty: then the softmax
         // has read tile jt - 2, so every GEMM1 and copy of Q up to it is complete.
-        // O-CTA: lane 0 of warp 1 issues GEMM2.
-        if (lane == 0) {
-            const int nslots = role == 0 ? (kFp8 ? kSlotsS8 : kSlotsS) : (kFp8 ? kSlotsO8 : kSlotsO);
-            const uint32_t me = warp == 1 ? 0u : 1u;
-            Ring rg;
-            uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
-            uint32_t phases = 0;  // per slot: parity of this issuer's next use
-            int prev_b = -1;
-            bool ok = true;
-            auto landed = [&]() -> bool {  // (once per use: the next call is for the slot's next use)
-                const uint32_t parity = (phases >> rg.slot) & 1;
-                phases ^= 1u << rg.slot;
-                return ptx::mbar_spin(bar(kBarFull + me * kRingSlots + rg.slot), parity, kErrWaitFull);
-            };
-            ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
-            Item it;
-            int i;
-            while (ok && items_next<kSched>(wl, cur, it, i)) {
-                const bool new_seq = role == 0 && it.b != prev_b;
-                prev_b = it.b;
-                for (int t0 = 0; ok && t0 < it.len; t0 += kTS, ++jt) {
-                    if (role == 0) {
-                        const bool mine = (jt & 1u) == me;
-                        const uint32_t sb = jt & 1, use = jt >> 1;
-                        if (mine && (*abort_flag || !ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma))) { ok = false; break; }
-                        if (new_seq && t0 == 0) {
-                            ++nseq;
-                            if (mine) {
-                                if (jt > 0) {
-                                    // An MMA is not ordered before a later tcgen05.cp: every
-                                    // GEMM1 reading the old Q completes first.
-                                    ptx::mma_commit(bar(kBarQFree + me));
-                                    if (!ptx::mbar_spin(bar(kBarQFree + me), qphase, kErrWaitMma)) { ok = false; break; }
-                                    qphase ^= 1;
-                                    const uint32_t pj = jt - 1;  // the other issuer's last tile
-                                    if (!ptx::mbar_spin(bar(kBarSFull + (pj & 1)), (pj >> 1) & 1, kErrWaitMma)) { ok = false; break; }
-                                    ptx::tc_fence_after();
-                                }
-                                // Ring slots filled by TMA need no tcgen05 fence: the full
-                                // barrier's complete_tx orders the loaded bytes before the
-                                // copy / MMA reads them.  (A fence stalls this thread until
-                                // the tensor pipe drains, ~230 cycles.)
-                                for (int kb = 0; ok && kb < kKBlocks; kb += kFp8 ? 1 : 2) {
-                                    if (*abort_flag || !landed()) { ok = false; break; }
-                                    if constexpr (kFp8) {
-                                        // K-block kb of the hi and lo planes: 64 B per row, 16 columns each
-                                        const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS8;
-#pragma unroll
-                                        for (int c = 0; c < 2; ++c) {
-                                            ptx::tmem_cp_128x256b(tmem + kTmemQ + kb * 16 + c * 8,
-                                                                  ptx::sdesc_sw64(slot + c * 32, 16, 512));
-                                            ptx::tmem_cp_128x256b(tmem + kTmemQ + kTmemQLo + kb * 16 + c * 8,
-                                                                  ptx::sdesc_sw64(slot + kQBox8 + c * 32, 16, 512));
-                                        }
-                                    } else {
-                                        const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
-                                        const int nb = min(2, kKBlocks - kb);
-                                        for (int j = 0; j < nb; ++j) {
-#pragma unroll
-                                            for (int c = 0; c < 4; ++c)
-                                                ptx::tmem_cp_128x256b(tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
-                                                                      ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
-                                        }
-                                    }
-                                    ptx::mma_commit(bar(kBarEmpty + rg.slot));
-                                    rg.next(nslots);
-                                }
-                                if (!ok) break;
-                                ptx::mma_commit(bar(kBarQReady));
-                                qready_seq = nseq;
-                            } else {
-                                for (int q = 0; q < (kFp8 ? kKBlocks : kQSlots); ++q) rg.next(nslots);
-                            }
+        const uint32_t e = ptx::elect_one();
+        constexpr int nslots = kFp8 ? kSlotsS8 : kSlotsS;
+        const uint32_t me = warp == 1 ? 0u : 1u;
+        Ring rg;
+        uint32_t jt = 0, qphase = 0, nseq = 0, qready_seq = 0;
+        uint32_t phases = 0;  // per slot: parity of this issuer's next use
+        int prev_b = -1;
+        bool ok = true;
+        auto landed = [&]() {
+            ok &= ptx::mbar_spin(bar(kBarFull + me * kRingSlots + rg.slot), (phases >> rg.slot) & 1, kErrWaitFull);
+            phases ^= 1u << rg.slot;
+        };
+        ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
+        Item it;
+        int i;
+        while (ok && items_next<kSched>(wl, cur, it, i)) {
+            const int len = __shfl_sync(0xffffffffu, it.len, 0), b = __shfl_sync(0xffffffffu, it.b, 0);
+            const bool new_seq = b != prev_b;
+            prev_b = b;
+            for (int t0 = 0; t0 < len; t0 += kTS, ++jt) {
+                const bool mine = (jt & 1u) == me;
+                const uint32_t sb = jt & 1, use = jt >> 1;
+                if (mine) {
+                    ok = ok && !*abort_flag && ptx::mbar_spin(bar(kBarSEmpty + sb), (use & 1) ^ 1, kErrWaitMma);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                }
+                if (new_seq && t0 == 0) {
+                    ++nseq;
+                    if (mine) {
+                        if (jt > 0) {
+                            // An MMA is not ordered before a later tcgen05.cp: every
+                            // GEMM1 reading the old Q completes first.
+                            ptx::mma_commit_if(e, bar(kBarQFree + me));
+                            ok = ptx::mbar_spin(bar(kBarQFree + me), qphase, kErrWaitMma);
+                            qphase ^= 1;
+                            const uint32_t pj = jt - 1;  // the other issuer's last tile
+                            ok = ok && ptx::mbar_spin(bar(kBarSFull + (pj & 1)), (pj >> 1) & 1, kErrWaitMma);
+                            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                            ptx::tc_fence_after();
                         }
-                        if (!mine) {
-                            for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(nslots);
-                            continue;
-                        }
-                        if (qready_seq != nseq) {  // the other issuer copied this sequence's Q
-                            if (!ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma)) { ok = false; break; }
-                            qready_seq = nseq;
-                        }
-                        ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
-                        const uint32_t d = tmem + kTmemS + sb * kTS;
-                        for (int sl = 0; sl < kSlotsPerTile; ++sl) {
-                            if (!landed()) { ok = false; break; }
-                            // descriptor of the slot, plus compile-time offsets per K-step: a
-                            // short issue sequence between MMAs
-                            const uint32_t acc0 = sl > 0 ? 1u : 0u;
+                        // Ring slots filled by TMA need no tcgen05 fence: the full
+                        // barrier's complete_tx orders the loaded bytes before the
+                        // copy / MMA reads them.  (A fence stalls the issuer until
+                        // the tensor pipe drains, ~230 cycles.)
+                        for (int kb = 0; kb < kKBlocks; kb += kFp8 ? 1 : 2) {
+                            landed();
                             if constexpr (kFp8) {
-                                // K-block j, K-step ks (32 e4m3): S += Q8hi.C8 + Q8lo.C8
-                                const uint64_t b0 = ptx::sdesc_sw64(sbase + kOffRing + rg.slot * kSlotS8, 16, 512);
-                                const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 16);
+                                // K-block kb of the hi and lo planes: 64 B per row, 16 columns each
+                                const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS8;
 #pragma unroll
-                                for (int k = 0; k < kKbPerSlot * 2; ++k) {
-                                    const uint64_t bk = b0 + (uint64_t)(((k >> 1) * kBoxS8 + (k & 1) * 32) >> 4);
-                                    const uint32_t ak = a0 + (k >> 1) * 16 + (k & 1) * 8;
-                                    ptx::mma_ts_f8(d, ak, bk, idesc_s8(), k > 0 ? 1u : acc0);
-                                    ptx::mma_ts_f8(d, ak + kTmemQLo, bk, idesc_s8(), 1u);
+                                for (int c = 0; c < 2; ++c) {
+                                    ptx::tmem_cp_128x256b_if(e, tmem + kTmemQ + kb * 16 + c * 8,
+                                                             ptx::sdesc_sw64(slot + c * 32, 16, 512));
+                                    ptx::tmem_cp_128x256b_if(e, tmem + kTmemQ + kTmemQLo + kb * 16 + c * 8,
+                                                             ptx::sdesc_sw64(slot + kQBox8 + c * 32, 16, 512));
                                 }
                             } else {
-                                // (paged slots interleave the K-blocks per 8-row group: stride 3 KB)
-                                const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kPaged ? kKbPerSlot * 1024 : 1024);
-                                const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 32);
-                                constexpr int kKbStride = kPaged ? 1024 : kBoxS;
+                                const uint32_t slot = sbase + kOffRing + rg.slot * kSlotS;
+                                const int nb = min(2, kKBlocks - kb);
+                                for (int j = 0; j < nb; ++j) {
 #pragma unroll
-                                for (int k = 0; k < kKbPerSlot * 4; ++k)
-                                    ptx::mma_ts(d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * kKbStride + (k & 3) * 32) >> 4),
-                                                idesc_s<kBf16>(), k > 0 ? 1u : acc0);
+                                    for (int c = 0; c < 4; ++c)
+                                        ptx::tmem_cp_128x256b_if(e, tmem + kTmemQ + ((kb + j) * 4 + c) * 8,
+                                                                 ptx::sdesc_sw128(slot + j * kQBoxBytes + c * 32, 16, 1024));
+                                }
                             }
-                            ptx::mma_commit(bar(kBarEmpty + rg.slot));
+                            ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
                             rg.next(nslots);
                         }
-                        if (!ok) break;
-                        ptx::mma_commit(bar(kBarSFull + sb));
+                        ptx::mma_commit_if(e, bar(kBarQReady));
+                        qready_seq = nseq;
                     } else {
-                        const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
-                        if (*abort_flag || !ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer) ||
-                            !ptx::mbar_spin(bar(kBarCorr + ms), mu & 1, kErrWaitMma)) { ok = false; break; }
-                        const int nct = (min(kTS, it.len - t0) + kTO - 1) / kTO;
-                        // the correction's TMEM stores to O (and fp8: the e4m3 P planes the
-                        // warpgroup wrote) come first
-                        ptx::tc_fence_after();
-                        const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsgO + ms * kMsgStride, 16, 512);
-                        for (int ct = 0; ct < nct; ++ct) {
-                            if (!landed()) { ok = false; break; }
-                            if constexpr (kPaged) {
-                                // an item's last tile ending inside a 32-row piece: the rows past
-                                // its end are zeroed by the whole warp (the other lanes wait at
-                                // __syncwarp meanwhile).  Items split sequences on 96-token tile
-                                // boundaries, so this is a sequence's end; elsewhere it would
-                                // only zero rows whose P is 0.
-                                const int tail = (it.len - t0) % kTO;
-                                if (ct == nct - 1 && t0 + kTS >= it.len && tail != 0) {
-                                    volatile int *za = reinterpret_cast<volatile int *>(smem + kOffZArg);
-                                    const uint32_t tile = sbase + kOffRing + rg.slot * kSlotO;
-                                    za[0] = (int)tile;
-                                    za[1] = tail;
-                                    __syncwarp();
-                                    zero_tail(tile, tail, 0);
-                                    __syncwarp();
-                                    ptx::tc_fence_after();
-                                }
-                            }
-                            const uint32_t acc0 = (t0 > 0 || ct > 0) ? 1u : 0u;
-                            if constexpr (kFp8) {
-                                // O += P8hi.C8 + P8lo.C8 (K = 32 tokens); C8_N MN-major: 128-column
-                                // groups 4 KB apart (LBO), 8-row groups 1 KB apart (SBO)
-                                const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO8, 4096, 1024);
-                                const uint32_t pm = sbase + kOffMsgO + ms * kMsgStride + ct * 4096;
-#pragma unroll
-                                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                                    for (int nh = 0; nh < 2; ++nh)
-                                        ptx::mma_ss_f8(tmem + nh * 256, ptx::sdesc_sw32(pm + x * kPlaneP8, 16, 256),
-                                                       c0 + (uint64_t)((nh * 2 * 4096) >> 4), idesc_o<false>(),
-                                                       x > 0 ? 1u : acc0);
-                            } else {
-                                const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO, kBoxO, 1024);
-                                const uint64_t pa = p0 + (uint64_t)(ct * (kSubP >> 4));
-#pragma unroll
-                                for (int kk = 0; kk < kTO / 16; ++kk) {
-#pragma unroll
-                                    for (int nh = 0; nh < 2; ++nh)
-                                        ptx::mma_ss(tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
-                                                    c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), idesc_o<kBf16>(),
-                                                    kk > 0 ? 1u : acc0);
-                                }
-                            }
-                            ptx::mma_commit(bar(kBarEmpty + rg.slot));
-                            rg.next(nslots);
-                        }
-                        if (!ok) break;
-                        // (in this order: once a message has come through a freed slot, the
-                        // slot's last kBarMmaDone phase is known to be complete)
-                        ptx::mma_commit(bar(kBarMmaDone + ms));
-                        ptx::mma_commit_mc(bar(kBarPFree + ms), 0x3);
+                        for (int q = 0; q < (kFp8 ? kKBlocks : kQSlots); ++q) rg.next(nslots);
                     }
                 }
-            }
-            if (!ok) *abort_flag = 1;
-            if constexpr (kPaged) {
-                if (role == 1) {  // release the helper lanes (every path out of the loop gets here)
-                    reinterpret_cast<volatile int *>(smem + kOffZArg)[2] = 1;
-                    __syncwarp();
+                if (!mine) {
+                    for (int sl = 0; sl < kSlotsPerTile; ++sl) rg.next(nslots);
+                    continue;
                 }
-            }
-            // every MMA this thread issued has retired before TMEM is freed
-            ptx::mma_commit(bar(kBarDrain + me));
-            ptx::mbar_wait(bar(kBarDrain + me), 0, kErrWaitMma);
-        } else if (kPaged && role == 1) {
-            // O-CTA, paged: lanes 1-31 of the GEMM2 warp.  Rows of a sequence's
-            // last C tile past its end hold whatever the page held, not
-            // necessarily finite numbers; P is 0 there, but 0 x NaN is NaN in
-            // GEMM2.  The issuing lane posts such a tile (landed) and these lanes
-            // zero its tail with it.  Between requests they wait inside
-            // __syncwarp, issuing nothing.
-            volatile int *za = reinterpret_cast<volatile int *>(smem + kOffZArg);
-            for (;;) {
-                __syncwarp();
-                if (za[2] != 0) break;
-                zero_tail((uint32_t)za[0], za[1], lane);
-                __syncwarp();
+                if (qready_seq != nseq) {  // the other issuer copied this sequence's Q
+                    ok &= ptx::mbar_spin(bar(kBarQReady), (nseq - 1) & 1, kErrWaitMma);
+                    qready_seq = nseq;
+                }
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ptx::tc_fence_after();  // the softmax's loads of this S buffer (and Q's copy) come first
+                const uint32_t d = tmem + kTmemS + sb * kTS;
+                for (int sl = 0; sl < kSlotsPerTile; ++sl) {
+                    landed();
+                    // descriptor of the slot, plus compile-time offsets per K-step: a
+                    // short issue sequence between MMAs
+                    const uint32_t acc0 = sl > 0 ? 1u : 0u;
+                    if constexpr (kFp8) {
+                        // K-block j, K-step ks (32 e4m3): S += Q8hi.C8 + Q8lo.C8
+                        const uint64_t b0 = ptx::sdesc_sw64(sbase + kOffRing + rg.slot * kSlotS8, 16, 512);
+                        const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 16);
+#pragma unroll
+                        for (int k = 0; k < kKbPerSlot * 2; ++k) {
+                            const uint64_t bk = b0 + (uint64_t)(((k >> 1) * kBoxS8 + (k & 1) * 32) >> 4);
+                            const uint32_t ak = a0 + (k >> 1) * 16 + (k & 1) * 8;
+                            ptx::mma_ts_f8_if(e, d, ak, bk, idesc_s8(), k > 0 ? 1u : acc0);
+                            ptx::mma_ts_f8_if(e, d, ak + kTmemQLo, bk, idesc_s8(), 1u);
+                        }
+                    } else {
+                        // (paged slots interleave the K-blocks per 8-row group: stride 3 KB)
+                        const uint64_t b0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotS, 16, kPaged ? kKbPerSlot * 1024 : 1024);
+                        const uint32_t a0 = tmem + kTmemQ + sl * (kKbPerSlot * 32);
+                        constexpr int kKbStride = kPaged ? 1024 : kBoxS;
+#pragma unroll
+                        for (int k = 0; k < kKbPerSlot * 4; ++k)
+                            ptx::mma_ts_if(e, d, a0 + k * 8, b0 + (uint64_t)(((k >> 2) * kKbStride + (k & 3) * 32) >> 4),
+                                           idesc_s<kBf16>(), k > 0 ? 1u : acc0);
+                    }
+                    ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
+                    rg.next(nslots);
+                }
+                ptx::mma_commit_if(e, bar(kBarSFull + sb));
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             }
         }
+        if (!ok) *abort_flag = 1;
+        // every MMA this warp issued has retired before TMEM is freed
+        ptx::mma_commit_if(e, bar(kBarDrain + me));
+        ptx::mbar_wait(bar(kBarDrain + me), 0, kErrWaitMma);
+    } else if (role == 1 && warp == 1) {
+        // ------------------------------------------------------------ O-CTA: GEMM2
+        // (a whole warp with one elected lane, as GEMM1's issuers)
+        const uint32_t e = ptx::elect_one();
+        constexpr int nslots = kFp8 ? kSlotsO8 : kSlotsO;
+        Ring rg;
+        uint32_t jt = 0;
+        bool ok = true;
+        ItemCursor cur = items_begin<kSched>(wl, cid, ncl);
+        Item it;
+        int i;
+        while (ok && items_next<kSched>(wl, cur, it, i)) {
+            const int len = __shfl_sync(0xffffffffu, it.len, 0);
+            for (int t0 = 0; t0 < len; t0 += kTS, ++jt) {
+                const uint32_t ms = jt % kMsgSlots, mu = jt / kMsgSlots;
+                ok = !*abort_flag && ptx::mbar_wait<true>(bar(kBarPFull + ms), mu & 1, kErrWaitPeer);
+                ok = ok && ptx::mbar_spin(bar(kBarCorr + ms), mu & 1, kErrWaitMma);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                const int nct = (min(kTS, len - t0) + kTO - 1) / kTO;
+                // the correction's TMEM stores to O (and fp8: the e4m3 P planes the
+                // warpgroup wrote) come first
+                ptx::tc_fence_after();
+                const uint64_t p0 = ptx::sdesc_sw64(sbase + kOffMsgO + ms * kMsgStride, 16, 512);
+                for (int ct = 0; ct < nct; ++ct) {
+                    ok &= ptx::mbar_spin(bar(kBarFull + rg.slot), rg.phase, kErrWaitFull);
+                    if constexpr (kPaged) {
+                        // Rows of a sequence's last C tile past its end hold whatever the
+                        // page held, not necessarily finite numbers; P is 0 there, but 0 x
+                        // NaN is NaN, so they are zeroed first.  (Items split sequences on
+                        // 96-token tile boundaries, so an item that ends inside a 32-row
+                        // piece ends its sequence; elsewhere this would only zero rows
+                        // whose P is 0.)
+                        const int tail = (len - t0) % kTO;
+                        if (ct == nct - 1 && t0 + kTS >= len && tail != 0) {
+                            zero_tail(sbase + kOffRing + rg.slot * kSlotO, tail, lane);
+                            __syncwarp();
+                        }
+                    }
+                    const uint32_t acc0 = (t0 > 0 || ct > 0) ? 1u : 0u;
+                    if constexpr (kFp8) {
+                        // O += P8hi.C8 + P8lo.C8 (K = 32 tokens); C8_N MN-major: 128-column
+                        // groups 4 KB apart (LBO), 8-row groups 1 KB apart (SBO)
+                        const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO8, 4096, 1024);
+                        const uint32_t pm = sbase + kOffMsgO + ms * kMsgStride + ct * 4096;
+#pragma unroll
+                        for (int x = 0; x < 2; ++x)
+#pragma unroll
+                            for (int nh = 0; nh < 2; ++nh)
+                                ptx::mma_ss_f8_if(e, tmem + nh * 256, ptx::sdesc_sw32(pm + x * kPlaneP8, 16, 256),
+                                                  c0 + (uint64_t)((nh * 2 * 4096) >> 4), idesc_o<false>(),
+                                                  x > 0 ? 1u : acc0);
+                    } else {
+                        const uint64_t c0 = ptx::sdesc_sw128(sbase + kOffRing + rg.slot * kSlotO, kBoxO, 1024);
+                        const uint64_t pa = p0 + (uint64_t)(ct * (kSubP >> 4));
+#pragma unroll
+                        for (int kk = 0; kk < kTO / 16; ++kk) {
+#pragma unroll
+                            for (int nh = 0; nh < 2; ++nh)
+                                ptx::mma_ss_if(e, tmem + nh * 256, pa + (uint64_t)((kk * 32) >> 4),
+                                               c0 + (uint64_t)((nh * 4 * kBoxO + kk * 16 * 128) >> 4), idesc_o<kBf16>(),
+                                               kk > 0 ? 1u : acc0);
+                        }
+                    }
+                    ptx::mma_commit_if(ok ? e : 0u, bar(kBarEmpty + rg.slot));
+                    rg.next(nslots);
+                }
+                // (in this order: once a message has come through a freed slot, the slot's
+                // last kBarMmaDone phase is known to be complete)
+                ptx::mma_commit_if(e, bar(kBarMmaDone + ms));
+                ptx::mma_commit_mc_if(e, bar(kBarPFree + ms), 0x3);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            }
+        }
+        if (!ok) *abort_flag = 1;
+        // every MMA this warp issued has retired before TMEM is freed
+        ptx::mma_commit_if(e, bar(kBarDrain));
+        ptx::mbar_wait(bar(kBarDrain), 0, kErrWaitMma);
     } else if (warp >= 4) {
         // ------------------------------------------------------------ math warpgroup
         const int h = tid - 128;                              // head row = TMEM lane
@@ -1065,8 +1064,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
 
     // ---------------------------------------------------------------- teardown
-    // (lane 0 of the producer and MMA warps arrives after its role loop: the
-    // warp reconverges before the CTA and cluster barriers, which are .aligned)
+    // (lane 0 of the producer warp arrives after its role loop: the warp
+    // reconverges before the CTA and cluster barriers, which are .aligned)
     ptx::tc_fence_before();
     __syncwarp();
     __syncthreads();

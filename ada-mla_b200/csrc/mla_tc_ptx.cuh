@@ -387,58 +387,11 @@ __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_
         : "memory");
 }
 
-// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16, fp32 accumulate.
-// Shared memory -> TMEM copy of a 128-row x 32-byte matrix (row r to lane r,
-// the 32 bytes to 8 consecutive columns), read through a matrix descriptor
-// like an MMA operand.  A later tcgen05.mma of this thread is ordered after it.
-__device__ __forceinline__ void tmem_cp_128x256b(uint32_t d_tmem, uint64_t s_desc) {
-    asm volatile("tcgen05.cp.cta_group::1.128x256b [%0], %1;" ::"r"(d_tmem), "l"(s_desc) : "memory");
-}
-
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f8f6f4 (A, B e4m3 per the
-// instruction descriptor), K = 32, fp32 accumulate.
-__device__ __forceinline__ void mma_ts_f8(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
-// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f8f6f4, K = 32, fp32 accumulate.
-__device__ __forceinline__ void mma_ss_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
-
 // Arrive on a local mbarrier once all prior tcgen05 async ops of this thread finish.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                      bar)
                  : "memory");
-}
-
-// Same, arriving on the barrier at this smem offset in every CTA of `mask`.
-__device__ __forceinline__ void mma_commit_mc(uint32_t bar, uint16_t mask) {
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 "
-        "[%0], %1;" ::"r"(bar),
-        "h"(mask)
-        : "memory");
 }
 
 // The same behind a predicate, for whole warps with one elected lane (lane_on != 0 in
@@ -453,6 +406,7 @@ __device__ __forceinline__ void mma_ss_if(uint32_t lane_on, uint32_t d_tmem, uin
         : "memory");
 }
 
+// D[tmem] (+)= A[tmem] * B[smem desc]^T, kind::f16, fp32 accumulate.
 __device__ __forceinline__ void mma_ts_if(uint32_t lane_on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
                                           uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -462,6 +416,28 @@ __device__ __forceinline__ void mma_ts_if(uint32_t lane_on, uint32_t d_tmem, uin
         : "memory");
 }
 
+// kind::f8f6f4 (A, B e4m3 per the instruction descriptor), K = 32, fp32 accumulate.
+__device__ __forceinline__ void mma_ts_f8_if(uint32_t lane_on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lane_on)
+        : "memory");
+}
+
+__device__ __forceinline__ void mma_ss_f8_if(uint32_t lane_on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                             uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(lane_on)
+        : "memory");
+}
+
+// Shared memory -> TMEM copy of a 128-row x 32-byte matrix (row r to lane r,
+// the 32 bytes to 8 consecutive columns), read through a matrix descriptor
+// like an MMA operand.  A later tcgen05.mma of this thread is ordered after it.
 __device__ __forceinline__ void tmem_cp_128x256b_if(uint32_t lane_on, uint32_t d_tmem, uint64_t s_desc) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.128x256b [%0], %1;\n\t}" ::"r"(
@@ -478,6 +454,7 @@ __device__ __forceinline__ void mma_commit_if(uint32_t lane_on, uint32_t bar) {
         : "memory");
 }
 
+// Arrives on the barrier at this smem offset in every CTA of `mask`.
 __device__ __forceinline__ void mma_commit_mc_if(uint32_t lane_on, uint32_t bar, uint16_t mask) {
     asm volatile(
         "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
