@@ -264,3 +264,9 @@ def test_dense_single_rows_of_longer_sequences(dtype):
         ada_mla.mla_prefill(qd[:, -2:], kvd[..., :128], rd, kvd[..., 128:])
     with pytest.raises(RuntimeError):
         ada_mla.mla_prefill(qd[:, -1:], kvd[:, 1:, :, :128], rd[:, 1:], kvd[:, 1:, :, 128:])
+
+
+def test_a_long_prompt():
+    """Up to 133 key tiles an item."""
+    check([16500], [16500], 2, torch.bfloat16, seed=22)
+    check([700, 9000], [17000, 9001], 1, torch.float16, seed=23)

@@ -348,3 +348,20 @@ def test_many_row_tiles(batch, k, heads):
     a, la = check(q, pool, table, n, mask, want=want)
     b, lb = check(q, pool, table, n, mask, want=want)
     assert torch.equal(a, b) and torch.equal(la, lb)
+
+
+def test_a_pool_past_32_bits_of_elements():
+    """Pages whose elements and bytes lie beyond 2^31 and 2^32 of the pool's start."""
+    rows = 4_200_000 // 64
+    q, pool, table, n = problem(2, 5, 16, [500, 130], 64, torch.float16, seed=70)
+    want = expect(q, pool, table, n, None, torch.float16)
+    big = torch.empty(rows, 64, 576, dtype=torch.float16, device="cuda")
+    first = rows - pool.shape[0]
+    big[first:] = pool.cuda()
+    at = torch.where(table >= 0, table + first, table)
+    import ada_mla
+
+    got, lse = ada_mla.mla_decode_tree(q.cuda(), big, at.cuda(), n.cuda(), max_seq_len=500, softmax_scale=SCALE, return_lse=True)
+    assert bool(((got.double().cpu() - want[0]).abs() <= want[2]).all())
+    assert bool(((lse.double().cpu() - want[1]).abs() <= LSE_TOL).all())
+    assert ada_mla.mla_get_device_error() == 0
