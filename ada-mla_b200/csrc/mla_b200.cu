@@ -834,12 +834,13 @@ TreeItems tree_items(int tiles, int longest, int num_splits, int clusters) {
 
 template <typename OutT>
 void launch_tree_merge(const tree::TreeParams &p, cudaStream_t stream, bool chain) {
-    // Few rows have many splits each: 8 warps per 32 rows and piece (1 tile of 128 rows: the
-    // call takes 21.7 us, 33.4 with one warp).  From 512 warps on, one is enough (4 tiles of
-    // 128 rows: 152 us, 156 with 8; 64 tiles of 112 rows: 99 us, 124 with 8).
+    // Few rows have many splits each: 8 warps per 32 rows and piece (calls with 8 and with one,
+    // us: 1 tile of 128 rows 22.9 and 40.8; tiles of 112 rows over up to 8192 tokens, 4 of
+    // them 33 and 47, 8 38 and 40).  Above 1024 warps one is enough (16 tiles 53 and 44, 64
+    // tiles 131 and 109).
     const dim3 block(32 * tree::kMergeWarps);
     const unsigned groups = (unsigned)cdiv(p.num_heads, 32), tiles = (unsigned)p.wl.batch, pieces = kDV / 16;
-    if (tiles * groups * pieces < 512)
+    if (tiles * groups * pieces <= 1024)
         launch_dependent(tree::merge_kernel<OutT, tree::kMergeWarps>, dim3(groups * pieces, tiles), block, 0, stream,
                          chain, p);
     else
@@ -928,9 +929,10 @@ int decode_tree(const void *query, const void *kv_pages, const int32_t *block_ta
     p.tiles = tt.tiles;
     p.tile_drafts = tt.tile_drafts;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // a few tiles chain decode -> merge -> next decode (see run_split_decode; all chained:
-    // 64 tiles 104 -> 102.5 us, 96 tiles 148 -> 155)
-    const bool chain = tiles < 8;
+    // Up to 64 tiles chain decode -> merge -> next decode (see run_split_decode; calls chained
+    // and not, us: 1 tile 22.9 and 26.7, 16 tiles 44 and 47.5, 31 tiles 59.6 and 63.6, 64
+    // tiles of 512 tokens 50.5 and 53.6, of up to 8192 tokens 110 and 109; 96 tiles 151 and 142)
+    const bool chain = tiles <= 64;
     p.chain = chain ? 1 : 0;
     if (empty) {
         wl.cost_off = nullptr;  // no items: the merge of nothing

@@ -123,8 +123,8 @@ constexpr int kOffMax = (kOffAbort + 4 + 15) / 16 * 16;     // S-CTA: row maxima
 // The plan of up to kPlanMax row tiles, made by every CTA for itself: offsets of the
 // tiles' sequences on a virtual packed axis, places on the cost line, drafts seen.
 constexpr int kPlanMax = 960;
-// Up to here every warp makes it (plan_few): 1 tile of 43 S tiles, 21.9 us against 22.7;
-// with 64 tiles 103.7 against 102.1.
+// Up to here every warp makes it (plan_few): 1 tile of 43 S tiles, 22.9 us against 24.2; 31
+// tiles 63.8 against 65.4; with 64 tiles there is no difference.
 constexpr int kPlanFew = 31;
 constexpr int kOffSeen = kOffMax + 2 * 2 * 128 * 4;
 constexpr int kOffCu = kOffSeen + kPlanMax * 8;

@@ -253,9 +253,9 @@ def test_calls_back_to_back():
     assert ada_mla.mla_get_device_error() == 0
 
 
-@pytest.mark.parametrize("batch,k,heads,n", [(1, 8, 16, 1500), (2, 7, 16, 700), (1, 12, 128, 900), (7, 3, 16, 400)])
+@pytest.mark.parametrize("batch,k,heads,n", [(1, 8, 16, 1500), (2, 7, 16, 700), (1, 12, 128, 900), (7, 3, 16, 400), (40, 7, 16, 1700)])
 def test_chained_calls_back_to_back(batch, k, heads, n):
-    """Up to 7 row tiles decode, merge and next decode are chained: a merge is resident while
+    """Few row tiles' decode, merge and next decode are chained: a merge is resident while
     its decode writes.  Calls on inputs in turn give each input's own bits."""
     import ada_mla
 
