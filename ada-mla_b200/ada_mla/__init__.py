@@ -209,7 +209,7 @@ def mla_decode_tree(query, kv_pages, block_table, seq_lens, tree_mask=None, max_
                  draft i's entry is set where i sees draft j (``ada_mla.tree_mask``
                  makes it from parents).  None: a chain, draft i sees drafts 0..i.
     Every draft sees the whole context before the drafts.  A draft's row that no draft
-    sees (a padded draft) may hold anything; a query that sees nothing gives zeros and
+    sees (a padded draft) may hold anything, all other rows are finite; a query that sees nothing gives zeros and
     an LSE of -inf.  Returns O* [B, k, n_h, 512] (input dtype, or fp32 with
     ``out_dtype=torch.float32``) and, with ``return_lse``, the natural-log LSE
     [B, k, n_h] fp32.  Pass ``max_seq_len`` to avoid a device->host read.
@@ -267,7 +267,9 @@ def mla_cache_write(latent, slots, cache, norm_weight=None, eps: float = 1e-6, p
                  their sines): rotates the rope columns, pairs (2i, 2i + 1), or
                  (i, i + 32) with ``interleaved=False``; None: stored as they are.
     kv_scales    fp32, one per cache row, written in place: with an e4m3 cache, row =
-                 cache * scale (what ``mla_decode_batched`` takes as ``kv_scale``).
+                 cache * scale (what ``mla_decode_batched`` takes as ``kv_scale``; the
+                 paged decodes read fp16 and bf16 pools only).
+    Slots are distinct: two rows with one slot leave a mixture of both.
     """
     _ext.mla_cache_write(latent, slots, cache, norm_weight, float(eps), positions, cos_sin,
                          bool(interleaved), kv_scales)
@@ -293,8 +295,9 @@ def mla_prefill(query, k_nope, k_rope, v, cu_seqlens_q=None, cu_seqlens_k=None, 
     causal       query i of a sequence sees keys 0 .. i + Lk - Lq: its queries are its
                  last Lq tokens, so a chunk of a prompt sees all that came before.
     Returns [.., n_h, 128] in the inputs' dtype and, with ``return_lse``, the
-    natural-log LSE [.., n_h] fp32 (for merging with attention over other keys).  A
-    query that sees no key gives zeros and -inf.  The form for single tokens is the
+    natural-log LSE [.., n_h] fp32 (for merging with attention over other keys).
+    Values have to be finite also where a query does not see them.  A query that sees no
+    key gives zeros and -inf.  The form for single tokens is the
     decode over the latent cache (``mla_decode_paged``, ``absorbed``).
     """
     out, lse = _ext.mla_prefill(query, k_nope, k_rope, v, cu_seqlens_q, cu_seqlens_k, int(max_seq_len_q),

@@ -310,8 +310,8 @@ __device__ void lens_to_offsets(const int32_t *lens, int batch, int max_len, int
     __syncthreads();
 }
 
-// Draft trees: seen[v] = the drafts that some draft of row tile v sees (tc_decode_kernel,
-// TcTreeParams); mask null: a chain, draft i sees drafts 0..i.  `tiles` row tiles share
+// Draft trees: seen[v] = the drafts that some draft of row tile v sees (TreeParams in
+// mla_tree.cuh); mask null: a chain, draft i sees drafts 0..i.  `tiles` row tiles share
 // a sequence; tiles 0: no trees.
 struct TreePlan {
     const unsigned long long *mask;

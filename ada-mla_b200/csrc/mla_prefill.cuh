@@ -29,10 +29,15 @@
 // shuffles).  The softmax warps rescale O themselves, rarely: the running maximum is
 // only raised when it grew by more than 2^8.  Every wait is bounded.
 //
-// 2048 queries over 8192 keys, 128 heads: 1155-1200 us, 1.00-1.04 PFLOP/s (the GPU's power
-// cap holds the clock near 1.5 GHz); six prompts of 262-1884 tokens, 128 heads: 570-590 us,
-// 0.62 PFLOP/s, where an item's start and end (11 key tiles long on average) cost a quarter;
-// 77 queries, 128 heads: 10.3 us.
+// A call among others on inputs that change: 2048 queries over 8192 keys, 128 heads: 1177
+// us, 1.02 PFLOP/s; six prompts of 262-1884 tokens, 128 heads: 597 us, 0.60 PFLOP/s, where
+// an item's start and end (11 key tiles long on average) cost a quarter; 77 queries, 128
+// heads: 10.3 us.  In a loop the power cap (990 W) holds the clock at 1575-1600 MHz of 1965.
+// That is not all: also in one launch alone (1.05 ms) the tensor pipe is active 59 % of the
+// cycles, as a tile's S waits for the last PV and its P for the softmax.
+//
+// A key's values reach the products of all queries of its tile pair, with weight 0 where the
+// mask hides it: they have to be finite.  (What lies past a sequence's end may be anything.)
 #pragma once
 
 #include "mla_combine.cuh"

@@ -42,13 +42,16 @@
 // zeroing (O-CTA), warps 4-11 math: thread h of each warpgroup owns row h.  Every wait
 // is bounded.
 //
-// A call, with its merge: 64 sequences of 1024-8192 tokens x 112 rows (356 MB of rows)
-// 99-104 us, 3.5 TB/s and 0.7 PFLOP/s at once; 8 x 1536 rows 143-150 us, 0.95 PFLOP/s; 512
-// rows over 131072 tokens 152-156 us, 0.95 PFLOP/s; 128 rows over 4104 tokens 21.7 us, one
-// tile through the pair after the other.  Bound by
-// shared memory: an S tile's rows are written and read once on either SM (220 KB) and its
-// weights as well (50 KB), 2110 cycles at 128 bytes a cycle; 2550 are measured, GEMM1 alone
-// needs 1728.  An item's epilogue takes 3 us: 128 KB of partials leave one SM.
+// A call among others, with its merge, on inputs that change (a loop of such calls runs at
+// the power cap, the larger ones near 1.5 GHz): 64 sequences of 1024-8192 tokens x 112 rows
+// (356 MB of rows) 121 us, 2.9 TB/s and 0.6 PFLOP/s at once; 8 x 1536 rows 154 us, 0.89
+// PFLOP/s; 512 rows over 131072 tokens 178 us, 0.82 PFLOP/s; 128 rows over 4104 tokens 23 us,
+// one tile through the pair after the other.  The loop is bound by shared memory: an S
+// tile's rows are written and read once on either SM (220 KB) and its weights as well (50
+// KB), 2110 cycles at 128 bytes a cycle; 2550-2900 are measured, GEMM1 alone needs 1728.
+// Over a whole launch there are 2950 cycles an S tile in long items (131072 tokens), 3270
+// with 8 x 1536 rows and 3900 with 64 x 112, two items a cluster: what an item's start (Q,
+// first tile) and end (its partial leaves one SM) add to the loop.
 #pragma once
 
 #include "mla_combine.cuh"

@@ -256,7 +256,7 @@ MLA_B200_API int mla_b200_decode_mtp_bf16(const void *query, const void *cache,
  * and past num_drafts are ignored).  shared_mask != 0: one tree for all sequences,
  * tree_mask [num_drafts].  tree_mask NULL: a chain, draft i sees drafts 0..i.  A
  * draft row that no draft sees may hold any bits (padded drafts); one that some
- * draft sees is a number.  A query that sees no row at all: O = 0 and LSE = -inf.
+ * draft sees, and every row before the drafts, is finite.  A query that sees no row at all: O = 0 and LSE = -inf.
  * Sequences shorter than num_drafts have only their last drafts' rows.
  * num_drafts <= 64, num_heads <= 128.  The drafts fill tiles of 128 / num_heads
  * whole drafts, and each tile is one pass over the cache.  out [batch, num_drafts,
@@ -375,8 +375,9 @@ MLA_B200_API int mla_b200_decode_split_f16_noalloc(const void *query, const void
  * [batch + 1]; q and k alike or both NULL: dense, total = batch * max_seq_len).
  * Lengths above max_seq_len_q / _k are cut to them.  causal != 0: query i of a
  * sequence with Lq queries and Lk keys sees keys 0 .. i + Lk - Lq (the queries are the
- * last Lq tokens: a chunk of a prompt sees what came before it).  Rows that see no
- * key: out 0 and LSE -inf.  out [total_q, num_heads, 128] in the inputs' type, 32-byte
+ * last Lq tokens: a chunk of a prompt sees what came before it).  v is finite, also
+ * where a query does not see it (queries up to 255 tokens earlier share its tiles);
+ * what lies past a sequence's last key may hold any bits.  Rows that see no key: out 0 and LSE -inf.  out [total_q, num_heads, 128] in the inputs' type, 32-byte
  * aligned; out_lse [total_q, num_heads] fp32 natural log, or NULL.  Rows of query
  * outside every sequence are not written.  Few queries over many keys are split over
  * the keys and joined.  Workspace, 32-byte aligned: mla_b200_workspace_size_prefill. */
@@ -435,10 +436,11 @@ MLA_B200_API int mla_b200_build_slots(const int32_t *seq_lens, const int32_t *ne
  * (2i, 2i + 1) when interleaved, else (i, i + 32).  Row t goes to cache row slots[t]
  * of cache [cache_rows, 576] (a page pool is its rows): F16, BF16, or E4M3 with
  * kv_scales [cache_rows] fp32, where the row's scale (largest value / 448, at least
- * the smallest normal number; 1 for zeros) is kept and the row stored divided by it
- * (what mla_b200_decode_batched_fp8_scaled reads).  A row whose slot is outside
+ * the smallest normal number; 1 for zeros) is kept and the row stored times 1 / scale
+ * (what mla_b200_decode_batched_fp8_scaled reads; the paged decodes read F16 and BF16
+ * pools only).  A row whose slot is outside
  * [0, cache_rows) or whose position is outside [0, max_positions) is not written.
- * Two rows with one slot leave either.  cache is 16-byte aligned. */
+ * Two rows with one slot leave a mixture of both.  cache is 16-byte aligned. */
 MLA_B200_API int mla_b200_cache_write(const void *latent, int latent_dtype, long long latent_stride,
                                       const int64_t *slots, int num_tokens, const void *norm_weight,
                                       float eps, const int32_t *positions, const float *cos_sin,
